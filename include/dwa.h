@@ -66,6 +66,7 @@ extern "C" {
 #define DWA_STATUS_BAD_LIST        0x4u  /* list offsets not monotone / out of range   */
 #define DWA_STATUS_LIST_OVERFLOW   0x8u  /* a probed list longer than max_list         */
 #define DWA_STATUS_FEW_CANDIDATES  0x10u /* fewer candidates than k (tail padded, a=0)  */
+#define DWA_STATUS_BAD_TOKEN       0x20u /* a teacher's index >= V, or twice in one row */
 
 /* Shape of one assembly call.  h_A is [B,T,d_A], pool rows are [.., D] with the
  * reference layout [U (d_B x r) | V (r x d_A) | b (d_B) | pad]
@@ -112,7 +113,8 @@ DWA_API void dwa_launch_counters(uint64_t* total, uint64_t* tensor_core_gemms, u
  * "gemm_Q", "colsum", "finalize", "bias_grad", "seq_mean", "merge",
  * "key_cache", "centroid_ema", "rmsnorm_fwd", "rmsnorm_bwd", "scatter_sort",
  * "scatter_add", "grad_send", "gather_rows", "peer_allgather", "key_grad", "sel_grad",
- * "aux_query", "aux_norm", the decode kernels ("factored_hv", "factored_out",
+ * "aux_query", "aux_norm", "top_logits", "distill_fwd", "distill_bwd",
+ * "sample", the decode kernels ("factored_hv", "factored_out",
  * "factored_combine", "base_rows", "cast_w_base", "gemm_base") and
  * "probe_lists"; up to 64 entries.  Passing NULL events removes the entry;
  * dwa_profile_clear() removes all. */
@@ -569,6 +571,101 @@ DWA_API int dwa_retrieve_noalloc(void* stream, const DwaRetrieveDims* dims, int 
  * `clear` is non-zero; DWA_ERR_DEVICE when a bit is set.  No counterpart in the
  * reference (companion of dwa_retrieve_noalloc).  Allocates nothing. */
 DWA_API int dwa_retrieve_noalloc_status(void* stream, uint32_t* status, int clear);
+
+/* ---------------------------------------------------------------------------
+ * Operators on rows of logits over a vocabulary: a teacher's top logits, the
+ * distillation loss of a student from them, and sampling.  They stand where the
+ * reference turns the model's logits into its loss (task_loss,
+ * src/dwa/losses.py:76-87) and into tokens (generate, train.py:598-735).
+ *
+ * Logits are `rows` rows of V contiguous elements (V <= DWA_MAX_VOCAB), row r
+ * at (r / rows_inner) * stride_outer + (r % rows_inner) * stride_inner
+ * elements: [rows, V] contiguous is rows_inner = rows, stride_inner = V; the
+ * view logits[:, :-1] of [B, T, V] is rows_inner = T - 1, stride_outer = T * V,
+ * stride_inner = V.  A row may start on any element; outputs are contiguous.
+ * rows may be 0 (nothing is launched).
+ * ------------------------------------------------------------------------- */
+#define DWA_MAX_VOCAB (1 << 20)
+#define DWA_MAX_TOP   1024
+
+typedef struct DwaLogitsDims {
+    int64_t rows, rows_inner;
+    int64_t stride_outer, stride_inner;   /* elements, not negative */
+    int32_t V;
+    int32_t dtype;                        /* DWA_F32 or DWA_BF16 */
+} DwaLogitsDims;
+
+/* The K largest logits of every row (K <= DWA_MAX_TOP): values [rows, K] in the
+ * logits' dtype and indices [rows, K] int32, largest first, equal ones by lower
+ * index (-0 equals +0; a NaN comes before every number), and lse [rows] f32 =
+ * log sum_j exp(z_j / temperature) (-inf for a row of -inf, +inf with a +inf in
+ * it, NaN with a NaN). */
+DWA_API int dwa_top_logits(void* stream, const DwaLogitsDims* dims, const void* logits, int K,
+                           float temperature, void* values, int32_t* indices, float* lse);
+
+/* Distillation loss.  teacher_logits [rows, K] (teacher_dtype) are the teacher's
+ * logits of the entries teacher_indices [rows, K] int32 (a negative index: an
+ * unused slot), K <= DWA_MAX_TOP.  With q = softmax(z / T):
+ *   teacher_lse == NULL: p = softmax(teacher_logits / T) over the listed entries;
+ *   teacher_lse [rows] (log-sum-exp of the teacher's whole row at T): p_k =
+ *     exp(t_k / T - lse), and all other entries form one class with
+ *     p_t = max(1 - sum p, 2^-24), q_t = the sum of their q.
+ *   reverse == 0: L = sum p (log p - log q);  else L = sum q (log q - log p)
+ *   (reverse needs teacher_lse).
+ * Terms with p = 0 (q = 0 in reverse) are 0; an empty q_t costs nothing if p_t
+ * <= 2^-16, the rounding of an fp32 lse.  A row without listed entries, or whose
+ * listed teacher logits are all -inf, has loss 0.
+ *   loss [rows] f32 = weights[r] * L (weights NULL: 1; weights[r] == 0: 0,
+ *     whatever the row's logits hold)
+ *   state [rows, DWA_DISTILL_STATE_FLOATS] f32 or NULL: what dwa_distill_bwd needs
+ *   g_logits [rows, V] in the logits' dtype or NULL: the gradient of sum loss;
+ *     may be the memory of contiguous logits
+ * dwa_distill_bwd writes the gradient of sum g_loss[r] * loss[r] from the same
+ * inputs and the state.  An index >= V, or one listed twice in a row, sets
+ * DWA_STATUS_BAD_TOKEN in the workspace's status word and makes the row's loss
+ * and gradient NaN. */
+#define DWA_DISTILL_STATE_FLOATS 8
+
+typedef struct DwaDistillDims {
+    int32_t K;
+    int32_t teacher_dtype;   /* DWA_F32 or DWA_BF16 */
+    float   temperature;     /* T > 0 */
+    int32_t reverse;
+} DwaDistillDims;
+
+DWA_API size_t dwa_distill_workspace_bytes(void);
+DWA_API int dwa_distill_fwd(void* stream, const DwaLogitsDims* dims, const DwaDistillDims* opts,
+                            const void* logits, const void* teacher_logits, const int32_t* teacher_indices,
+                            const float* teacher_lse, const float* weights, float* loss, float* state,
+                            void* g_logits, void* workspace, size_t workspace_bytes);
+DWA_API int dwa_distill_bwd(void* stream, const DwaLogitsDims* dims, const DwaDistillDims* opts,
+                            const void* logits, const void* teacher_logits, const int32_t* teacher_indices,
+                            const float* teacher_lse, const float* weights, const float* state,
+                            const float* g_loss, void* g_logits);
+
+/* One token per row.  noise: row r's V numbers at r * noise_stride, drawn from
+ * the exponential distribution (positive).  With w_i = exp((z_i - max z) / T):
+ * the top_k largest stay (top_k <= 0 or >= V: all; ties by lower index), of
+ * these the entries before which less than top_p of their mass lies (top_p >= 1:
+ * all; the first always stays), of these the ones with w_i >= min_p; the token
+ * is the one with the largest w_i / noise_i (ties by lower index), logprob the
+ * log of its share of the kept mass.  T <= 0 takes the largest logit, logprob 0.
+ * A row of -inf alone, or with a NaN, gives token -1 and logprob NaN.  Each
+ * parameter is one value for all rows, or a device array [rows] where its
+ * pointer is not NULL. */
+typedef struct DwaSampleParams {
+    const float*   temperature_rows;
+    const int32_t* top_k_rows;
+    const float*   top_p_rows;
+    const float*   min_p_rows;
+    float   temperature;
+    int32_t top_k;
+    float   top_p, min_p;
+} DwaSampleParams;
+
+DWA_API int dwa_sample_tokens(void* stream, const DwaLogitsDims* dims, const DwaSampleParams* params,
+                              const void* logits, const float* noise, int64_t noise_stride,
+                              int32_t* tokens, float* logprobs);
 
 #ifdef __cplusplus
 }

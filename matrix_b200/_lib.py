@@ -18,6 +18,9 @@ DWA_ERR_DEVICE = -5
 DWA_PAD_INDEX = -(2 ** 31)
 DWA_F32 = 0
 DWA_BF16 = 1
+DWA_MAX_VOCAB = 1 << 20
+DWA_MAX_TOP = 1024
+DWA_DISTILL_STATE_FLOATS = 8
 
 STATUS_BITS = {
     0x1: "row index outside the pool",
@@ -25,6 +28,7 @@ STATUS_BITS = {
     0x4: "list offsets not monotone or out of range",
     0x8: "a probed list is longer than max_list",
     0x10: "fewer candidates than k",
+    0x20: "a teacher's index outside the vocabulary, or listed twice in a row",
 }
 
 
@@ -69,6 +73,21 @@ class AuxShard(C.Structure):
 
 class AuxWeights(C.Structure):
     _fields_ = [("util", C.c_float), ("div", C.c_float), ("norm", C.c_float), ("sparse", C.c_float)]
+
+
+class LogitsDims(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("rows_inner", C.c_int64), ("stride_outer", C.c_int64),
+                ("stride_inner", C.c_int64), ("V", C.c_int32), ("dtype", C.c_int32)]
+
+
+class DistillDims(C.Structure):
+    _fields_ = [("K", C.c_int32), ("teacher_dtype", C.c_int32), ("temperature", C.c_float), ("reverse", C.c_int32)]
+
+
+class SampleParams(C.Structure):
+    _fields_ = [("temperature_rows", C.c_void_p), ("top_k_rows", C.c_void_p), ("top_p_rows", C.c_void_p),
+                ("min_p_rows", C.c_void_p), ("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float),
+                ("min_p", C.c_float)]
 
 
 _P = C.c_void_p
@@ -142,6 +161,13 @@ _SIGNATURES = {
     "dwa_retrieve_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(RetrieveDims), C.c_int]),
     "dwa_retrieve_bwd": (C.c_int, [_P, C.POINTER(RetrieveDims), C.c_int, C.c_int, _P, _P, _P, _P, _P, _P,
                                    _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t]),
+    "dwa_top_logits": (C.c_int, [_P, C.POINTER(LogitsDims), _P, C.c_int, C.c_float, _P, _P, _P]),
+    "dwa_distill_workspace_bytes": (C.c_size_t, []),
+    "dwa_distill_fwd": (C.c_int, [_P, C.POINTER(LogitsDims), C.POINTER(DistillDims), _P, _P, _P, _P, _P, _P, _P, _P,
+                                  _P, C.c_size_t]),
+    "dwa_distill_bwd": (C.c_int, [_P, C.POINTER(LogitsDims), C.POINTER(DistillDims), _P, _P, _P, _P, _P, _P, _P,
+                                  _P]),
+    "dwa_sample_tokens": (C.c_int, [_P, C.POINTER(LogitsDims), C.POINTER(SampleParams), _P, _P, C.c_int64, _P, _P]),
     "dwa_retrieve_merge": (C.c_int, [_P, C.POINTER(RetrieveDims), C.c_int, _P, C.c_int, _P, _P, _P,
                                      _P, _P, _P, C.c_size_t]),
 }

@@ -1,0 +1,161 @@
+"""Distillation from a teacher's top logits on libdwa's B200 kernels.
+
+The reference trains its model on hard labels (``task_loss``,
+src/dwa/losses.py:76-87).  Here the student's logits ``z [..., V]`` learn from
+what a teacher hands out for every position: its K largest logits, their
+indices and, for the mass it does not list, its log-sum-exp (``top_logits``).
+
+With ``q = softmax(z / T)`` and the teacher's logits ``t_k`` of entries ``i_k``:
+
+* ``teacher_lse=None``: ``p = softmax(t / T)`` over the listed entries alone;
+* with ``teacher_lse`` (at the same temperature): ``p_k = exp(t_k / T - lse)``,
+  and all entries not listed form one class with ``p = max(1 - sum p_k,
+  2^-24)`` and ``q`` = the sum of their ``q``.
+
+The loss of a row is ``sum p (log p - log q)``, or with ``reverse=True``
+(which needs ``teacher_lse``) ``sum q (log q - log p)``, times the row's weight.
+No factor T^2 is applied; pass it in the weights.
+
+Three calls: ``distill_loss`` (values), ``distill_loss_and_grad`` (values and the
+gradient of their sum in one pass, for a step that knows its row weights) and
+``distill_loss_with_grad`` (through autograd).  Logits may be float32 or
+bfloat16 and any view with dense rows, e.g. ``logits[:, :-1]``; a negative
+index is an unused slot; a row of weight 0 is skipped, whatever it holds; a row
+with nothing listed has loss 0.  An index >= V, or one listed twice in a row,
+makes the row's loss and gradient NaN and is reported by
+``runtime.raise_on_device_status``.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .runtime import dtype_code, logits_view, ptr, require_cuda, stream_of, workspace
+
+MAX_TOP = _lib.DWA_MAX_TOP
+
+
+def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0):
+    """The ``k`` largest of every row of ``logits [..., V]`` (``k <= 1024``):
+    ``(values [..., k] in the logits' dtype, indices [..., k] int32, lse [...]
+    f32)``, largest first and equal ones by lower index, with ``lse`` the log of
+    the row's ``sum exp(z / temperature)``.  A NaN comes before every number.
+    """
+    z, dims = logits_view("logits", logits)
+    lead, dev = logits.shape[:-1], logits.device
+    values = torch.empty((*lead, k), dtype=logits.dtype, device=dev)
+    indices = torch.empty((*lead, k), dtype=torch.int32, device=dev)
+    lse = torch.empty(lead, dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        rc = _lib.load().dwa_top_logits(stream_of(dev), dims, ptr(z), int(k), float(temperature), ptr(values),
+                                        ptr(indices), ptr(lse))
+    _lib.check(rc, "dwa_top_logits")
+    return values, indices, lse
+
+
+class _Call:
+    """The checked arguments of one distillation call."""
+
+    def __init__(self, logits, teacher_logits, teacher_indices, teacher_lse, temperature, reverse, weights):
+        self.z, self.dims = logits_view("logits", logits)
+        self.dev, self.lead = logits.device, logits.shape[:-1]
+        if teacher_logits.dim() != logits.dim() or teacher_logits.shape[:-1] != self.lead:
+            raise ValueError(f"teacher_logits must be {[*self.lead, 'K']}, got {list(teacher_logits.shape)}")
+        if teacher_indices.shape != teacher_logits.shape:
+            raise ValueError("teacher_indices must have the shape of teacher_logits")
+        if teacher_indices.dtype not in (torch.int32, torch.int64):
+            raise TypeError("teacher_indices must be int32 or int64")
+        if reverse and teacher_lse is None:
+            raise ValueError("reverse=True needs teacher_lse: without it the teacher gives unlisted entries no mass")
+        self.t = self._input("teacher_logits", teacher_logits.detach())
+        self.idx = self._input("teacher_indices", teacher_indices).to(torch.int32)
+        self.lse = self._row("teacher_lse", teacher_lse)
+        self.w = self._row("weights", weights)
+        self.opts = _lib.DistillDims(teacher_logits.shape[-1], dtype_code(teacher_logits.dtype, "teacher_logits"),
+                                     float(temperature), int(bool(reverse)))
+
+    def _input(self, name, t):
+        t = t.contiguous()
+        require_cuda(name, t, self.dev)
+        return t
+
+    def _row(self, name, t):
+        if t is None:
+            return None
+        if t.shape != self.lead:
+            raise ValueError(f"{name} must be {list(self.lead)}, got {list(t.shape)}")
+        if t.dtype != torch.float32:
+            raise TypeError(f"{name} must be float32")
+        return self._input(name, t.detach())
+
+    def _common(self):
+        return ptr(self.z), ptr(self.t), ptr(self.idx), ptr(self.lse), ptr(self.w)
+
+    def forward(self, state=None, g=None):
+        lib = _lib.load()
+        loss = torch.empty(self.lead, dtype=torch.float32, device=self.dev)
+        ws = workspace(self.dev, "distill", lib.dwa_distill_workspace_bytes())
+        with torch.cuda.device(self.dev):
+            rc = lib.dwa_distill_fwd(stream_of(self.dev), self.dims, self.opts, *self._common(), ptr(loss), ptr(state),
+                                     ptr(g), ptr(ws), ws.numel())
+        _lib.check(rc, "dwa_distill_fwd")
+        return loss
+
+    def backward(self, state, g_loss, g):
+        with torch.cuda.device(self.dev):
+            rc = _lib.load().dwa_distill_bwd(stream_of(self.dev), self.dims, self.opts, *self._common(), ptr(state),
+                                             ptr(g_loss), ptr(g))
+        _lib.check(rc, "dwa_distill_bwd")
+        return g
+
+
+def distill_loss(logits, teacher_logits, teacher_indices, *, teacher_lse=None, temperature=1.0, reverse=False,
+                 weights=None) -> torch.Tensor:
+    """The rows' losses ``[...]`` f32, each times its weight (no gradient)."""
+    return _Call(logits.detach(), teacher_logits, teacher_indices, teacher_lse, temperature, reverse,
+                 weights).forward()
+
+
+def distill_loss_and_grad(logits, teacher_logits, teacher_indices, *, teacher_lse=None, temperature=1.0,
+                          reverse=False, weights=None, out=None):
+    """``(loss [...], g_logits [..., V])``: the rows' losses and the gradient of
+    their sum (of the weighted sum: a mean is ``weights = 1 / rows``), in the
+    logits' dtype.  ``out`` takes the gradient; it may be contiguous ``logits``
+    themselves, which are then overwritten."""
+    logits = logits.detach()
+    call = _Call(logits, teacher_logits, teacher_indices, teacher_lse, temperature, reverse, weights)
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    else:
+        require_cuda("out", out, logits.device)
+        if out.shape != logits.shape or out.dtype != logits.dtype:
+            raise ValueError("out must have the logits' shape and dtype")
+    return call.forward(g=out), out
+
+
+class _DistillFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, call):
+        state = torch.empty((*call.lead, _lib.DWA_DISTILL_STATE_FLOATS), dtype=torch.float32, device=call.dev)
+        loss = call.forward(state)
+        ctx.save_for_backward(call.z, call.t, call.idx, call.lse, call.w, state)
+        ctx.call, ctx.like = call, (logits.shape, logits.dtype)
+        call.z = call.t = call.idx = call.lse = call.w = None   # held, and checked for changes, by autograd
+        return loss
+
+    @staticmethod
+    def backward(ctx, g_loss):
+        call = ctx.call
+        call.z, call.t, call.idx, call.lse, call.w, state = ctx.saved_tensors
+        g = torch.empty(ctx.like[0], dtype=ctx.like[1], device=call.dev)
+        call.backward(state, g_loss.float().contiguous(), g)
+        call.z = call.t = call.idx = call.lse = call.w = None
+        return g, None
+
+
+def distill_loss_with_grad(logits, teacher_logits, teacher_indices, *, teacher_lse=None, temperature=1.0,
+                           reverse=False, weights=None) -> torch.Tensor:
+    """The rows' losses ``[...]`` f32, differentiable in ``logits``."""
+    call = _Call(logits, teacher_logits, teacher_indices, teacher_lse, temperature, reverse, weights)
+    return _DistillFunction.apply(logits, call)

@@ -77,3 +77,37 @@ def raise_on_device_status() -> None:
     if bad:
         msg = "; ".join(f"{k[1]}@cuda:{k[0]}: {_lib.describe_status(v)}" for k, v in bad.items())
         raise _lib.DwaError(f"device status: {msg}")
+
+
+def logits_view(name: str, t: torch.Tensor) -> tuple[torch.Tensor, "_lib.LogitsDims"]:
+    """``t [..., V]`` as libdwa reads logits: the tensor and its row layout.
+
+    Any view whose leading dimensions collapse into two strides and whose last
+    one is dense is read in place (``logits[:, :-1]``, ``logits[..., :V]``);
+    others are made contiguous first.
+    """
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on a CUDA device (the hot path has no CPU fallback)")
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError(f"{name} must be [..., V] with V >= 1")
+    code, V = dtype_code(t.dtype, name), t.shape[-1]
+    if t.is_contiguous():
+        rows = t.numel() // V
+        return t, _lib.LogitsDims(rows, max(rows, 1), 0, V, V, code)
+    rows = 1
+    levels: list[list[int]] = []   # [size, stride], innermost first
+    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        rows *= size
+        if size == 1:
+            continue
+        if levels and stride == levels[-1][0] * levels[-1][1]:
+            levels[-1][0] *= size
+        else:
+            levels.append([size, stride])
+    if rows == 0 or len(levels) > 2 or (V > 1 and t.stride(-1) != 1):
+        return logits_view(name, t.contiguous())
+    inner = levels[0] if levels else [1, V]
+    outer = levels[1][1] if len(levels) == 2 else 0
+    return t, _lib.LogitsDims(rows, inner[0], outer, inner[1], V, code)

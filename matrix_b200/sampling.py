@@ -1,0 +1,66 @@
+"""Sampling tokens from logits on libdwa's B200 kernels.
+
+The reference samples inside ``generate`` (train.py:598-735).  ``sample_tokens``
+draws one token a row from given random numbers, so that a program owns its
+randomness: ``noise [..., V]`` holds numbers from the exponential distribution
+(``torch.empty_like(logits, dtype=torch.float32).exponential_(generator=g)``),
+and the token is the kept entry with the largest ``weight / noise``, which draws
+an entry with probability proportional to its weight.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .runtime import logits_view, ptr, stream_of
+
+
+def _per_row(name, value, lead, dev, dtype):
+    """``(tensor or None, scalar)`` of a parameter given for all rows or for each."""
+    if not isinstance(value, torch.Tensor):
+        return None, value
+    if not value.is_cuda or value.device != dev:
+        raise ValueError(f"{name} must be on {dev}")
+    if value.shape != lead:
+        raise ValueError(f"{name} must be a number or {list(lead)}, got {list(value.shape)}")
+    if value.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}")
+    return value.contiguous(), 0
+
+
+def sample_tokens(logits: torch.Tensor, noise: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """``(tokens [...] int32, logprobs [...] f32)`` of ``logits [..., V]``.
+
+    With ``w_i = exp((z_i - max z) / temperature)``: the ``top_k`` largest entries
+    stay (``<= 0`` or ``>= V``: all; equal ones by lower index), of these the ones
+    before which less than ``top_p`` of their mass lies (``>= 1``: all; the first
+    always stays), of these the ones with ``w_i >= min_p``.  ``logprobs`` is the
+    log of the token's share of the kept mass.  A temperature ``<= 0`` takes the
+    largest logit (logprob 0).  A row that holds only -inf, or a NaN, gives token
+    -1 and logprob NaN.  Each parameter is a number, or a tensor ``[...]`` with
+    one per row (float32; ``top_k`` int32)."""
+    z, dims = logits_view("logits", logits.detach())
+    lead, dev = logits.shape[:-1], logits.device
+    if not isinstance(noise, torch.Tensor) or noise.device != dev:
+        raise ValueError(f"noise must be a tensor on {dev}")
+    if noise.shape != logits.shape:
+        raise ValueError("noise must have the shape of logits")
+    if noise.dtype != torch.float32:
+        raise TypeError("noise must be float32")
+    noise, nd = logits_view("noise", noise)
+    if nd.rows_inner < nd.rows:
+        noise, nd = logits_view("noise", noise.contiguous())
+    t, t0 = _per_row("temperature", temperature, lead, dev, torch.float32)
+    k, k0 = _per_row("top_k", top_k, lead, dev, torch.int32)
+    p, p0 = _per_row("top_p", top_p, lead, dev, torch.float32)
+    m, m0 = _per_row("min_p", min_p, lead, dev, torch.float32)
+    params = _lib.SampleParams(*(None if x is None else x.data_ptr() for x in (t, k, p, m)), float(t0), int(k0),
+                               float(p0), float(m0))
+    tokens = torch.empty(lead, dtype=torch.int32, device=dev)
+    logprobs = torch.empty(lead, dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        rc = _lib.load().dwa_sample_tokens(stream_of(dev), dims, params, ptr(z), ptr(noise), nd.stride_inner,
+                                           ptr(tokens), ptr(logprobs))
+    _lib.check(rc, "dwa_sample_tokens")
+    return tokens, logprobs

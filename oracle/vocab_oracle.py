@@ -1,0 +1,112 @@
+"""NumPy restatement, in float64, of the operators on rows of logits: a teacher's
+top logits, the distillation loss and its gradient, and sampling.
+
+Written from the definitions, one row at a time; the tests of the CUDA
+operators compare with these, and these are checked against finite differences
+and by hand-made rows.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+
+TAIL_FLOOR = 2.0 ** -24   # the least mass a teacher's tail is given
+TAIL_NONE = 2.0 ** -16    # a tail up to this may be the rounding of an fp32 log-sum-exp
+
+
+def order(z) -> np.ndarray:
+    """Indices by descending value, equal values by index, NaN first."""
+    z = np.asarray(z, dtype=np.float64)
+    return np.lexsort((np.arange(z.size), -np.where(np.isnan(z), np.inf, z), ~np.isnan(z)))
+
+
+def logsumexp(x) -> float:
+    x = np.asarray(x, dtype=np.float64)
+    if np.isnan(x).any():
+        return np.nan
+    m = x.max(initial=-np.inf)
+    if np.isinf(m):
+        return m
+    return m + np.log(np.exp(x - m).sum())
+
+
+def top_logits(z, k, temperature=1.0):
+    """``(values, indices, lse)`` of one row."""
+    i = order(z)[:k]
+    return np.asarray(z)[i], i, logsumexp(np.asarray(z, dtype=np.float64) / temperature)
+
+
+def distill(z, t, idx, lse=None, temperature=1.0, reverse=False, weight=1.0):
+    """``(weight * L, its gradient [V])`` of one row.  Negative ``idx``: unused."""
+    z = np.asarray(z, dtype=np.float64)
+    idx = np.asarray(idx)
+    use = idx >= 0
+    idx, t = idx[use], np.asarray(t, dtype=np.float64)[use] / temperature
+    if weight == 0.0 or idx.size == 0 or (lse is None and np.all(t == -np.inf)):
+        return 0.0, np.zeros_like(z)
+    x = z / temperature
+    with np.errstate(all="ignore"):
+        log_q = x - logsumexp(x)
+        q = np.exp(log_q)
+        log_p = t - (logsumexp(t) if lse is None else lse)
+        p = np.exp(log_p)
+        unlisted = np.ones(z.size, dtype=bool)
+        unlisted[idx] = False
+        has_tail = lse is not None and unlisted.any()
+        lq, qk = log_q[idx], q[idx]
+        if reverse:
+            loss = sum(a * (b - c) for a, b, c in zip(qk, lq, log_p) if a != 0)
+        else:
+            loss = sum(a * (b - c) for a, b, c in zip(p, log_p, lq) if a != 0)
+        of_tail = 1.0
+        if has_tail:
+            p_t = max(1.0 - p.sum(), TAIL_FLOOR)
+            log_qt = logsumexp(log_q[unlisted])
+            q_t = np.exp(log_qt)
+            if q_t == 0.0:
+                of_tail = 0.0
+                if not reverse and p_t > TAIL_NONE:
+                    loss = np.inf
+            else:
+                r_t = log_qt - np.log(p_t)
+                loss += q_t * r_t if reverse else -p_t * r_t
+                of_tail = r_t - loss if reverse else 1.0 - p_t / q_t
+        g = q * of_tail
+        g[idx] = np.where(qk == 0.0, 0.0, qk * (lq - log_p - loss)) if reverse else qk - p
+    return weight * loss, weight / temperature * g
+
+
+def sample(z, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, shift=0.0):
+    """``(token, logprob, margin)`` of one row.  ``margin`` is how much larger,
+    relatively, the winning score is than the next.  ``shift`` moves both cuts by
+    that part of their mass: where it changes the token, rounding may."""
+    z = np.asarray(z, dtype=np.float64)
+    if np.isnan(z).any() or np.all(z == -np.inf):
+        return -1, np.nan, np.inf
+    i = order(z)
+    if not temperature > 0:
+        return int(i[0]), 0.0, np.inf
+    m = z[i[0]]
+    with np.errstate(all="ignore"):
+        w = np.where(z[i] == m, 1.0, np.where((z[i] == -np.inf) | (m == np.inf), 0.0, np.exp((z[i] - m) / temperature)))
+    n = top_k if 0 < top_k < z.size else z.size
+    i, w = i[:n], w[:n]
+    if top_p < 1:
+        before = np.concatenate(([0.0], np.cumsum(w)[:-1]))
+        n = max(1, int((before < (max(top_p, 0.0) + shift) * w.sum()).sum()))
+        i, w = i[:n], w[:n]
+    keep = w > 0
+    if min_p > 0:
+        keep &= w >= min(min_p, 1.0) * (1.0 - shift)
+        keep[0] = True
+    i, w = i[keep], w[keep]
+    with np.errstate(all="ignore"):
+        score = w / np.asarray(noise, dtype=np.float64)[i]
+    ok = score >= 0
+    if not ok.any():
+        return -1, np.nan, np.inf
+    best = max(np.flatnonzero(ok), key=lambda a: (score[a], -i[a]))
+    others = np.delete(score, best)
+    others = others[others >= 0].max(initial=0.0)
+    margin = np.inf if others == score[best] else 1.0 - others / score[best]   # equal scores: the index decides
+    return int(i[best]), float(np.log(w[best] / w.sum())), float(margin)
