@@ -66,7 +66,7 @@ struct DistillArgs {
 
 // dL/dx of listed entry k, from its logits.
 __device__ __forceinline__ float listed_grad(const RowState& s, const DistillArgs& a, float zk, float tk) {
-    const float q = exp2f((zk - s.m) * a.c) / s.S;
+    const float q = exp2_fast((zk - s.m) * a.c) / s.S;
     const double T = a.o.temperature;
     const double lp = (static_cast<double>(tk) - s.t_hi) / T - s.t_lo;
     if (!a.o.reverse) return q - (tk == -INFINITY ? 0.f : expf(static_cast<float>(lp)));
@@ -86,10 +86,11 @@ __device__ __forceinline__ void write_grad(const RowWords<T>& w, T* g, const Row
     const int kind = static_cast<int>(s.kind);
     const float unl = kind == kRowPlain ? s.of_tail * scale / s.S : kind == kRowZero ? 0.f : NAN;
     const bool same = (reinterpret_cast<uintptr_t>(g) - reinterpret_cast<uintptr_t>(w.row)) % 16 == 0;
-    w.template each<4>(0, w.words, tid, n, [&](const float* v, int j0) {
+    w.template each<4>(0, w.words, tid, n, [&](uint4 x, int j0, int) {
         float o[VEC];
+        word_exp<T>(x, s.m, a.c, o);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = kind == kRowPlain ? exp2f((v[i] - s.m) * a.c) * unl : unl;
+        for (int i = 0; i < VEC; ++i) o[i] = kind == kRowPlain ? o[i] * unl : unl;
         if (same && j0 >= 0 && j0 + VEC <= w.V) {
             *reinterpret_cast<uint4*>(g + j0) = pack<T>(o);
         } else {
@@ -157,27 +158,28 @@ __global__ void __launch_bounds__(kDistillThreads) distill_fwd_kernel(DistillArg
 
     // one pass: the row's maximum, and the sum over unlisted entries
     MaxSum ms;
-    w.template each<4>(0, w.words, tid, n, [&](const float* v, int j0) {
-        float top = v[0];
-#pragma unroll
-        for (int i = 1; i < VEC; ++i) top = fmaxf(top, v[i]);
-        ms.raise(top, a.c);
+    w.template each<4>(0, w.words, tid, n, [&](uint4 x, int j0, int) {
+        ms.raise(word_max<T>(x), a.c);
+        float e[VEC];
+        word_exp<T>(x, ms.m, a.c, e);
         const int b = j0 + w.shift;
-        const uint32_t listed = bits[b >> 5] >> (b & 31);
-        if (ms.m > -INFINITY) {
+        const uint32_t listed = bits[b >> 5] >> (b & 31) & ((1u << VEC) - 1u);
+        if (listed == 0u && ms.m > -INFINITY) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i)
-                ms.s += (listed >> i) & 1u ? 0.f : exp2f((v[i] - ms.m) * a.c);
+            for (int i = 0; i < VEC; ++i) ms.s += e[i];
+        } else if (ms.m > -INFINITY) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) ms.s += (listed >> i) & 1u ? 0.f : e[i];
         }
     });
     s.m = block_reduce(ms.m, MaxOp(), -INFINITY, redf);
-    const float S_u = block_reduce(ms.m > -INFINITY ? ms.s * exp2f((ms.m - s.m) * a.c) : ms.s, AddOp(), 0.f, redf);
+    const float S_u = block_reduce(ms.at(s.m, a.c), AddOp(), 0.f, redf);
 
     // the listed entries
     const double T0 = a.o.temperature;
     float S_l = 0.f;
     for (int k = tid; k < K; k += n)
-        if (idx[k] >= 0) S_l += exp2f((zk[k] - s.m) * a.c);
+        if (idx[k] >= 0) S_l += exp2_fast((zk[k] - s.m) * a.c);
     S_l = block_reduce(S_l, AddOp(), 0.f, redf);
     s.S = S_u + S_l;
     const double log_S = log(static_cast<double>(S_u) + S_l);
@@ -201,7 +203,7 @@ __global__ void __launch_bounds__(kDistillThreads) distill_fwd_kernel(DistillArg
         const float p = tk[k] == -INFINITY ? 0.f : expf(static_cast<float>(lp));
         P += p;
         if (a.o.reverse) {
-            const float q = exp2f((zk[k] - s.m) * a.c) / s.S;
+            const float q = exp2_fast((zk[k] - s.m) * a.c) / s.S;
             if (q != 0.f) L += q * (lq - lp);
         } else if (p != 0.f) {
             L += p * (lp - lq);

@@ -25,7 +25,11 @@ namespace dwa {
 
 extern std::atomic<uint64_t> g_launches_total;
 
-constexpr int kSelThreads = 512;
+constexpr int kSelThreads = 256;
+constexpr int kSelGroups = 8 * kSelThreads;   // groups of words whose maxima are compared
+constexpr int kSelList = 2048;                // candidates held
+constexpr int kTryTop = 256;                  // entries sorted first when only a mass or a floor limits the row
+constexpr int kSelMaxCluster = 8;
 
 // A logit as an unsigned integer of the same order.
 __device__ __forceinline__ uint32_t ordered(float z) {
@@ -76,7 +80,9 @@ __device__ uint64_t cut_key(const RowWords<T>& w, uint64_t floor, uint64_t targe
         __syncthreads();
         for (int i = tid; i < 256; i += blockDim.x) hist[i] = 0ull;
         __syncthreads();
-        w.template each<2>(0, w.words, tid, blockDim.x, [&](const float* v, int j0) {
+        w.template each<2>(0, w.words, tid, blockDim.x, [&](uint4 x, int j0, int) {
+            float v[kRowVec<T>];
+            unpack<T>(x, v);
 #pragma unroll
             for (int i = 0; i < kRowVec<T>; ++i) {
                 const uint64_t key = entry_key(v[i], j0 + i);
@@ -85,9 +91,9 @@ __device__ uint64_t cut_key(const RowWords<T>& w, uint64_t floor, uint64_t targe
                     const unsigned peers = __match_any_sync(__activemask(), digit);
                     unsigned long long sum;
                     if (MASS) {
-                        const uint32_t x = weigh.fixed(v[i]);
-                        sum = (static_cast<unsigned long long>(__reduce_add_sync(peers, x >> 16)) << 16) +
-                              __reduce_add_sync(peers, x & 0xffffu);
+                        const uint32_t units = weigh.fixed(v[i]);
+                        sum = (static_cast<unsigned long long>(__reduce_add_sync(peers, units >> 16)) << 16) +
+                              __reduce_add_sync(peers, units & 0xffffu);
                     } else {
                         sum = __popc(peers);
                     }
@@ -123,77 +129,270 @@ __device__ uint64_t cut_key(const RowWords<T>& w, uint64_t floor, uint64_t targe
 }
 
 // ---------------------------------------------------------------------------
-// the largest logits
+// a row's largest entries
 // ---------------------------------------------------------------------------
+// A cluster of P CTAs scans a row, CTA p the words [words p / P, words (p + 1) / P).
+// A thread's words fall into 8 / P groups (its i-th word into group i mod 8 / P),
+// 2048 groups in all, whose maxima go to rank 0's shared memory.  The K-th
+// largest of these maxima is at most the K-th largest entry, and only the groups
+// that reach it hold candidates: about K of them, 1/2048 of the row each (and a row's
+// ragged first and last word, which are in no group and looked at each time).  So the
+// row is read once and a few percent of it again, and the candidates (K and a
+// few more) are sorted in shared memory.
+struct SelShared {
+    union {
+        uint32_t group[kSelGroups];
+        unsigned long long hist[256];
+    };
+    unsigned long long list[kSelList];   // candidates; sorted: the K largest in descending order
+    uint16_t chosen[kSelGroups];
+    float part_m[kSelMaxCluster], part_s[kSelMaxCluster], part_b[kSelMaxCluster];
+    int part_j[kSelMaxCluster];
+    uint32_t warp_count[2][kSelThreads / 32];
+    unsigned long long found[2];
+    unsigned long long red64[33];
+    double redd[33], scan[kSelThreads / 32 + 1];
+    float redf[33];
+    int n_chosen, n_list;
+};
+
+struct Chunk {
+    int lo, hi;
+    __device__ __forceinline__ Chunk(int words, int p, int P)
+        : lo(static_cast<int>(static_cast<int64_t>(words) * p / P)),
+          hi(static_cast<int>(static_cast<int64_t>(words) * (p + 1) / P)) {}
+};
+
+// This CTA's share: the maxima of the thread's words by position mod 8 (`edge`:
+// of a row's first and last word where they are not whole) and, with SUM, the
+// running maximum and sum of exp((z - m) / T).
+template <class T, bool SUM>
+__device__ __forceinline__ void scan_chunk(const RowWords<T>& w, Chunk ch, float c, float (&top)[8], float& edge,
+                                           MaxSum& ms) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) top[u] = -INFINITY;
+    edge = -INFINITY;
+    w.template each<8>(ch.lo, ch.hi, threadIdx.x, kSelThreads, [&](uint4 x, int, int u) {
+        const float m = word_max<T>(x);
+        if (u < 0) edge = m;
+        else top[u] = max_nan(top[u], m);
+        if constexpr (SUM) {
+            ms.raise(m, c);
+            if (ms.m > -INFINITY) {
+                float e[kRowVec<T>];
+                word_exp<T>(x, ms.m, c, e);
+#pragma unroll
+                for (int i = 0; i < kRowVec<T>; ++i) ms.s += e[i];
+            }
+        }
+    });
+}
+
+// The groups' maxima and the CTA's (m, s) into rank 0's shared memory.  Ends in
+// a cluster barrier; only rank 0 goes on with what lies there.
+__device__ __forceinline__ void push_groups(SelShared& sh, int p, int P, float (&top)[8], float edge, const MaxSum& ms,
+                                            float c) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cl = cg::this_cluster();
+    const int tid = threadIdx.x, per = 8 / P;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        if (P >= 2) top[u] = max_nan(top[u], top[u + 4]);
+    if (P >= 4) {
+        top[0] = max_nan(top[0], top[2]);
+        top[1] = max_nan(top[1], top[3]);
+    }
+    if (P >= 8) top[0] = max_nan(top[0], top[1]);
+    float all = edge;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) all = max_nan(all, top[u]);
+    // NaN above everything, as in the keys
+    const uint32_t first = block_reduce(ordered(all), MaxOp(), 0u, reinterpret_cast<uint32_t*>(sh.redf));
+    const float M = block_reduce(ms.m, MaxOp(), -INFINITY, sh.redf);
+    const float S = block_reduce(ms.at(M, c), AddOp(), 0.f, sh.redf);
+    if (P > 1) cluster_wait();   // every CTA of the cluster has started
+    SelShared* to = P > 1 ? cl.map_shared_rank(&sh, 0) : &sh;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+        if (u < per) to->group[(p * per + u) * kSelThreads + tid] = ordered(top[u]);
+    if (tid == 0) {
+        to->part_j[p] = static_cast<int>(first);
+        to->part_m[p] = M;
+        to->part_s[p] = S;
+    }
+    if (P > 1) cl.sync();
+    else __syncthreads();
+}
+
+__device__ __forceinline__ float unordered(uint32_t o) {
+    return o == 0xffffffffu ? NAN : __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+
+// What the parts say of the row: its maximum (NaN if there is one) and, relative
+// to it, the sum.
+__device__ __forceinline__ void row_stats(const SelShared& sh, int P, float c, float& m, float& s) {
+    uint32_t first = 0u;
+    for (int p = 0; p < P; ++p) first = max(first, static_cast<uint32_t>(sh.part_j[p]));
+    m = unordered(first);
+    s = 0.f;
+    for (int p = 0; p < P; ++p) s += sh.part_m[p] > -INFINITY ? sh.part_s[p] * exp2_fast((sh.part_m[p] - m) * c) : 0.f;
+}
+
+// Rank 0: the K largest entries of the row into sh.list, in descending order.
+template <class T>
+__device__ void sort_top(SelShared& sh, const RowWords<T>& w, int P, int K) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint32_t g[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] = sh.group[i * kSelThreads + tid] >> 16;
+    // the largest 16-bit prefix that at least K maxima reach, two bits a round
+    uint32_t t = 0u;
+#pragma unroll 1
+    for (int s = 14; s >= 0; s -= 2) {
+        uint32_t cnt = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            cnt += (g[i] >= (t | 1u << s) ? 1u : 0u) + (g[i] >= (t | 2u << s) ? 1u << 10 : 0u) +
+                   (g[i] >= (t | 3u << s) ? 1u << 20 : 0u);
+        cnt = __reduce_add_sync(0xffffffffu, cnt);
+        uint32_t* wc = sh.warp_count[(s >> 1) & 1];
+        if (lane == 0) wc[warp] = cnt;
+        __syncthreads();
+        int c1 = 0, c2 = 0, c3 = 0;
+#pragma unroll
+        for (int i = 0; i < kSelThreads / 32; ++i) {
+            const uint32_t v = wc[i];
+            c1 += v & 1023u;
+            c2 += v >> 10 & 1023u;
+            c3 += v >> 20;
+        }
+        t |= (c3 >= K ? 3u : c2 >= K ? 2u : c1 >= K ? 1u : 0u) << s;
+    }
+    if (tid == 0) sh.n_chosen = sh.n_list = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (g[i] >= t) sh.chosen[atomicAdd(&sh.n_chosen, 1)] = static_cast<uint16_t>(i * kSelThreads + tid);
+    __syncthreads();
+    const int per = 8 / P, chosen = sh.n_chosen;
+    const int rounds = ((w.words + P - 1) / P + kSelThreads * per - 1) / (kSelThreads * per);   // words of a group
+    const uint64_t floor = static_cast<uint64_t>(t) << 48;
+    const auto take = [&](uint4 x, int j0) {
+        float v[kRowVec<T>];
+        unpack<T>(x, v);
+#pragma unroll
+        for (int e = 0; e < kRowVec<T>; ++e) {
+            const uint64_t key = entry_key(v[e], j0 + e);
+            if (key >= floor && static_cast<unsigned>(j0 + e) < static_cast<unsigned>(w.V)) {
+                const int to = atomicAdd(&sh.n_list, 1);
+                if (to < kSelList) sh.list[to] = key;
+            }
+        }
+    };
+    constexpr int U = 4;
+    for (int i0 = tid; i0 < chosen * rounds; i0 += U * kSelThreads) {
+        uint4 x[U];
+        int at[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * kSelThreads;
+            at[u] = -1;
+            if (i < chosen * rounds) {
+                const int q = sh.chosen[i / rounds], p = q / (kSelThreads * per), r = q % (kSelThreads * per);
+                const Chunk ch(w.words, p, P);
+                const int word = ch.lo + r % kSelThreads + (r / kSelThreads + (i % rounds) * per) * kSelThreads;
+                if (word < ch.hi && w.whole(word)) {
+                    at[u] = word;
+                    x[u] = w.word(word);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (at[u] >= 0) take(x[u], w.first(at[u]));
+        }
+    }
+    w.edges(0, w.words, tid, take);
+    __syncthreads();
+    int n = sh.n_list;
+    if (n > kSelList) {   // equal or ordered entries crowd the groups: find the K-th key itself
+        const uint64_t cut = cut_key<T, false>(w, 0, K, Weigh(0.f, 1.f), sh.hist, sh.found);
+        if (tid == 0) sh.n_list = 0;
+        __syncthreads();
+        w.template each<4>(0, w.words, tid, kSelThreads, [&](uint4 x, int j0, int) {
+            float v[kRowVec<T>];
+            unpack<T>(x, v);
+#pragma unroll
+            for (int e = 0; e < kRowVec<T>; ++e) {
+                const uint64_t key = entry_key(v[e], j0 + e);
+                if (key >= cut && static_cast<unsigned>(j0 + e) < static_cast<unsigned>(w.V))
+                    sh.list[atomicAdd(&sh.n_list, 1)] = key;
+            }
+        });
+        __syncthreads();
+        n = K;
+    }
+    if (n <= kSelThreads) {   // each key to its rank
+        const unsigned long long key = tid < n ? sh.list[tid] : 0ull;
+        int rank = 0;
+        for (int i = 0; i < n; ++i) rank += sh.list[i] > key;
+        __syncthreads();
+        if (tid < n) sh.list[rank] = key;
+    } else {                  // bitonic, padded to a power of two
+        int size = 2 * kSelThreads;
+        while (size < n) size <<= 1;
+        for (int i = n + tid; i < size; i += kSelThreads) sh.list[i] = 0ull;
+        for (int k = 2; k <= size; k <<= 1) {
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                __syncthreads();
+                for (int i = tid; i < size / 2; i += kSelThreads) {
+                    const int a = (i / j) * 2 * j + i % j, b = a + j;
+                    const unsigned long long x = sh.list[a], y = sh.list[b];
+                    if ((x < y) == ((a & k) == 0)) {
+                        sh.list[a] = y;
+                        sh.list[b] = x;
+                    }
+                }
+            }
+        }
+    }
+    __syncthreads();
+}
+
 struct TopArgs {
     const void* z;
     DwaLogitsDims d;
-    int K;
+    int K, P;
     float c, temperature;
     void* values;
     int32_t* indices;
     float* lse;
 };
 
-// A row's maximum and sum of exp((z - max) c); `nan` tells whether one is there.
 template <class T>
-__device__ MaxSum row_max_sum(const RowWords<T>& w, float c, float* red, bool& nan) {
-    MaxSum ms;
-    w.template each<4>(0, w.words, threadIdx.x, blockDim.x, [&](const float* v, int) {
-        float top = v[0];
-#pragma unroll
-        for (int i = 1; i < kRowVec<T>; ++i) top = fmaxf(top, v[i]);
-        ms.raise(top, c);
-#pragma unroll
-        for (int i = 0; i < kRowVec<T>; ++i) ms.s += v[i] == -INFINITY ? 0.f : exp2f((v[i] - ms.m) * c);
-    });
-    const float m = block_reduce(ms.m, MaxOp(), -INFINITY, red);
-    float s = ms.m > -INFINITY ? ms.s * exp2f((ms.m - m) * c) : ms.s;
-    ms.s = block_reduce(s, AddOp(), 0.f, red);
-    ms.m = m;
-    nan = ms.s != ms.s;
-    if (m == INFINITY) {   // inf - inf above: look for a NaN itself
-        int seen = 0;
-        w.template each<1>(0, w.words, threadIdx.x, blockDim.x, [&](const float* v, int) {
-#pragma unroll
-            for (int i = 0; i < kRowVec<T>; ++i) seen |= v[i] != v[i];
-        });
-        nan = __syncthreads_or(seen);
-    }
-    return ms;
-}
-
-template <class T>
-__global__ void __launch_bounds__(kSelThreads) top_logits_kernel(TopArgs a) {
+__global__ void __launch_bounds__(kSelThreads, 4) top_logits_kernel(TopArgs a) {
+    __shared__ SelShared sh;
+    const int P = a.P, tid = threadIdx.x;
+    if (P > 1) cluster_arrive_relaxed();
     pdl_enter();
-    __shared__ unsigned long long hist[256], found[2], list[DWA_MAX_TOP];
-    __shared__ float red[33];
-    __shared__ int count;
-    const int tid = threadIdx.x, K = a.K;
-    const int64_t r = blockIdx.x;
+    const int64_t r = blockIdx.x / P;
+    const int p = blockIdx.x % P;
     const RowWords<T> w(static_cast<const T*>(a.z) + row_offset(a.d, r), a.d.V);
-    bool nan;
-    const MaxSum ms = row_max_sum(w, a.c, red, nan);
+    float top[8], edge;
+    MaxSum ms;
+    scan_chunk<T, true>(w, Chunk(w.words, p, P), a.c, top, edge, ms);
+    push_groups(sh, p, P, top, edge, ms, a.c);
+    if (p != 0) return;
     if (tid == 0) {
-        count = 0;
-        a.lse[r] = nan ? NAN : isinf(ms.m) ? ms.m : ms.m / a.temperature + logf(ms.s);
+        float m, s;
+        row_stats(sh, P, a.c, m, s);
+        a.lse[r] = m != m || isinf(m) ? m : m / a.temperature + logf(s);
     }
-    const uint64_t cut = cut_key<T, false>(w, 0, K, Weigh(0.f, 1.f), hist, found);
-    w.template each<4>(0, w.words, tid, blockDim.x, [&](const float* v, int j0) {
-#pragma unroll
-        for (int i = 0; i < kRowVec<T>; ++i) {
-            const uint64_t key = entry_key(v[i], j0 + i);
-            if (static_cast<unsigned>(j0 + i) < static_cast<unsigned>(w.V) && key >= cut) list[atomicAdd(&count, 1)] = key;
-        }
-    });
-    __syncthreads();
-    for (int k = tid; k < K; k += blockDim.x) {
-        const unsigned long long key = list[k];
-        int rank = 0;
-        for (int i = 0; i < K; ++i) rank += list[i] > key;
-        const int j = key_index(key);
-        static_cast<T*>(a.values)[r * K + rank] = w.row[j];
-        a.indices[r * K + rank] = j;
+    sort_top(sh, w, P, a.K);
+    for (int k = tid; k < a.K; k += kSelThreads) {
+        const unsigned long long key = sh.list[k];
+        static_cast<T*>(a.values)[r * a.K + k] = Elem<T>::from_f(unordered(static_cast<uint32_t>(key >> 32)));
+        a.indices[r * a.K + k] = key_index(key);
     }
 }
 
@@ -206,79 +405,295 @@ struct SampleArgs {
     const float* noise;
     int64_t noise_stride;
     DwaSampleParams p;
+    int P;
     int32_t* tokens;
     float* logprobs;
 };
 
-template <class T>
-__global__ void __launch_bounds__(kSelThreads) sample_kernel(SampleArgs a) {
-    pdl_enter();
-    __shared__ unsigned long long hist[256], found[2], red64[33];
-    __shared__ float red[33];
-    const int tid = threadIdx.x, V = a.d.V;
-    const int64_t r = blockIdx.x;
-    const RowWords<T> w(static_cast<const T*>(a.z) + row_offset(a.d, r), V);
-    const float T0 = a.p.temperature_rows ? a.p.temperature_rows[r] : a.p.temperature;
-    const int top_k = a.p.top_k_rows ? a.p.top_k_rows[r] : a.p.top_k;
-    const float top_p = a.p.top_p_rows ? a.p.top_p_rows[r] : a.p.top_p;
-    const float min_p0 = a.p.min_p_rows ? a.p.min_p_rows[r] : a.p.min_p;
-    const float min_p = min_p0 > 0.f ? fminf(min_p0, 1.f) : 0.f;
-    const bool greedy = !(T0 > 0.f);
-    const float c = greedy ? kLog2e : kLog2e / T0;
+// One row's parameters, as they apply.
+struct Request {
+    float T, top_p, min_p;
+    int k;   // entries that stay
+    bool greedy;
+    __device__ __forceinline__ Request(const DwaSampleParams& q, int64_t r, int V) {
+        T = q.temperature_rows ? q.temperature_rows[r] : q.temperature;
+        k = q.top_k_rows ? q.top_k_rows[r] : q.top_k;
+        top_p = q.top_p_rows ? q.top_p_rows[r] : q.top_p;
+        min_p = q.min_p_rows ? q.min_p_rows[r] : q.min_p;
+        greedy = !(T > 0.f);
+        if (k <= 0 || k > V) k = V;
+        min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
+        top_p = top_p < 1.f ? fmaxf(top_p, 0.f) : 1.f;
+        if (greedy) {
+            T = 1.f;
+            k = 1;
+            top_p = 1.f;
+            min_p = 0.f;
+        }
+    }
+};
 
-    bool nan;
-    const MaxSum ms = row_max_sum(w, c, red, nan);
-    if (nan || ms.m == -INFINITY) {   // nothing to draw from
+__device__ __forceinline__ unsigned long long race_key(float score, int j) {
+    return static_cast<unsigned long long>(__float_as_uint(score)) << 32 | (0xffffffffu - static_cast<uint32_t>(j));
+}
+
+template <class T>
+__device__ __forceinline__ void write_token(const SampleArgs& a, const RowWords<T>& w, int64_t r, const Request& q,
+                                            float m, unsigned long long best, double kept) {
+    const int j = best ? key_index(best) : -1;
+    a.tokens[r] = j;
+    float lp = NAN;
+    if (q.greedy) {
+        lp = 0.f;
+    } else if (j >= 0) {
+        const float z = Elem<T>::to_f(w.row[j]);
+        lp = static_cast<float>((z == m ? 0. : (static_cast<double>(z) - m) / q.T) - log(kept));
+    }
+    a.logprobs[r] = lp;
+}
+
+// Rank 0, any row: cuts by passes over the whole row, then the race over it.
+template <class T>
+__device__ void sample_wide(SelShared& sh, const SampleArgs& a, const RowWords<T>& w, int64_t r, const Request& q,
+                            const float* noise, float m) {
+    const int tid = threadIdx.x;
+    const Weigh weigh(m, q.T);
+    uint64_t floor = 0;
+    if (q.k < w.V) floor = cut_key<T, false>(w, 0, q.k, weigh, sh.hist, sh.found);
+    if (q.top_p < 1.f) {
+        unsigned long long mass = 0ull;
+        w.template each<4>(0, w.words, tid, kSelThreads, [&](uint4 x, int j0, int) {
+            float v[kRowVec<T>];
+            unpack<T>(x, v);
+#pragma unroll
+            for (int i = 0; i < kRowVec<T>; ++i)
+                if (entry_key(v[i], j0 + i) >= floor) mass += weigh.fixed(v[i]);
+        });
+        mass = block_reduce(mass, AddOp(), 0ull, sh.red64);
+        const double want = ceil(static_cast<double>(q.top_p) * static_cast<double>(mass));
+        floor = cut_key<T, true>(w, floor, want < 1. ? 1ull : static_cast<unsigned long long>(want), weigh, sh.hist,
+                                 sh.found);
+    }
+    unsigned long long best = 0ull;
+    float kept = 0.f;
+    w.template each<4>(0, w.words, tid, kSelThreads, [&](uint4 x, int j0, int) {
+        float v[kRowVec<T>];
+        unpack<T>(x, v);
+#pragma unroll
+        for (int i = 0; i < kRowVec<T>; ++i) {
+            const int j = j0 + i;
+            const float e = weigh(v[i]);
+            if (!(e > 0.f && e >= q.min_p) || entry_key(v[i], j) < floor) continue;
+            kept += e;
+            const float score = e / noise[j];
+            const unsigned long long key = race_key(score, j);
+            if (score >= 0.f && key > best) best = key;
+        }
+    });
+    best = block_reduce(best, MaxOp(), 0ull, sh.red64);
+    const double sum = block_reduce(static_cast<double>(kept), AddOp(), 0., sh.redd);
+    if (tid == 0) write_token(a, w, r, q, m, best, sum);
+}
+
+// Rank 0: the draw among the n largest entries, sorted in sh.list.  `total`: the
+// mass that top_p is a part of, or negative for that of these entries.  False if
+// entries beyond the n may be kept too (then nothing is written).
+template <class T>
+__device__ bool sample_listed(SelShared& sh, const SampleArgs& a, const RowWords<T>& w, int64_t r, const Request& q,
+                              const float* noise, float m, int n, double total, bool complete) {
+    constexpr int MOST = DWA_MAX_TOP / kSelThreads;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const Weigh weigh(m, q.T);
+    const int per = (n + kSelThreads - 1) / kSelThreads;
+    float e[MOST];
+    int j[MOST];
+    double own = 0.;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+        const int k = tid * per + i;
+        e[i] = 0.f;
+        j[i] = -1;
+        if (i < per && k < n) {
+            const unsigned long long key = sh.list[k];
+            e[i] = weigh(unordered(static_cast<uint32_t>(key >> 32)));
+            j[i] = key_index(key);
+        }
+        own += e[i];
+    }
+    double incl = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+    }
+    if (lane == 31) sh.scan[warp] = incl;
+    __syncthreads();
+    double before = incl - own, all = 0.;
+#pragma unroll
+    for (int i = 0; i < kSelThreads / 32; ++i) {
+        if (i < warp) before += sh.scan[i];
+        all += sh.scan[i];
+    }
+    if (total < 0.) total = all;
+    const double limit = q.top_p < 1.f ? q.top_p * total : INFINITY;
+    if (!complete) {
+        const float last = weigh(unordered(static_cast<uint32_t>(sh.list[n - 1] >> 32)));
+        if (!(all >= limit || last < q.min_p || last == 0.f)) return false;   // the same in every thread
+    }
+    unsigned long long best = 0ull;
+    double kept = 0.;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+        if (j[i] >= 0 && e[i] > 0.f && e[i] >= q.min_p && (before < limit || (tid == 0 && i == 0))) {
+            kept += e[i];
+            const float score = q.greedy ? 1.f : e[i] / noise[j[i]];
+            const unsigned long long key = race_key(score, j[i]);
+            if (score >= 0.f && key > best) best = key;
+        }
+        before += e[i];
+    }
+    best = block_reduce(best, MaxOp(), 0ull, sh.red64);
+    kept = block_reduce(kept, AddOp(), 0., sh.redd);
+    if (tid == 0) write_token(a, w, r, q, m, best, kept);
+    return true;
+}
+
+// The whole row races: one pass over its logits and numbers.
+template <class T>
+__device__ __forceinline__ void race_chunk(const RowWords<T>& w, Chunk ch, float c, const float* noise, MaxSum& ms,
+                                           float& top, float& best, int& best_j) {
+    constexpr int VEC = kRowVec<T>;
+    top = -INFINITY;
+    best = 0.f;
+    best_j = -1;
+    w.template each<2>(ch.lo, ch.hi, threadIdx.x, kSelThreads, [&](uint4 x, int j0, int) {
+        const float m = word_max<T>(x);
+        top = max_nan(top, m);
+        if (m > ms.m) {
+            const float f = exp2_fast((ms.m - m) * c);
+            best = f > 0.f ? best * f : 0.f;
+            ms.raise(m, c);
+        }
+        if (ms.m == -INFINITY) return;
+        float e[VEC], score[VEC];
+        word_exp<T>(x, ms.m, c, e);
+        float lead = -1.f;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            ms.s += e[i];
+            score[i] = -1.f;
+            if (e[i] > 0.f) score[i] = __fdividef(e[i], noise[j0 + i]);   // e > 0 only inside the row
+            lead = fmaxf(lead, score[i]);
+        }
+        if (lead > best || best_j < 0) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+                if (score[i] > best || (best_j < 0 && score[i] >= 0.f)) {
+                    best = score[i];
+                    best_j = j0 + i;
+                }
+        }
+    });
+}
+
+template <class T>
+__global__ void __launch_bounds__(kSelThreads, 4) sample_kernel(SampleArgs a) {
+    namespace cg = cooperative_groups;
+    __shared__ SelShared sh;
+    const int P = a.P, tid = threadIdx.x;
+    if (P > 1) cluster_arrive_relaxed();
+    pdl_enter();
+    const int64_t r = blockIdx.x / P;
+    const int p = blockIdx.x % P, V = a.d.V;
+    const RowWords<T> w(static_cast<const T*>(a.z) + row_offset(a.d, r), V);
+    const Request q(a.p, r, V);
+    const float* noise = a.noise + r * a.noise_stride;
+    const float c = kLog2e / q.T;
+    const Chunk ch(w.words, p, P);
+    const bool limited = q.top_p < 1.f || q.min_p > 0.f;
+    MaxSum ms;
+    float m, s;
+    if (q.k == V && !limited) {
+        float top, best;
+        int j;
+        race_chunk(w, ch, c, noise, ms, top, best, j);
+        const float M = block_reduce(ms.m, MaxOp(), -INFINITY, sh.redf);
+        const float S = block_reduce(ms.at(M, c), AddOp(), 0.f, sh.redf);
+        const uint32_t first = block_reduce(ordered(top), MaxOp(), 0u, reinterpret_cast<uint32_t*>(sh.redf));
+        const unsigned long long won =
+            block_reduce(j >= 0 ? race_key(best * exp2_fast((ms.m - M) * c), j) : 0ull, MaxOp(), 0ull, sh.red64);
+        cg::cluster_group cl = cg::this_cluster();
+        if (P > 1) cluster_wait();
+        SelShared* to = P > 1 ? cl.map_shared_rank(&sh, 0) : &sh;
+        if (tid == 0) {
+            to->part_j[p] = static_cast<int>(first);
+            to->part_m[p] = M;
+            to->part_s[p] = S;
+            to->list[p] = won;
+        }
+        if (P > 1) cl.sync();
+        else __syncthreads();
+        if (p != 0) return;
+        row_stats(sh, P, c, m, s);
+        if (fabsf(m) < INFINITY) {
+            if (tid == 0) {
+                unsigned long long best_of = 0ull;
+                for (int i = 0; i < P; ++i) {
+                    unsigned long long x = sh.list[i];
+                    if (!x) continue;
+                    const float score = __uint_as_float(static_cast<uint32_t>(x >> 32)) * exp2_fast((sh.part_m[i] - m) * c);
+                    x = race_key(score, key_index(x));
+                    best_of = x > best_of ? x : best_of;
+                }
+                write_token(a, w, r, q, m, best_of, s);
+            }
+            return;
+        }
+    } else {
+        const bool list = q.k <= DWA_MAX_TOP;
+        const bool masses = !list && q.top_p < 1.f && q.k == V;
+        float top[8], edge;
+        if (masses) scan_chunk<T, true>(w, ch, c, top, edge, ms);
+        else scan_chunk<T, false>(w, ch, c, top, edge, ms);
+        push_groups(sh, p, P, top, edge, ms, c);
+        if (p != 0) return;
+        row_stats(sh, P, c, m, s);
+        if (m > -INFINITY && (list || m < INFINITY)) {
+            if (list || masses || q.top_p >= 1.f) {
+                const int n = list ? q.k : kTryTop;
+                if (list || limited) {
+                    sort_top(sh, w, P, n);
+                    if (sample_listed(sh, a, w, r, q, noise, m, n, masses ? s : -1., list)) return;
+                    __syncthreads();
+                }
+            }
+        }
+    }
+    if (m != m || m == -INFINITY) {   // nothing to draw from
         if (tid == 0) {
             a.tokens[r] = -1;
             a.logprobs[r] = NAN;
         }
         return;
     }
-    const Weigh weigh(ms.m, greedy ? 1.f : T0);
-    uint64_t floor = 0;
-    if (!greedy && top_k > 0 && top_k < V) floor = cut_key<T, false>(w, 0, top_k, weigh, hist, found);
-    if (!greedy && top_p < 1.f) {
-        unsigned long long mass = 0ull;
-        w.template each<4>(0, w.words, tid, blockDim.x, [&](const float* v, int j0) {
-#pragma unroll
-            for (int i = 0; i < kRowVec<T>; ++i)
-                if (entry_key(v[i], j0 + i) >= floor) mass += weigh.fixed(v[i]);
-        });
-        mass = block_reduce(mass, AddOp(), 0ull, red64);
-        const double want = ceil(static_cast<double>(fmaxf(top_p, 0.f)) * static_cast<double>(mass));
-        floor = cut_key<T, true>(w, floor, want < 1. ? 1ull : static_cast<unsigned long long>(want), weigh, hist, found);
-    }
-    const float* noise = a.noise + r * a.noise_stride;
-    unsigned long long best = 0ull;   // score over complement of index
-    float kept = 0.f;
-    w.template each<4>(0, w.words, tid, blockDim.x, [&](const float* v, int j0) {
-#pragma unroll
-        for (int i = 0; i < kRowVec<T>; ++i) {
-            const int j = j0 + i;
-            const float x = weigh(v[i]);
-            if (!(x > 0.f && x >= min_p) || entry_key(v[i], j) < floor || (greedy && x < 1.f)) continue;
-            kept += x;
-            const float score = greedy ? 1.f : x / noise[j];
-            const unsigned long long key = static_cast<unsigned long long>(__float_as_uint(score)) << 32 |
-                                           (0xffffffffu - static_cast<uint32_t>(j));
-            if (score >= 0.f && key > best) best = key;
-        }
-    });
-    best = block_reduce(best, MaxOp(), 0ull, red64);
-    kept = block_reduce(kept, AddOp(), 0.f, red);
-    if (tid == 0) {
-        const int j = best ? key_index(best) : -1;
-        a.tokens[r] = j;
-        float lp = NAN;
-        if (greedy) {
-            lp = 0.f;
-        } else if (j >= 0) {
-            const float z = Elem<T>::to_f(w.row[j]);
-            lp = (z == ms.m ? 0.f : (z - ms.m) / T0) - logf(kept);
-        }
-        a.logprobs[r] = lp;
-    }
+    sample_wide(sh, a, w, r, q, noise, m);
+}
+
+// CTAs per row: while the launch has room on the GPU (four CTAs an SM) and each
+// CTA at least a word a thread.
+static int ctas_per_row(const DwaLogitsDims& d) {
+    const int64_t room = 4 * static_cast<int64_t>(tc::sm_count());
+    const int words = d.V / (16 / static_cast<int>(dtype_bytes(d.dtype)));
+    int P = kSelMaxCluster;
+    while (P > 1 && (d.rows * P > room || words < P * kSelThreads)) P /= 2;
+    return P;
+}
+
+template <class K, class A>
+static cudaError_t launch_rows(K kernel, const A& a, cudaStream_t st) {
+    const dim3 grid(static_cast<unsigned>(a.d.rows * a.P));
+    return a.P > 1 ? launch_pdl_cluster(kernel, grid, dim3(kSelThreads), 0, st, dim3(a.P), a)
+                   : launch_pdl(kernel, grid, dim3(kSelThreads), 0, st, a);
 }
 
 }  // namespace dwa
@@ -298,13 +713,10 @@ extern "C" int dwa_top_logits(void* stream, const DwaLogitsDims* dims, const voi
     if (reinterpret_cast<uintptr_t>(logits) % dtype_bytes(dims->dtype) ||
         reinterpret_cast<uintptr_t>(values) % dtype_bytes(dims->dtype))
         return fail(DWA_ERR_INVALID_ARG, "top_logits: a pointer is not aligned to its element");
-    const TopArgs a = {logits, *dims, K, kLog2e / temperature, temperature, values, indices, lse};
+    const TopArgs a = {logits, *dims, K, ctas_per_row(*dims), kLog2e / temperature, temperature, values, indices, lse};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const dim3 grid(static_cast<unsigned>(dims->rows));
-    if (dims->dtype == DWA_BF16)
-        DWA_TIMED("top_logits", st, (launch_pdl(top_logits_kernel<__nv_bfloat16>, grid, dim3(kSelThreads), 0, st, a)));
-    else
-        DWA_TIMED("top_logits", st, (launch_pdl(top_logits_kernel<float>, grid, dim3(kSelThreads), 0, st, a)));
+    if (dims->dtype == DWA_BF16) DWA_TIMED("top_logits", st, (launch_rows(top_logits_kernel<__nv_bfloat16>, a, st)));
+    else DWA_TIMED("top_logits", st, (launch_rows(top_logits_kernel<float>, a, st)));
     DWA_LAUNCH_CHECK("top_logits_kernel");
     ++g_launches_total;
     return DWA_OK;
@@ -322,13 +734,10 @@ extern "C" int dwa_sample_tokens(void* stream, const DwaLogitsDims* dims, const 
         return fail(DWA_ERR_INVALID_ARG, "sample_tokens: a required pointer is NULL");
     if (reinterpret_cast<uintptr_t>(logits) % dtype_bytes(dims->dtype) || reinterpret_cast<uintptr_t>(noise) % 4)
         return fail(DWA_ERR_INVALID_ARG, "sample_tokens: a pointer is not aligned to its element");
-    const SampleArgs a = {logits, *dims, noise, noise_stride, *params, tokens, logprobs};
+    const SampleArgs a = {logits, *dims, noise, noise_stride, *params, ctas_per_row(*dims), tokens, logprobs};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const dim3 grid(static_cast<unsigned>(dims->rows));
-    if (dims->dtype == DWA_BF16)
-        DWA_TIMED("sample", st, (launch_pdl(sample_kernel<__nv_bfloat16>, grid, dim3(kSelThreads), 0, st, a)));
-    else
-        DWA_TIMED("sample", st, (launch_pdl(sample_kernel<float>, grid, dim3(kSelThreads), 0, st, a)));
+    if (dims->dtype == DWA_BF16) DWA_TIMED("sample", st, (launch_rows(sample_kernel<__nv_bfloat16>, a, st)));
+    else DWA_TIMED("sample", st, (launch_rows(sample_kernel<float>, a, st)));
     DWA_LAUNCH_CHECK("sample_kernel");
     ++g_launches_total;
     return DWA_OK;

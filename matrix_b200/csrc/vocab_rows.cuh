@@ -54,6 +54,70 @@ __device__ __forceinline__ uint4 pack(const float* v) {
     }
 }
 
+// 2^x by the hardware's approximation (relative error 2^-22, results below 2^-126
+// are 0): the weights that sum to a row's total need no more.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The larger of two, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// The largest value of a word, NaN if one is there.
+template <class T>
+__device__ __forceinline__ float word_max(uint4 w) {
+    if constexpr (sizeof(T) == 2) {
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+        const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+        return max_nan(__low2float(m), __high2float(m));
+    } else {
+        float v[4];
+        unpack<T>(w, v);
+        return max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3]));
+    }
+}
+
+// Pairs of floats in one 64-bit register: one instruction for two lanes.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// e[i] = exp2((v[i] - m) * c) of one word
+template <class T>
+__device__ __forceinline__ void word_exp(uint4 w, float m, float c, float* e) {
+    float v[kRowVec<T>];
+    unpack<T>(w, v);
+    const uint64_t nm = pair(-m, -m), cc = pair(c, c);
+#pragma unroll
+    for (int i = 0; i < kRowVec<T>; i += 2) {
+        float a, b;
+        unpair(mul2(add2(pair(v[i], v[i + 1]), nm), cc), a, b);
+        e[i] = exp2_fast(a);
+        e[i + 1] = exp2_fast(b);
+    }
+}
+
 // The words of one row.
 template <class T>
 struct RowWords {
@@ -68,48 +132,45 @@ struct RowWords {
         full_hi = (V + shift) / VEC;
     }
     __device__ __forceinline__ int first(int g) const { return g * kRowVec<T> - shift; }
+    __device__ __forceinline__ bool whole(int g) const { return g >= full_lo && g < full_hi; }
     __device__ __forceinline__ uint4 word(int g) const { return *reinterpret_cast<const uint4*>(row + first(g)); }
-    // a first or last word: -inf outside the row
-    __device__ __forceinline__ void edge(int g, float* v) const {
+    // f(word, its first index) for a row's first and last word where they are not
+    // whole (threads 0 and 1); -inf stands outside the row
+    template <class F>
+    __device__ __forceinline__ void edges(int lo, int hi, int tid, F f) const {
+        if (tid > 1) return;
+        const int g = tid == 0 ? 0 : words - 1;
+        if (whole(g) || (tid == 1 && words == 1) || g < lo || g >= hi) return;
+        float v[kRowVec<T>];
 #pragma unroll
         for (int i = 0; i < kRowVec<T>; ++i) {
             const int j = first(g) + i;
             v[i] = (j >= 0 && j < V) ? Elem<T>::to_f(row[j]) : -INFINITY;
         }
+        f(pack<T>(v), first(g));
     }
-
-    // f(v, j0) for every word of [lo, hi) in this thread's share (threads tid of
-    // n): the word's VEC values and its first index.  U words are in flight.
+    // f(word, its first index, u) for the whole ones of the words lo + tid,
+    // lo + tid + n, ... below hi; the u-th, (u + U)-th, ... word of a thread come
+    // with the same u.  U words are in flight.
     template <int U, class F>
-    __device__ __forceinline__ void each(int lo, int hi, int tid, int n, F f) const {
-        constexpr int VEC = kRowVec<T>;
+    __device__ __forceinline__ void each_whole(int lo, int hi, int tid, int n, F f) const {
         const int a = lo > full_lo ? lo : full_lo, b = hi < full_hi ? hi : full_hi;
-        int g = a + tid;
-        for (; g + (U - 1) * n < b; g += U * n) {
+        for (int g = lo + tid; g < b; g += U * n) {
+            const uint4* p = reinterpret_cast<const uint4*>(row + first(g));
             uint4 w[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) w[u] = word(g + u * n);
+            for (int u = 0; u < U; ++u)
+                if (g + u * n >= a && g + u * n < b) w[u] = p[u * n];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                float v[VEC];
-                unpack<T>(w[u], v);
-                f(v, first(g + u * n));
-            }
+            for (int u = 0; u < U; ++u)
+                if (g + u * n >= a && g + u * n < b) f(w[u], first(g + u * n), u);
         }
-        for (; g < b; g += n) {
-            float v[VEC];
-            unpack<T>(word(g), v);
-            f(v, first(g));
-        }
-        if (tid < 2) {   // thread 0 the first word, thread 1 the last, where they are not whole
-            const int e = tid == 0 ? 0 : words - 1;
-            const bool is_edge = tid == 0 ? full_lo > 0 : (full_hi < words && words - 1 >= full_lo);
-            if (is_edge && e >= lo && e < hi) {
-                float v[VEC];
-                edge(e, v);
-                f(v, first(e));
-            }
-        }
+    }
+    // every word; u is -1 on the edges
+    template <int U, class F>
+    __device__ __forceinline__ void each(int lo, int hi, int tid, int n, F f) const {
+        each_whole<U>(lo, hi, tid, n, f);
+        edges(lo, hi, tid, [&](uint4 x, int j0) { f(x, j0, -1); });
     }
 };
 
@@ -143,12 +204,14 @@ struct AddOp {
 // The running maximum and sum of exp2((v - m) * c): one pass over the data.
 struct MaxSum {
     float m = -INFINITY, s = 0.f;
-    __device__ __forceinline__ void raise(float to, float c) {   // m becomes `to` >= m
+    __device__ __forceinline__ void raise(float to, float c) {   // m becomes `to` if that is larger
         if (to > m) {
-            s *= exp2f((m - to) * c);   // m = -inf: s is 0 and stays 0
+            s *= exp2_fast((m - to) * c);   // m = -inf: s is 0 and stays 0
             m = to;
         }
     }
+    // the sum once the maximum of all is M
+    __device__ __forceinline__ float at(float M, float c) const { return m > -INFINITY ? s * exp2_fast((m - M) * c) : s; }
 };
 
 int check_logits(const DwaLogitsDims* d, const char* what);   // distill.cu
