@@ -13,9 +13,8 @@
 // largest w_i / e_i (an exponential race, which draws i with probability
 // w_i / sum w), its log-probability log(w_i / sum of the kept w).
 //
-// Masses that decide a cut are summed as integers in units of 2^-31 of the
-// largest weight: sums that no order of additions changes, so a row's token does
-// not depend on how its entries are spread over threads.
+// A cut by mass through a long row is found with sums of whole units of 2^-36 of
+// the largest weight, which no order of additions changes.
 
 #include <atomic>
 
@@ -30,6 +29,9 @@ constexpr int kSelGroups = 8 * kSelThreads;   // groups of words whose maxima ar
 constexpr int kSelList = 2048;                // candidates held
 constexpr int kTryTop = 256;                  // entries sorted first when only a mass or a floor limits the row
 constexpr int kSelMaxCluster = 8;
+constexpr int kBins = 2048;                   // bins of a wide cut: 32 octaves of weight, 64 bins each, at first
+constexpr float kUnit = 262144.f;             // 2^18: a weight is 2^36 units, in two parts of 18 bits
+constexpr int kDrain = 8192;                  // entries after which a bin's 32-bit parts are emptied: 2^13 * 2^18
 
 // A logit as an unsigned integer of the same order.
 __device__ __forceinline__ uint32_t ordered(float z) {
@@ -51,21 +53,32 @@ struct Weigh {
         c = static_cast<float>(cd);
         c_lo = isinf(c) ? 0.f : static_cast<float>(cd - c);
     }
-    __device__ __forceinline__ float operator()(float z) const {
-        if (z == m) return 1.f;
+    // log2 of the weight: 0 at the maximum, -inf for what has none
+    __device__ __forceinline__ float log2_of(float z) const {
         const float d = z - m;
-        return z == -INFINITY || m == INFINITY ? 0.f : exp2f(fmaf(d, c, d * c_lo));
+        return z == m ? 0.f : z == -INFINITY || m == INFINITY ? -INFINITY : fmaf(d, c, d * c_lo);
     }
-    // in units of 2^-31
-    __device__ __forceinline__ uint32_t fixed(float z) const { return static_cast<uint32_t>((*this)(z) * 2147483648.f + 0.5f); }
+    __device__ __forceinline__ float operator()(float z) const { return exp2_fast(log2_of(z)); }
 };
 
-// The key at which the entries at or above `floor`, taken in descending order,
-// reach `target`: in number (MASS = false) or in mass.  Eight bits of the key a
+// An entry's measure: 1, or its weight in units of 2^-36 of the largest; in two
+// parts of 18 bits (and one bit more when they round up).
+template <bool MASS>
+__device__ __forceinline__ void measure(float log2_w, uint32_t& hi, uint32_t& lo) {
+    if constexpr (MASS) {
+        const float x = exp2_fast(log2_w) * kUnit;
+        hi = static_cast<uint32_t>(x);
+        lo = static_cast<uint32_t>(rintf((x - static_cast<float>(hi)) * kUnit));
+    } else {
+        hi = 0u;
+        lo = 1u;
+    }
+}
+
+// The `target`-th largest key of a row by one block, eight bits of the key a
 // pass.  hist: 256 values, found: 2 values in shared memory.
-template <class T, bool MASS>
-__device__ uint64_t cut_key(const RowWords<T>& w, uint64_t floor, uint64_t target, const Weigh& weigh,
-                            unsigned long long* hist, unsigned long long* found) {
+template <class T>
+__device__ uint64_t cut_key(const RowWords<T>& w, uint64_t target, unsigned long long* hist, unsigned long long* found) {
     const int tid = threadIdx.x, lane = tid & 31;
     uint64_t prefix = 0, mask = 0;
     int index_bytes = 1;
@@ -86,18 +99,10 @@ __device__ uint64_t cut_key(const RowWords<T>& w, uint64_t floor, uint64_t targe
 #pragma unroll
             for (int i = 0; i < kRowVec<T>; ++i) {
                 const uint64_t key = entry_key(v[i], j0 + i);
-                if (static_cast<unsigned>(j0 + i) < static_cast<unsigned>(w.V) && key >= floor && (key & mask) == prefix) {
+                if (static_cast<unsigned>(j0 + i) < static_cast<unsigned>(w.V) && (key & mask) == prefix) {
                     const uint32_t digit = static_cast<uint32_t>(key >> shift) & 0xffu;
                     const unsigned peers = __match_any_sync(__activemask(), digit);
-                    unsigned long long sum;
-                    if (MASS) {
-                        const uint32_t units = weigh.fixed(v[i]);
-                        sum = (static_cast<unsigned long long>(__reduce_add_sync(peers, units >> 16)) << 16) +
-                              __reduce_add_sync(peers, units & 0xffffu);
-                    } else {
-                        sum = __popc(peers);
-                    }
-                    if ((peers & ((1u << lane) - 1u)) == 0u) atomicAdd(&hist[digit], sum);
+                    if ((peers & ((1u << lane) - 1u)) == 0u) atomicAdd(&hist[digit], static_cast<unsigned long long>(__popc(peers)));
                 }
             }
         });
@@ -143,9 +148,15 @@ struct SelShared {
     union {
         uint32_t group[kSelGroups];
         unsigned long long hist[256];
+        uint32_t bin[2][kBins];          // high and low part of a bin's measure
     };
-    unsigned long long list[kSelList];   // candidates; sorted: the K largest in descending order
+    union {
+        unsigned long long list[kSelList];   // candidates; sorted: the K largest in descending order
+        unsigned long long sum[kBins];       // the bins' measure so far
+    };
     uint16_t chosen[kSelGroups];
+    unsigned long long part_lo[kSelMaxCluster], part_hi[kSelMaxCluster];
+    unsigned long long told[4];          // what rank 0 tells the cluster
     float part_m[kSelMaxCluster], part_s[kSelMaxCluster], part_b[kSelMaxCluster];
     int part_j[kSelMaxCluster];
     uint32_t warp_count[2][kSelThreads / 32];
@@ -238,6 +249,36 @@ __device__ __forceinline__ void row_stats(const SelShared& sh, int P, float c, f
     for (int p = 0; p < P; ++p) s += sh.part_m[p] > -INFINITY ? sh.part_s[p] * exp2_fast((sh.part_m[p] - m) * c) : 0.f;
 }
 
+// The first n <= kSelList keys of sh.list into descending order.
+__device__ void sort_list(SelShared& sh, int n) {
+    const int tid = threadIdx.x;
+    if (n <= kSelThreads) {   // each key to its rank
+        const unsigned long long key = tid < n ? sh.list[tid] : 0ull;
+        int rank = 0;
+        for (int i = 0; i < n; ++i) rank += sh.list[i] > key;
+        __syncthreads();
+        if (tid < n) sh.list[rank] = key;
+    } else {                  // bitonic, padded to a power of two
+        int size = 2 * kSelThreads;
+        while (size < n) size <<= 1;
+        for (int i = n + tid; i < size; i += kSelThreads) sh.list[i] = 0ull;
+        for (int k = 2; k <= size; k <<= 1) {
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                __syncthreads();
+                for (int i = tid; i < size / 2; i += kSelThreads) {
+                    const int a = (i / j) * 2 * j + i % j, b = a + j;
+                    const unsigned long long x = sh.list[a], y = sh.list[b];
+                    if ((x < y) == ((a & k) == 0)) {
+                        sh.list[a] = y;
+                        sh.list[b] = x;
+                    }
+                }
+            }
+        }
+    }
+    __syncthreads();
+}
+
 // Rank 0: the K largest entries of the row into sh.list, in descending order.
 template <class T>
 __device__ void sort_top(SelShared& sh, const RowWords<T>& w, int P, int K) {
@@ -316,7 +357,7 @@ __device__ void sort_top(SelShared& sh, const RowWords<T>& w, int P, int K) {
     __syncthreads();
     int n = sh.n_list;
     if (n > kSelList) {   // equal or ordered entries crowd the groups: find the K-th key itself
-        const uint64_t cut = cut_key<T, false>(w, 0, K, Weigh(0.f, 1.f), sh.hist, sh.found);
+        const uint64_t cut = cut_key(w, K, sh.hist, sh.found);
         if (tid == 0) sh.n_list = 0;
         __syncthreads();
         w.template each<4>(0, w.words, tid, kSelThreads, [&](uint4 x, int j0, int) {
@@ -332,31 +373,7 @@ __device__ void sort_top(SelShared& sh, const RowWords<T>& w, int P, int K) {
         __syncthreads();
         n = K;
     }
-    if (n <= kSelThreads) {   // each key to its rank
-        const unsigned long long key = tid < n ? sh.list[tid] : 0ull;
-        int rank = 0;
-        for (int i = 0; i < n; ++i) rank += sh.list[i] > key;
-        __syncthreads();
-        if (tid < n) sh.list[rank] = key;
-    } else {                  // bitonic, padded to a power of two
-        int size = 2 * kSelThreads;
-        while (size < n) size <<= 1;
-        for (int i = n + tid; i < size; i += kSelThreads) sh.list[i] = 0ull;
-        for (int k = 2; k <= size; k <<= 1) {
-            for (int j = k >> 1; j > 0; j >>= 1) {
-                __syncthreads();
-                for (int i = tid; i < size / 2; i += kSelThreads) {
-                    const int a = (i / j) * 2 * j + i % j, b = a + j;
-                    const unsigned long long x = sh.list[a], y = sh.list[b];
-                    if ((x < y) == ((a & k) == 0)) {
-                        sh.list[a] = y;
-                        sh.list[b] = x;
-                    }
-                }
-            }
-        }
-    }
-    __syncthreads();
+    sort_list(sh, n);
 }
 
 struct TopArgs {
@@ -452,47 +469,249 @@ __device__ __forceinline__ void write_token(const SampleArgs& a, const RowWords<
     a.logprobs[r] = lp;
 }
 
-// Rank 0, any row: cuts by passes over the whole row, then the race over it.
-template <class T>
-__device__ void sample_wide(SelShared& sh, const SampleArgs& a, const RowWords<T>& w, int64_t r, const Request& q,
-                            const float* noise, float m) {
-    const int tid = threadIdx.x;
-    const Weigh weigh(m, q.T);
-    uint64_t floor = 0;
-    if (q.k < w.V) floor = cut_key<T, false>(w, 0, q.k, weigh, sh.hist, sh.found);
-    if (q.top_p < 1.f) {
-        unsigned long long mass = 0ull;
-        w.template each<4>(0, w.words, tid, kSelThreads, [&](uint4 x, int j0, int) {
-            float v[kRowVec<T>];
+// Tells every CTA of the cluster four values of rank 0's; a cluster barrier.
+__device__ __forceinline__ void tell(SelShared& sh, int P, int p, uint64_t a, uint64_t b, uint64_t c, uint64_t d) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cl = cg::this_cluster();
+    if (p == 0 && static_cast<int>(threadIdx.x) < P) {
+        unsigned long long* t = cl.map_shared_rank(sh.told, threadIdx.x);
+        t[0] = a;
+        t[1] = b;
+        t[2] = c;
+        t[3] = d;
+    }
+    cl.sync();
+}
+
+// The whole cluster: the key at which the entries at or above `floor`, taken in
+// descending order, reach `target` in number or, with MASS, the part top_p of
+// their mass.  A histogram of the measure finds the bin of the cut and what lies
+// above it; the bin's entries go to rank 0, which sorts them and walks to the
+// cut.  Bins are even in the logarithm of the weight; where one holds more than
+// can be sorted (equal logits), the bins of the next round divide its keys.
+// All sums are whole numbers, so no order of additions shows in the result.
+template <class T, bool MASS>
+__device__ uint64_t wide_cut(SelShared& sh, const RowWords<T>& w, Chunk ch, int p, int P, const Weigh& weigh,
+                             uint64_t floor, uint64_t target, float top_p) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cl = cg::this_cluster();
+    constexpr int VEC = kRowVec<T>, PER = kBins / kSelThreads;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint64_t key_lo = floor, key_hi = ~uint64_t(0);   // the cut lies in here
+    int shift = -1;                                   // < 0: bins of the logarithm of the weight
+    for (;;) {
+        const auto bin_of = [&](uint64_t key, float log2_w) {
+            return shift < 0 ? static_cast<int>(fminf(log2_w * -64.f, kBins - 1.f))
+                             : static_cast<int>((key_hi - key) >> shift);
+        };
+        // the histogram of this CTA's share
+        __syncthreads();
+        for (int i = tid; i < kBins; i += kSelThreads) {
+            sh.bin[0][i] = sh.bin[1][i] = 0u;
+            sh.sum[i] = 0ull;
+        }
+        __syncthreads();
+        for (int a = ch.lo; a < ch.hi; a += kDrain / VEC) {
+            const int b = a + kDrain / VEC < ch.hi ? a + kDrain / VEC : ch.hi;
+            w.template each<2>(a, b, tid, kSelThreads, [&](uint4 x, int j0, int) {
+                float v[VEC];
+                unpack<T>(x, v);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const uint64_t key = entry_key(v[i], j0 + i);
+                    if (key < key_lo || key > key_hi || static_cast<unsigned>(j0 + i) >= static_cast<unsigned>(w.V)) continue;
+                    const float l = weigh.log2_of(v[i]);
+                    uint32_t hi, lo;
+                    measure<MASS>(l, hi, lo);
+                    const int at = bin_of(key, l);
+                    if (hi) atomicAdd(&sh.bin[0][at], hi);
+                    if (lo) atomicAdd(&sh.bin[1][at], lo);
+                }
+            });
+            __syncthreads();
+            for (int i = tid; i < kBins; i += kSelThreads) {
+                sh.sum[i] += (static_cast<unsigned long long>(sh.bin[0][i]) << 18) + sh.bin[1][i];
+                sh.bin[0][i] = sh.bin[1][i] = 0u;
+            }
+            __syncthreads();
+        }
+        cl.sync();
+        // rank 0: the bin of the cut
+        if (p == 0) {
+            unsigned long long v[PER], own = 0ull;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) v[i] = 0ull;
+            for (int q = 0; q < P; ++q) {
+                const unsigned long long* from = cl.map_shared_rank(sh.sum, q) + tid * PER;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) v[i] += from[i];
+            }
+#pragma unroll
+            for (int i = 0; i < PER; ++i) own += v[i];
+            unsigned long long incl = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned long long up = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += up;
+            }
+            if (lane == 31) sh.red64[warp] = incl;
+            __syncthreads();
+            unsigned long long all = 0ull, acc = incl - own;
+#pragma unroll
+            for (int i = 0; i < kSelThreads / 32; ++i) {
+                if (i < warp) acc += sh.red64[i];
+                all += sh.red64[i];
+            }
+            if (MASS && target == 0) {
+                const double want = ceil(static_cast<double>(top_p) * static_cast<double>(all));
+                target = want < 1. ? 1ull : static_cast<unsigned long long>(want);
+            }
+            if (acc < target && target <= acc + own) {   // one thread
+                int i = 0;
+#pragma unroll
+                for (int k = 0; k < PER - 1; ++k)
+                    if (i == k && acc + v[k] < target) {
+                        acc += v[k];
+                        i = k + 1;
+                    }
+                sh.found[0] = static_cast<unsigned long long>(tid * PER + i);
+                sh.found[1] = acc;
+            }
+            if (tid == 0) sh.n_list = 0;
+            __syncthreads();
+        }
+        tell(sh, P, p, sh.found[0], target, sh.found[1], 0);
+        const int cut_bin = static_cast<int>(sh.told[0]);
+        target = sh.told[1] - sh.told[2];   // what is left to reach inside the bin
+        // its entries to rank 0
+        SelShared* to = cl.map_shared_rank(&sh, 0);
+        unsigned long long least = ~0ull, most = 0ull;
+        w.template each<2>(ch.lo, ch.hi, tid, kSelThreads, [&](uint4 x, int j0, int) {
+            float v[VEC];
             unpack<T>(x, v);
 #pragma unroll
-            for (int i = 0; i < kRowVec<T>; ++i)
-                if (entry_key(v[i], j0 + i) >= floor) mass += weigh.fixed(v[i]);
+            for (int i = 0; i < VEC; ++i) {
+                const unsigned long long key = entry_key(v[i], j0 + i);
+                if (key < key_lo || key > key_hi || static_cast<unsigned>(j0 + i) >= static_cast<unsigned>(w.V) ||
+                    bin_of(key, weigh.log2_of(v[i])) != cut_bin)
+                    continue;
+                least = key < least ? key : least;
+                most = key > most ? key : most;
+                const int at = atomicAdd(&to->n_list, 1);
+                if (at < kSelList) to->list[at] = key;
+            }
         });
-        mass = block_reduce(mass, AddOp(), 0ull, sh.red64);
-        const double want = ceil(static_cast<double>(q.top_p) * static_cast<double>(mass));
-        floor = cut_key<T, true>(w, floor, want < 1. ? 1ull : static_cast<unsigned long long>(want), weigh, sh.hist,
-                                 sh.found);
+        least = ~block_reduce(~least, MaxOp(), 0ull, sh.red64);
+        most = block_reduce(most, MaxOp(), 0ull, sh.red64);
+        if (tid == 0) {
+            to->part_lo[p] = least;
+            to->part_hi[p] = most;
+        }
+        cl.sync();
+        if (p == 0) {
+            const int n = sh.n_list;
+            if (n <= kSelList) {
+                sort_list(sh, n);
+                constexpr int MOST = kSelList / kSelThreads;
+                const int per = (n + kSelThreads - 1) / kSelThreads;
+                unsigned long long own = 0ull, u[MOST];
+#pragma unroll
+                for (int i = 0; i < MOST; ++i) {
+                    u[i] = 0ull;
+                    if (i < per && tid * per + i < n) {
+                        uint32_t hi, lo;
+                        measure<MASS>(weigh.log2_of(unordered(static_cast<uint32_t>(sh.list[tid * per + i] >> 32))), hi, lo);
+                        u[i] = (static_cast<unsigned long long>(hi) << 18) + lo;
+                    }
+                    own += u[i];
+                }
+                unsigned long long incl = own;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned long long up = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += up;
+                }
+                if (lane == 31) sh.red64[warp] = incl;
+                __syncthreads();
+                unsigned long long acc = incl - own;
+                for (int i = 0; i < warp; ++i) acc += sh.red64[i];
+                if (acc < target && target <= acc + own) {
+#pragma unroll
+                    for (int i = 0; i < MOST; ++i) {
+                        if (acc < target && acc + u[i] >= target) sh.found[0] = sh.list[tid * per + i];
+                        acc += u[i];
+                    }
+                }
+                sh.found[1] = 1ull;
+            } else {
+                sh.found[1] = 0ull;
+            }
+            __syncthreads();
+        }
+        least = ~0ull;
+        most = 0ull;
+        if (p == 0) {
+            for (int q = 0; q < P; ++q) {
+                least = sh.part_lo[q] < least ? sh.part_lo[q] : least;
+                most = sh.part_hi[q] > most ? sh.part_hi[q] : most;
+            }
+        }
+        tell(sh, P, p, sh.found[0], sh.found[1], least, most);
+        if (sh.told[1]) return sh.told[0];
+        key_lo = sh.told[2];
+        key_hi = sh.told[3];
+        shift = 0;
+        while ((key_hi - key_lo) >> shift >= kBins) ++shift;
     }
+}
+
+// The whole cluster, any row with a finite maximum or +inf: the cuts, then the
+// race over what stays.
+template <class T>
+__device__ void sample_wide(SelShared& sh, const SampleArgs& a, const RowWords<T>& w, Chunk ch, int p, int64_t r,
+                            const Request& q, const float* noise, float m) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cl = cg::this_cluster();
+    const int tid = threadIdx.x, P = a.P;
+    const Weigh weigh(m, q.T);
+    uint64_t floor = 0;
+    if (q.k < w.V) floor = wide_cut<T, false>(sh, w, ch, p, P, weigh, floor, q.k, 1.f);
+    if (q.top_p < 1.f) floor = wide_cut<T, true>(sh, w, ch, p, P, weigh, floor, 0, q.top_p);
+    const float fz = floor ? unordered(static_cast<uint32_t>(floor >> 32)) : -INFINITY;
+    const int fj = floor ? key_index(floor) : w.V;
     unsigned long long best = 0ull;
     float kept = 0.f;
-    w.template each<4>(0, w.words, tid, kSelThreads, [&](uint4 x, int j0, int) {
+    w.template each<4>(ch.lo, ch.hi, tid, kSelThreads, [&](uint4 x, int j0, int) {
         float v[kRowVec<T>];
         unpack<T>(x, v);
 #pragma unroll
         for (int i = 0; i < kRowVec<T>; ++i) {
             const int j = j0 + i;
             const float e = weigh(v[i]);
-            if (!(e > 0.f && e >= q.min_p) || entry_key(v[i], j) < floor) continue;
+            if (!(v[i] > fz || (v[i] == fz && j <= fj)) || !(e > 0.f && e >= q.min_p)) continue;
             kept += e;
-            const float score = e / noise[j];
+            const float score = __fdividef(e, noise[j]);
             const unsigned long long key = race_key(score, j);
             if (score >= 0.f && key > best) best = key;
         }
     });
     best = block_reduce(best, MaxOp(), 0ull, sh.red64);
     const double sum = block_reduce(static_cast<double>(kept), AddOp(), 0., sh.redd);
-    if (tid == 0) write_token(a, w, r, q, m, best, sum);
+    SelShared* to = cl.map_shared_rank(&sh, 0);
+    if (tid == 0) {
+        to->part_lo[p] = best;
+        to->part_hi[p] = __double_as_longlong(sum);
+    }
+    cl.sync();
+    if (p == 0 && tid == 0) {
+        double all = 0.;
+        best = 0ull;
+        for (int i = 0; i < P; ++i) {
+            best = sh.part_lo[i] > best ? sh.part_lo[i] : best;
+            all += __longlong_as_double(sh.part_hi[i]);
+        }
+        write_token(a, w, r, q, m, best, all);
+    }
 }
 
 // Rank 0: the draw among the n largest entries, sorted in sh.list.  `total`: the
@@ -611,9 +830,11 @@ __global__ void __launch_bounds__(kSelThreads, 4) sample_kernel(SampleArgs a) {
     const float c = kLog2e / q.T;
     const Chunk ch(w.words, p, P);
     const bool limited = q.top_p < 1.f || q.min_p > 0.f;
+    const bool whole = q.k == V && !limited, list = !whole && q.k <= DWA_MAX_TOP;
     MaxSum ms;
     float m, s;
-    if (q.k == V && !limited) {
+    bool done = false;
+    if (whole) {
         float top, best;
         int j;
         race_chunk(w, ch, c, noise, ms, top, best, j);
@@ -622,61 +843,59 @@ __global__ void __launch_bounds__(kSelThreads, 4) sample_kernel(SampleArgs a) {
         const uint32_t first = block_reduce(ordered(top), MaxOp(), 0u, reinterpret_cast<uint32_t*>(sh.redf));
         const unsigned long long won =
             block_reduce(j >= 0 ? race_key(best * exp2_fast((ms.m - M) * c), j) : 0ull, MaxOp(), 0ull, sh.red64);
-        cg::cluster_group cl = cg::this_cluster();
         if (P > 1) cluster_wait();
-        SelShared* to = P > 1 ? cl.map_shared_rank(&sh, 0) : &sh;
+        SelShared* to = cg::this_cluster().map_shared_rank(&sh, 0);
         if (tid == 0) {
             to->part_j[p] = static_cast<int>(first);
             to->part_m[p] = M;
             to->part_s[p] = S;
-            to->list[p] = won;
+            to->part_lo[p] = won;
         }
-        if (P > 1) cl.sync();
-        else __syncthreads();
-        if (p != 0) return;
-        row_stats(sh, P, c, m, s);
-        if (fabsf(m) < INFINITY) {
-            if (tid == 0) {
+        cg::this_cluster().sync();
+        if (p == 0) {
+            row_stats(sh, P, c, m, s);
+            done = fabsf(m) < INFINITY;
+            if (done && tid == 0) {
                 unsigned long long best_of = 0ull;
                 for (int i = 0; i < P; ++i) {
-                    unsigned long long x = sh.list[i];
+                    unsigned long long x = sh.part_lo[i];
                     if (!x) continue;
-                    const float score = __uint_as_float(static_cast<uint32_t>(x >> 32)) * exp2_fast((sh.part_m[i] - m) * c);
-                    x = race_key(score, key_index(x));
+                    x = race_key(__uint_as_float(static_cast<uint32_t>(x >> 32)) * exp2_fast((sh.part_m[i] - m) * c),
+                                 key_index(x));
                     best_of = x > best_of ? x : best_of;
                 }
                 write_token(a, w, r, q, m, best_of, s);
             }
-            return;
         }
     } else {
-        const bool list = q.k <= DWA_MAX_TOP;
         const bool masses = !list && q.top_p < 1.f && q.k == V;
         float top[8], edge;
         if (masses) scan_chunk<T, true>(w, ch, c, top, edge, ms);
         else scan_chunk<T, false>(w, ch, c, top, edge, ms);
         push_groups(sh, p, P, top, edge, ms, c);
-        if (p != 0) return;
-        row_stats(sh, P, c, m, s);
-        if (m > -INFINITY && (list || m < INFINITY)) {
-            if (list || masses || q.top_p >= 1.f) {
+        if (p == 0) {
+            row_stats(sh, P, c, m, s);
+            // a mass relative to +inf, or of the k largest of many, is not at hand
+            if (m > -INFINITY && (list || (m < INFINITY && (masses || q.top_p >= 1.f) && limited))) {
                 const int n = list ? q.k : kTryTop;
-                if (list || limited) {
-                    sort_top(sh, w, P, n);
-                    if (sample_listed(sh, a, w, r, q, noise, m, n, masses ? s : -1., list)) return;
-                    __syncthreads();
-                }
+                sort_top(sh, w, P, n);
+                done = sample_listed(sh, a, w, r, q, noise, m, n, masses ? s : -1., list);
             }
         }
+        if (list && p != 0) return;
     }
-    if (m != m || m == -INFINITY) {   // nothing to draw from
+    if (p == 0 && !done && !(m > -INFINITY)) {   // NaN or nothing to draw from
         if (tid == 0) {
             a.tokens[r] = -1;
             a.logprobs[r] = NAN;
         }
-        return;
+        done = true;
     }
-    sample_wide(sh, a, w, r, q, noise, m);
+    if (list) return;
+    tell(sh, P, p, done, __float_as_uint(m), 0, 0);
+    if (sh.told[0]) return;
+    m = __uint_as_float(static_cast<uint32_t>(sh.told[1]));
+    sample_wide(sh, a, w, ch, p, r, q, noise, m);
 }
 
 // CTAs per row: while the launch has room on the GPU (four CTAs an SM) and each
@@ -692,8 +911,7 @@ static int ctas_per_row(const DwaLogitsDims& d) {
 template <class K, class A>
 static cudaError_t launch_rows(K kernel, const A& a, cudaStream_t st) {
     const dim3 grid(static_cast<unsigned>(a.d.rows * a.P));
-    return a.P > 1 ? launch_pdl_cluster(kernel, grid, dim3(kSelThreads), 0, st, dim3(a.P), a)
-                   : launch_pdl(kernel, grid, dim3(kSelThreads), 0, st, a);
+    return launch_pdl_cluster(kernel, grid, dim3(kSelThreads), 0, st, dim3(a.P), a);
 }
 
 }  // namespace dwa
