@@ -585,7 +585,7 @@ DWA_API int dwa_retrieve_noalloc_status(void* stream, uint32_t* status, int clea
  * stride_inner = V.  A row may start on any element; outputs are contiguous.
  * rows may be 0 (nothing is launched).
  * ------------------------------------------------------------------------- */
-#define DWA_MAX_VOCAB (1 << 20)
+#define DWA_MAX_VOCAB 393216
 #define DWA_MAX_TOP   1024
 
 typedef struct DwaLogitsDims {
@@ -624,7 +624,7 @@ DWA_API int dwa_top_logits(void* stream, const DwaLogitsDims* dims, const void* 
  * inputs and the state.  An index >= V, or one listed twice in a row, sets
  * DWA_STATUS_BAD_TOKEN in the workspace's status word and makes the row's loss
  * and gradient NaN. */
-#define DWA_DISTILL_STATE_FLOATS 8
+#define DWA_DISTILL_STATE_FLOATS 9
 
 typedef struct DwaDistillDims {
     int32_t K;

@@ -18,9 +18,9 @@ DWA_ERR_DEVICE = -5
 DWA_PAD_INDEX = -(2 ** 31)
 DWA_F32 = 0
 DWA_BF16 = 1
-DWA_MAX_VOCAB = 1 << 20
+DWA_MAX_VOCAB = 393216
 DWA_MAX_TOP = 1024
-DWA_DISTILL_STATE_FLOATS = 8
+DWA_DISTILL_STATE_FLOATS = 9
 
 STATUS_BITS = {
     0x1: "row index outside the pool",

@@ -15,13 +15,15 @@
 // entries set apart.
 //
 // Bound: HBM.  The loss has to read the row once, the gradient to write it once;
-// everything else is K entries a row.  The forward keeps a running maximum and
-// the sum of exp((z - max) / T) over the UNLISTED entries alone (a bitmap of the
-// row in shared memory tells which, one byte per 16-byte word of bf16): q_t as
-// total minus listed would lose all its digits where the listed entries hold
-// nearly everything.  Row sums are kept in fp32, what is left of a row (K terms
-// and a few logarithms) is done in fp64, where differences of logarithms keep
-// the digits that fp32 would round away.
+// everything else is K entries a row.  A cluster of P CTAs holds a row in its
+// shared memory (chunks of at most 72 KB, so that three CTAs share an SM and one
+// loads while another writes), so the gradient reads nothing again.  One pass
+// over the chunk keeps a running maximum and the sum of exp((z - max) / T) over
+// the UNLISTED entries alone (a bitmap of the chunk tells which, one byte per
+// 16-byte word of bf16): q_t as total minus listed would lose all its digits
+// where the listed entries hold nearly everything.  Row sums are kept in fp32;
+// what is left of a row (K terms and a few logarithms) is done in fp64, where
+// differences of logarithms keep the digits that fp32 would round away.
 
 #include <atomic>
 
@@ -31,7 +33,11 @@ namespace dwa {
 
 extern std::atomic<uint64_t> g_launches_total;
 
-constexpr int kDistillThreads = 512;
+constexpr int kDistillThreads = 256;
+constexpr int kDistillWarps = kDistillThreads / 32;
+constexpr int kDistillMaxCluster = 8;
+constexpr int kDistillPieces = 4;                // pieces in which a chunk arrives
+constexpr int kDistillChunkBytes = 72 * 1024;    // three CTAs an SM
 constexpr float kTailFloor = 5.9604645e-8f;      // 2^-24: what an fp32 log-sum-exp can tell from no tail
 constexpr float kTailNone = 1.52587890625e-5f;   // 2^-16: a teacher's tail that may be its rounding alone
 
@@ -39,12 +45,13 @@ enum : int { kRowPlain = 0, kRowZero = 1, kRowBad = 2 };
 
 // What the backward needs of a row.
 struct RowState {
-    float m, S;        // the student's maximum and sum of exp((z - m) / T)
+    float m, S;        // a reference and the sum of the student's weights relative to it (Ref)
+    float log2_S;      // log2 S less its rounding to an integer, and
+    float log2_S_int;  // that integer
     float of_tail;     // dL/dx of an unlisted entry over its q
     float L;           // the loss before its weight
     float t_hi, t_lo;  // log p_k = (t_k - t_hi) / T - t_lo
     float kind;        // kRowPlain, kRowZero (nothing to learn) or kRowBad
-    float unused;
 };
 static_assert(sizeof(RowState) == DWA_DISTILL_STATE_FLOATS * sizeof(float), "layout of the saved row state");
 
@@ -61,202 +68,374 @@ struct DistillArgs {
     const float* g_loss;
     void* g;
     uint32_t* status;
-    float c;   // log2(e) / T
+    float c;       // log2(e) / T
+    double inv_T;
+    int P, log_P;  // CTAs per row
+    int room;      // words of the largest chunk
 };
 
-// dL/dx of listed entry k, from its logits.
+constexpr double kLn2 = 0.6931471805599453;
+
+// log2(x) as an integer and a rest in [-0.5, 0.5], which fp32 holds to 2^-25.
+__device__ __forceinline__ void log2_parts(float x, float& whole, float& rest) {
+    const float l = log2f(x);
+    whole = rintf(l);
+    rest = fabsf(l) < INFINITY ? log2f(ldexpf(x, -static_cast<int>(whole))) : l;
+}
+// log(x) with the relative precision of fp32 also where x is 1 - y with a small y.
+__device__ __forceinline__ double log_of_rest(double x, double y) {
+    return x > 0.5 ? log1pf(static_cast<float>(-y)) : logf(static_cast<float>(x));
+}
+
+// dL/dx of a listed entry from its logits.
 __device__ __forceinline__ float listed_grad(const RowState& s, const DistillArgs& a, float zk, float tk) {
-    const float q = exp2_fast((zk - s.m) * a.c) / s.S;
-    const double T = a.o.temperature;
-    const double lp = (static_cast<double>(tk) - s.t_hi) / T - s.t_lo;
+    const Ref ref(s.m, a.c);
+    const float q = ref.weight(zk, a.c) / s.S;
+    const double lp = (static_cast<double>(tk) - s.t_hi) * a.inv_T - s.t_lo;
     if (!a.o.reverse) return q - (tk == -INFINITY ? 0.f : expf(static_cast<float>(lp)));
     if (q == 0.f) return 0.f;
-    const double lq = (static_cast<double>(zk) - s.m) / T - log(static_cast<double>(s.S));
-    return q * static_cast<float>(lq - lp - s.L);
+    const double x = static_cast<double>(zk) * a.c, r = kLn2 * (x - ref.a(a.c) - s.log2_S_int - s.log2_S) - lp - s.L;
+    return fabs(r) > 1e-14 * (fabs(x) + fabs(lp)) ? q * static_cast<float>(r) : 0.f;   // else the terms' rounding
 }
 
-// The gradient of one row into g [V]: the unlisted coefficient times q over the
-// whole row, then the listed entries.  `zk`, `tk` (shared memory) were read
-// before, so g may be the logits' own memory.
+// The unlisted entries' gradient of one row, word by word.
 template <class T>
-__device__ __forceinline__ void write_grad(const RowWords<T>& w, T* g, const RowState& s, const DistillArgs& a,
-                                           float scale, const float* zk, const float* tk, const int32_t* idx) {
-    constexpr int VEC = kRowVec<T>;
-    const int tid = threadIdx.x, n = blockDim.x;
-    const int kind = static_cast<int>(s.kind);
-    const float unl = kind == kRowPlain ? s.of_tail * scale / s.S : kind == kRowZero ? 0.f : NAN;
-    const bool same = (reinterpret_cast<uintptr_t>(g) - reinterpret_cast<uintptr_t>(w.row)) % 16 == 0;
-    w.template each<4>(0, w.words, tid, n, [&](uint4 x, int j0, int) {
+struct GradWriter {
+    T* g;          // the row's gradient
+    int V;
+    bool fast;     // a plain row, and g has the phase of the logits
+    int kind;
+    Ref ref;
+    float c, unl;
+
+    __device__ __forceinline__ GradWriter(const RowWords<T>& w, T* g_, const RowState& s, const DistillArgs& a, float scale)
+        : g(g_), V(w.V), kind(static_cast<int>(s.kind)), ref(s.m, a.c), c(a.c) {
+        fast = kind == kRowPlain && (reinterpret_cast<uintptr_t>(g) - reinterpret_cast<uintptr_t>(w.row)) % 16 == 0;
+        unl = kind == kRowPlain ? s.of_tail * scale / s.S : kind == kRowZero ? 0.f : NAN;
+    }
+    // any word
+    __device__ __forceinline__ void operator()(uint4 x, int j0) const {
+        constexpr int VEC = kRowVec<T>;
+        uint64_t e[VEC / 2];
         float o[VEC];
-        word_exp<T>(x, s.m, a.c, o);
+        word_weights<T>(x, ref, c, e);
+        unpair_word<T>(e, o);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = kind == kRowPlain ? o[i] * unl : unl;
-        if (same && j0 >= 0 && j0 + VEC <= w.V) {
-            *reinterpret_cast<uint4*>(g + j0) = pack<T>(o);
-        } else {
+        for (int i = 0; i < VEC; ++i)
+            if (j0 + i >= 0 && j0 + i < V) g[j0 + i] = Elem<T>::from_f(kind == kRowPlain ? o[i] * unl : unl);
+    }
+    // a whole word of a fast row
+    __device__ __forceinline__ void whole(uint4 x, uint4* to) const {
+        constexpr int VEC = kRowVec<T>;
+        uint64_t e[VEC / 2];
+        float o[VEC];
+        word_weights<T>(x, ref, c, e);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i)
-                if (j0 + i >= 0 && j0 + i < w.V) g[j0 + i] = Elem<T>::from_f(o[i]);
-        }
-    });
-    if (kind != kRowPlain) return;
-    __syncthreads();
-    for (int k = tid; k < a.o.K; k += n)
-        if (idx[k] >= 0) g[idx[k]] = Elem<T>::from_f(listed_grad(s, a, zk[k], tk[k]) * scale);
+        for (int i = 0; i < VEC / 2; ++i) e[i] = mul2(e[i], pair(unl, unl));
+        unpair_word<T>(e, o);
+        __stcs(to, pack<T>(o));
+    }
+};
+
+// What one warp of a row's CTAs hands to all of them.
+struct DistillPart {
+    double P, L, S_l;  // sum p; forward: sum p (log p - x), reverse: sum w (x - log p), x = log2(e) z / T ln 2; sum w
+    float m, S_u;      // reference; sum of the weights w of unlisted entries
+    int bad;
+};
+
+__device__ __forceinline__ double warp_sum_d(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
 }
 
-// One CTA per row: the loss, the state for a backward (a.state) and, with GRAD,
-// the gradient of weight * L (the row is read again, out of L2).
-template <class T, bool GRAD>
-__global__ void __launch_bounds__(kDistillThreads) distill_fwd_kernel(DistillArgs a) {
-    pdl_enter();
-    constexpr int VEC = kRowVec<T>;
-    extern __shared__ float sm[];
-    __shared__ float redf[33];
-    __shared__ double redd[33];
-    __shared__ int bad, valid;
-    const int tid = threadIdx.x, n = blockDim.x, K = a.o.K, V = a.d.V;
-    const int64_t r = blockIdx.x;
-    const RowWords<T> w(static_cast<const T*>(a.z) + row_offset(a.d, r), V);
-    T* g = GRAD ? static_cast<T*>(a.g) + r * V : nullptr;
-    const int32_t* idx = a.idx + r * K;
-    float* zk = sm;
-    float* tk = zk + K;
-    uint32_t* bits = reinterpret_cast<uint32_t*>(tk + K);
-    const float weight = a.weights ? a.weights[r] : 1.f;
-    RowState s = {};
-    if (weight == 0.f) {   // a row left out: its logits and teacher are not looked at
-        s.kind = kRowZero;
-        if (tid == 0) {
-            a.loss[r] = 0.f;
-            if (a.state) a.state[r] = s;
-        }
-        if constexpr (GRAD) write_grad(w, g, s, a, 0.f, zk, tk, idx);
-        return;
+// A row's state from its parts, and its loss: one warp.
+__device__ __forceinline__ double finish_row(RowState& s, const DistillPart* part, const DistillArgs& a, int valid) {
+    const int lane = threadIdx.x & 31;
+    double P = 0., S_u = 0., S_l = 0., L = 0.;
+    float m = -INFINITY;
+    int bad = 0;
+    for (int i = lane; i < a.P * kDistillWarps; i += 32) {
+        m = fmaxf(m, part[i].m);
+        bad |= part[i].bad;
     }
-    for (int i = tid; i < (w.words * VEC + 31) / 32; i += n) bits[i] = 0u;
-    if (tid == 0) bad = valid = 0;
-    __syncthreads();
-    int mine = 0;
-    for (int k = tid; k < K; k += n) {
-        const int j = idx[k];
-        float z = -INFINITY, t = -INFINITY;
-        if (j >= V) {
-            bad = 1;
-        } else if (j >= 0) {
-            const int b = j + w.shift;
-            if (atomicOr(&bits[b >> 5], 1u << (b & 31)) & (1u << (b & 31))) bad = 1;
-            z = Elem<T>::to_f(w.row[j]);
-            t = load_elem(a.t, r * K + k, a.o.teacher_dtype);
-            ++mine;
-        }
-        zk[k] = z;
-        tk[k] = t;
+    s.m = warp_max(m);
+    bad = __any_sync(0xffffffffu, bad);
+    const Ref ref(s.m, a.c);
+    for (int i = lane; i < a.P * kDistillWarps; i += 32) {
+        const DistillPart& x = part[i];
+        // a part without anything above -inf: its sums are 0 (NaN with a NaN)
+        const double f = x.m > -INFINITY ? Ref(x.m, a.c).rescale(ref, a.c) : 1.f;
+        P += x.P;
+        S_u += f * x.S_u;
+        S_l += f * x.S_l;
+        L += a.o.reverse ? f * x.L : x.L;
     }
-    if (mine) atomicAdd(&valid, mine);
-    __syncthreads();
-
-    // one pass: the row's maximum, and the sum over unlisted entries
-    MaxSum ms;
-    w.template each<4>(0, w.words, tid, n, [&](uint4 x, int j0, int) {
-        ms.raise(word_max<T>(x), a.c);
-        float e[VEC];
-        word_exp<T>(x, ms.m, a.c, e);
-        const int b = j0 + w.shift;
-        const uint32_t listed = bits[b >> 5] >> (b & 31) & ((1u << VEC) - 1u);
-        if (listed == 0u && ms.m > -INFINITY) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) ms.s += e[i];
-        } else if (ms.m > -INFINITY) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) ms.s += (listed >> i) & 1u ? 0.f : e[i];
-        }
-    });
-    s.m = block_reduce(ms.m, MaxOp(), -INFINITY, redf);
-    const float S_u = block_reduce(ms.at(s.m, a.c), AddOp(), 0.f, redf);
-
-    // the listed entries
-    const double T0 = a.o.temperature;
-    float S_l = 0.f;
-    for (int k = tid; k < K; k += n)
-        if (idx[k] >= 0) S_l += exp2_fast((zk[k] - s.m) * a.c);
-    S_l = block_reduce(S_l, AddOp(), 0.f, redf);
-    s.S = S_u + S_l;
-    const double log_S = log(static_cast<double>(S_u) + S_l);
-    if (a.t_lse) {
-        s.t_hi = 0.f;
-        s.t_lo = a.t_lse[r];
-    } else {
-        float top = -INFINITY;
-        for (int k = tid; k < K; k += n) top = fmaxf(top, tk[k]);
-        s.t_hi = block_reduce(top, MaxOp(), -INFINITY, redf);
-        double sum = 0.;
-        for (int k = tid; k < K; k += n)
-            if (idx[k] >= 0) sum += expf(static_cast<float>((static_cast<double>(tk[k]) - s.t_hi) / T0));
-        s.t_lo = static_cast<float>(log(block_reduce(sum, AddOp(), 0., redd)));
-    }
-    double P = 0., L = 0.;
-    for (int k = tid; k < K; k += n) {
-        if (idx[k] < 0) continue;
-        const double lp = (static_cast<double>(tk[k]) - s.t_hi) / T0 - s.t_lo;
-        const double lq = (static_cast<double>(zk[k]) - s.m) / T0 - log_S;
-        const float p = tk[k] == -INFINITY ? 0.f : expf(static_cast<float>(lp));
-        P += p;
-        if (a.o.reverse) {
-            const float q = exp2_fast((zk[k] - s.m) * a.c) / s.S;
-            if (q != 0.f) L += q * (lq - lp);
-        } else if (p != 0.f) {
-            L += p * (lp - lq);
-        }
-    }
-    P = block_reduce(P, AddOp(), 0., redd);
-    L = block_reduce(L, AddOp(), 0., redd);
-    const bool nothing = valid == 0 || (!a.t_lse && s.t_hi == -INFINITY);
+    P = warp_sum_d(P);
+    S_u = warp_sum_d(S_u);
+    S_l = warp_sum_d(S_l);
+    L = warp_sum_d(L);
+    const double S = S_u + S_l;
+    s.S = static_cast<float>(S);
+    log2_parts(s.S, s.log2_S_int, s.log2_S);
+    // log q = x - log_S
+    const double log_S = kLn2 * (ref.a(a.c) + s.log2_S_int + s.log2_S);
+    if (a.o.reverse) L = (L - (S_l != 0. ? S_l * log_S : 0.)) / S;
+    else L += P != 0. ? P * log_S : 0.;
     s.of_tail = 1.f;
-    if (a.t_lse && valid < V) {
-        const double p_t = fmax(1. - P, static_cast<double>(kTailFloor));
-        const double q_t = S_u / (static_cast<double>(S_u) + S_l);
+    if (a.t_lse && valid < a.d.V) {
+        const double p_t = fmax(1. - P, static_cast<double>(kTailFloor)), q_t = S_u / S;
         if (q_t == 0.) {
             if (!a.o.reverse && p_t > kTailNone) L = INFINITY;
             s.of_tail = 0.f;
         } else {
-            const double r_t = log(q_t) - log(p_t);
+            const double r_t = log_of_rest(q_t, S_l / S) - log_of_rest(p_t, P);
             L += a.o.reverse ? q_t * r_t : -p_t * r_t;
             s.of_tail = static_cast<float>(a.o.reverse ? r_t - L : 1. - p_t / q_t);
         }
     }
+    const bool nothing = valid == 0 || (!a.t_lse && s.t_hi == -INFINITY);
     s.L = static_cast<float>(L);
     s.kind = bad ? kRowBad : nothing ? kRowZero : kRowPlain;
-    if (tid == 0) {
-        if (bad) raise_status(a.status, DWA_STATUS_BAD_TOKEN);
-        a.loss[r] = bad ? NAN : nothing ? 0.f : static_cast<float>(L * weight);
-        if (a.state) a.state[r] = s;
-    }
-    if constexpr (GRAD) write_grad(w, g, s, a, weight / a.o.temperature, zk, tk, idx);
+    return bad ? NAN : nothing ? 0. : L;
 }
 
-// The gradient from a saved state: one CTA per row.
-template <class T>
-__global__ void __launch_bounds__(kDistillThreads) distill_bwd_kernel(DistillArgs a) {
+// A cluster of P CTAs per row: the loss, the state for a backward (a.state) and,
+// with GRAD, the gradient of weight * L.
+template <class T, bool GRAD>
+__global__ void __launch_bounds__(kDistillThreads, 4) distill_fwd_kernel(const __grid_constant__ DistillArgs a) {
+    namespace cg = cooperative_groups;
+    constexpr int VEC = kRowVec<T>;
+    extern __shared__ __align__(16) uint4 data[];
+    __shared__ DistillPart part[kDistillMaxCluster * kDistillWarps];
+    __shared__ double redd[33];
+    __shared__ float redf[33];
+    __shared__ RowState row_state;
+    __shared__ int bad, valid;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.o.K, V = a.d.V;
+    const uint32_t r = blockIdx.x >> a.log_P;
+    const int p = blockIdx.x & (a.P - 1);
+    uint32_t* bits = reinterpret_cast<uint32_t*>(data + a.room);
+    float* tk = reinterpret_cast<float*>(bits + (a.room * VEC + 127) / 128 * 4);
+    int* at = reinterpret_cast<int*>(tk + K);   // a listed entry's place in the chunk, -1 elsewhere
+    if (a.P > 1) cluster_arrive_relaxed();
+    if (tid == 0) bad = valid = 0;
     pdl_enter();
-    extern __shared__ float sm[];
-    const int tid = threadIdx.x, n = blockDim.x, K = a.o.K, V = a.d.V;
-    const int64_t r = blockIdx.x;
     const RowWords<T> w(static_cast<const T*>(a.z) + row_offset(a.d, r), V);
-    const int32_t* idx = a.idx + r * K;
-    float* zk = sm;
-    float* tk = zk + K;
-    const RowState s = a.state[r];
-    if (s.kind == kRowPlain) {
-        for (int k = tid; k < K; k += n) {
-            if (idx[k] < 0) continue;
-            zk[k] = Elem<T>::to_f(w.row[idx[k]]);
-            tk[k] = load_elem(a.t, r * K + k, a.o.teacher_dtype);
+    const Chunk ch(w.words, p, a.log_P);
+    const int n = ch.hi - ch.lo;
+    T* g = GRAD ? static_cast<T*>(a.g) + static_cast<int64_t>(r) * V : nullptr;
+    const int32_t* idx = a.idx + static_cast<int64_t>(r) * K;
+    const float weight = a.weights ? a.weights[r] : 1.f;
+    if (weight == 0.f) {   // a row left out: its logits and teacher are not looked at
+        RowState s = {};
+        s.kind = kRowZero;
+        if (p == 0 && tid == 0) {
+            a.loss[r] = 0.f;
+            if (a.state) a.state[r] = s;
+        }
+        if constexpr (GRAD) {
+            const GradWriter<T> write(w, g, s, a, 0.f);
+            for (int i = ch.lo + tid; i < ch.hi; i += kDistillThreads) write(make_uint4(0u, 0u, 0u, 0u), w.first(i));
+        }
+        if (a.P > 1) cluster_wait();
+        return;
+    }
+    // the chunk, in pieces: every thread copies the words that it will look at
+    int from, to;
+    w.own_whole(ch.lo, ch.hi, tid, kDistillThreads, from, to);
+    uint4* const own_words = data + tid;
+    const auto piece = [&](int i) { return from + (to - from) * i / kDistillPieces; };
+    const uint4* const src = reinterpret_cast<const uint4*>(w.row + w.first(ch.lo + tid));
+#pragma unroll
+    for (int i = 0; i < kDistillPieces; ++i) {
+        const int end = piece(i + 1);
+#pragma unroll 4
+        for (int k = piece(i); k < end; ++k) copy_async(own_words + k * kDistillThreads, src + k * kDistillThreads);
+        copy_commit();
+    }
+    // meanwhile the teacher
+    for (int i = tid; i < (n * VEC + 127) / 128; i += kDistillThreads)
+        reinterpret_cast<uint4*>(bits)[i] = make_uint4(0u, 0u, 0u, 0u);
+    __syncthreads();
+    int mine = 0;
+    float t_top = -INFINITY;
+    for (int k = tid; k < K; k += kDistillThreads) {
+        const int j = idx[k];
+        float t = -INFINITY;
+        int place = -1;
+        if (j >= V) {
+            bad = 1;
+        } else if (j >= 0) {
+            t = load_elem(a.t, static_cast<int64_t>(r) * K + k, a.o.teacher_dtype);
+            ++mine;
+            const int b = j + w.shift - ch.lo * VEC;
+            if (b >= 0 && b < n * VEC) {
+                place = b;
+                if (atomicOr(&bits[b >> 5], 1u << (b & 31)) & (1u << (b & 31))) bad = 1;
+            }
+        }
+        tk[k] = t;
+        at[k] = place;
+        t_top = fmaxf(t_top, t);
+    }
+    if (mine) atomicAdd(&valid, mine);
+    RowState s = {};
+    if (a.t_lse) {
+        s.t_lo = a.t_lse[r];
+        __syncthreads();
+    } else {
+        s.t_hi = block_reduce(t_top, MaxOp(), -INFINITY, redf);
+        double sum = 0.;
+        for (int k = tid; k < K; k += kDistillThreads)
+            if (tk[k] > -INFINITY) sum += expf(static_cast<float>((static_cast<double>(tk[k]) - s.t_hi) * a.inv_T));
+        s.t_lo = logf(static_cast<float>(block_reduce(sum, AddOp(), 0., redd)));
+    }
+    // one pass: the chunk's maximum, and the sum over unlisted entries
+    MaxSum ms;
+    const uint8_t* byte = reinterpret_cast<const uint8_t*>(bits);
+    const auto add_word = [&](uint4 x, int k) {
+        const float top = word_max<T>(x);
+        const uint32_t listed = VEC == 8 ? byte[k] : (byte[k >> 1] >> (4 * (k & 1))) & 15u;
+        if (!ms.covers(top)) {
+            ms.raise(top, a.c);
+            if (top != top) ms.poison();
+            if (ms.ref.m == -INFINITY) return;
+        }
+        uint64_t e[VEC / 2];
+        word_weights<T>(x, ms.ref, a.c, e);
+        if (listed != 0u) {
+            float f[VEC];
+            unpair_word<T>(e, f);
+#pragma unroll
+            for (int v = 0; v < VEC; v += 2)
+                e[v / 2] = pair((listed >> v) & 1u ? 0.f : f[v], (listed >> v) & 2u ? 0.f : f[v + 1]);
+        }
+        ms.s2 = add2(ms.s2, sum_pairs<T>(e));
+    };
+    const auto add = [&](int i) {
+        const int end = piece(i + 1);
+#pragma unroll 2
+        for (int k = piece(i); k < end; ++k) add_word(own_words[k * kDistillThreads], tid + k * kDistillThreads);
+    };
+    w.edges(ch.lo, ch.hi, tid, [&](uint4 x, int j0) {
+        const int k = (j0 + w.shift) / VEC - ch.lo;
+        data[k] = x;
+        add_word(x, k);
+    });
+    static_assert(kDistillPieces == 4, "one wait a piece");
+    copy_wait<3>();
+    add(0);
+    copy_wait<2>();
+    add(1);
+    copy_wait<1>();
+    add(2);
+    copy_wait<0>();
+    add(3);
+    __syncthreads();   // the listed entries may be other threads' words
+    const Ref ref(warp_max(ms.ref.m), a.c);   // the warp's
+    DistillPart own = {0., 0., 0., ref.m, warp_sum(ms.at(ref, a.c)), bad};
+    // the warp's share of the chunk's listed entries
+    float z_top = ref.m;
+    for (int k = tid; k < K; k += kDistillThreads)
+        if (at[k] >= 0) z_top = fmaxf(z_top, Elem<T>::to_f(reinterpret_cast<const T*>(data)[at[k]]));
+    const Ref all(warp_max(z_top), a.c);
+    if (ref.m > -INFINITY) own.S_u *= ref.rescale(all, a.c);
+    own.m = all.m;
+    if (warp * 32 < K) {
+        for (int k = tid; k < K; k += kDistillThreads) {
+            if (at[k] < 0) continue;
+            const float z = Elem<T>::to_f(reinterpret_cast<const T*>(data)[at[k]]);
+            const double lp = (static_cast<double>(tk[k]) - s.t_hi) * a.inv_T - s.t_lo, x = kLn2 * a.c * z;
+            const float e = z == -INFINITY ? 0.f : all.weight(z, a.c);   // the reference may be -inf too
+            const float prob = tk[k] == -INFINITY ? 0.f : expf(static_cast<float>(lp));
+            own.S_l += e;
+            own.P += prob;
+            if (a.o.reverse) own.L += e != 0.f ? e * (x - lp) : 0.;
+            else own.L += prob != 0.f ? prob * (lp - x) : 0.;
+        }
+        own.S_l = warp_sum_d(own.S_l);
+        own.P = warp_sum_d(own.P);
+        own.L = warp_sum_d(own.L);
+    }
+    if (a.P > 1) {
+        cluster_wait();   // every CTA of the cluster has started
+        if (lane < a.P) *cg::this_cluster().map_shared_rank(&part[p * kDistillWarps + warp], lane) = own;
+        cg::this_cluster().sync();
+    } else {
+        if (lane == 0) part[warp] = own;
+        __syncthreads();
+    }
+    if (!GRAD && p != 0) return;
+    if (warp == 0) {
+        const double L = finish_row(s, part, a, valid);
+        if (lane == 0) row_state = s;
+        if (p == 0 && lane == 0) {
+            if (s.kind == kRowBad) raise_status(a.status, DWA_STATUS_BAD_TOKEN);
+            a.loss[r] = static_cast<float>(L * weight);
+            if (a.state) a.state[r] = s;
         }
     }
+    if constexpr (GRAD) {
+        __syncthreads();
+        s = row_state;
+        const float scale = weight / a.o.temperature;
+        const GradWriter<T> write(w, g, s, a, scale);
+        if (write.fast) {
+            uint4* const to_g = reinterpret_cast<uint4*>(g + w.first(ch.lo + tid));
+#pragma unroll 4
+            for (int k = from; k < to; ++k) write.whole(own_words[k * kDistillThreads], to_g + k * kDistillThreads);
+            w.edges(ch.lo, ch.hi, tid, write);
+        } else {
+            for (int k = tid; k < n; k += kDistillThreads) write(data[k], w.first(ch.lo + k));
+        }
+        if (s.kind != kRowPlain) return;
+        __syncthreads();
+        for (int k = tid; k < K; k += kDistillThreads) {
+            if (at[k] < 0) continue;
+            const float z = Elem<T>::to_f(reinterpret_cast<const T*>(data)[at[k]]);
+            g[at[k] + w.first(ch.lo)] = Elem<T>::from_f(listed_grad(s, a, z, tk[k]) * scale);
+        }
+    }
+}
+
+// The gradient from a saved state: P CTAs per row, each its words.  g may be the
+// logits' own memory: a listed entry is read before its word is written.
+template <class T>
+__global__ void __launch_bounds__(kDistillThreads) distill_bwd_kernel(const __grid_constant__ DistillArgs a) {
+    pdl_enter();
+    constexpr int VEC = kRowVec<T>;
+    extern __shared__ float zk[];
+    const int tid = threadIdx.x, K = a.o.K, V = a.d.V;
+    const uint32_t r = blockIdx.x >> a.log_P;
+    const RowWords<T> w(static_cast<const T*>(a.z) + row_offset(a.d, r), V);
+    const Chunk ch(w.words, blockIdx.x & (a.P - 1), a.log_P);
+    const int32_t* idx = a.idx + static_cast<int64_t>(r) * K;
+    const RowState s = a.state[r];
+    const bool plain = s.kind == kRowPlain;
+    const auto here = [&](int j) { return j >= 0 && (j + w.shift) / VEC >= ch.lo && (j + w.shift) / VEC < ch.hi; };
+    if (plain) {
+        for (int k = tid; k < K; k += kDistillThreads)
+            if (here(idx[k])) zk[k] = Elem<T>::to_f(w.row[idx[k]]);
+        __syncthreads();
+    }
+    const float scale = (a.weights ? a.weights[r] : 1.f) * a.g_loss[r] / a.o.temperature;
+    T* g = static_cast<T*>(a.g) + static_cast<int64_t>(r) * V;
+    const GradWriter<T> write(w, g, s, a, scale);
+    if (write.fast) {
+        w.template each_whole<4>(ch.lo, ch.hi, tid, kDistillThreads, [&](uint4 x, int j0, int) {
+            write.whole(x, reinterpret_cast<uint4*>(g + j0));
+        });
+        w.edges(ch.lo, ch.hi, tid, write);
+    } else {
+        w.template each<1>(ch.lo, ch.hi, tid, kDistillThreads, [&](uint4 x, int j0, int) { write(x, j0); });
+    }
+    if (!plain) return;
     __syncthreads();
-    const float weight = (a.weights ? a.weights[r] : 1.f) * a.g_loss[r];
-    write_grad(w, static_cast<T*>(a.g) + r * V, s, a, weight / a.o.temperature, zk, tk, idx);
+    for (int k = tid; k < K; k += kDistillThreads)
+        if (here(idx[k]))
+            g[idx[k]] = Elem<T>::from_f(listed_grad(s, a, zk[k], load_elem(a.t, static_cast<int64_t>(r) * K + k, a.o.teacher_dtype)) * scale);
 }
 
 int check_logits(const DwaLogitsDims* d, const char* what) {
@@ -269,7 +448,7 @@ int check_logits(const DwaLogitsDims* d, const char* what) {
     if (d->stride_outer < 0 || d->stride_inner < 0)
         return fail(DWA_ERR_INVALID_ARG, w + ": strides must not be negative");
     if (d->V > DWA_MAX_VOCAB) return fail(DWA_ERR_UNSUPPORTED, w + ": V > " + std::to_string(DWA_MAX_VOCAB));
-    if (d->rows >= (int64_t(1) << 31)) return fail(DWA_ERR_UNSUPPORTED, w + ": rows >= 2^31");
+    if (d->rows >= (int64_t(1) << 28)) return fail(DWA_ERR_UNSUPPORTED, w + ": rows >= 2^28");
     return DWA_OK;
 }
 
@@ -304,12 +483,29 @@ static int allow_smem(K kernel, size_t bytes) {
     return DWA_OK;
 }
 
+// CTAs per row: enough that a chunk leaves room for three CTAs an SM (or fits at
+// all), more while the launch is short of two CTAs an SM and chunks stay above
+// 16 KB.
+static int log_ctas_per_row(const DwaLogitsDims& d) {
+    const int64_t bytes = static_cast<int64_t>(d.V) * dtype_bytes(d.dtype);
+    int l = 0;
+    while (1 << l < kDistillMaxCluster &&
+           (bytes > kDistillChunkBytes << l || (d.rows << l < 2 * tc::sm_count() && bytes > 32 * 1024 << l)))
+        ++l;
+    return l;
+}
+
 template <class T, bool GRAD>
-static int launch_fwd(cudaStream_t st, const DistillArgs& a) {
-    const size_t sh = static_cast<size_t>(a.o.K) * 8 + align_up(static_cast<size_t>(a.d.V) / 8 + 8, 16);
+static int launch_fwd(cudaStream_t st, DistillArgs a) {
+    constexpr int VEC = kRowVec<T>;
+    a.log_P = log_ctas_per_row(a.d);
+    a.P = 1 << a.log_P;
+    a.room = (a.d.V + 2 * VEC - 2) / VEC / a.P + 1;
+    const size_t sh = static_cast<size_t>(a.room) * 16 + (static_cast<size_t>(a.room) * VEC + 127) / 128 * 16 +
+                      static_cast<size_t>(a.o.K) * 8;
     if (int rc = allow_smem(distill_fwd_kernel<T, GRAD>, sh)) return rc;
-    DWA_TIMED("distill_fwd", st, (launch_pdl(distill_fwd_kernel<T, GRAD>, dim3(static_cast<unsigned>(a.d.rows)),
-                                             dim3(kDistillThreads), sh, st, a)));
+    DWA_TIMED("distill_fwd", st, (launch_pdl_cluster(distill_fwd_kernel<T, GRAD>, dim3(static_cast<unsigned>(a.d.rows * a.P)),
+                                                     dim3(kDistillThreads), sh, st, dim3(a.P), a)));
     DWA_LAUNCH_CHECK("distill_fwd_kernel");
     ++g_launches_total;
     return DWA_OK;
@@ -336,7 +532,7 @@ extern "C" int dwa_distill_fwd(void* stream, const DwaLogitsDims* dims, const Dw
     if ((rc = check_workspace(workspace, workspace_bytes))) return rc;
     const DistillArgs a = {logits, *dims, *opts, teacher_logits, teacher_indices, teacher_lse, weights, loss,
                            reinterpret_cast<RowState*>(state), nullptr, g_logits, static_cast<uint32_t*>(workspace),
-                           kLog2e / opts->temperature};
+                           kLog2e / opts->temperature, 1. / opts->temperature, 1, 0, 0};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dims->dtype == DWA_BF16)
         return g_logits ? launch_fwd<__nv_bfloat16, true>(st, a) : launch_fwd<__nv_bfloat16, false>(st, a);
@@ -354,12 +550,13 @@ extern "C" int dwa_distill_bwd(void* stream, const DwaLogitsDims* dims, const Dw
     if (misaligned(logits, dims->dtype) || misaligned(g_logits, dims->dtype) ||
         misaligned(teacher_logits, opts->teacher_dtype))
         return fail(DWA_ERR_INVALID_ARG, "distill: a pointer is not aligned to its element");
+    const int log_P = log_ctas_per_row(*dims);
     const DistillArgs a = {logits, *dims, *opts, teacher_logits, teacher_indices, teacher_lse, weights, nullptr,
                            reinterpret_cast<RowState*>(const_cast<float*>(state)), g_loss, g_logits, nullptr,
-                           kLog2e / opts->temperature};
+                           kLog2e / opts->temperature, 1. / opts->temperature, 1 << log_P, log_P, 0};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const size_t sh = static_cast<size_t>(opts->K) * 8;
-    const dim3 grid(static_cast<unsigned>(dims->rows));
+    const size_t sh = static_cast<size_t>(opts->K) * 4;
+    const dim3 grid(static_cast<unsigned>(dims->rows << log_P));
     if (dims->dtype == DWA_BF16)
         DWA_TIMED("distill_bwd", st,
                   (launch_pdl(distill_bwd_kernel<__nv_bfloat16>, grid, dim3(kDistillThreads), sh, st, a)));

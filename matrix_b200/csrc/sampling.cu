@@ -167,13 +167,6 @@ struct SelShared {
     int n_chosen, n_list;
 };
 
-struct Chunk {
-    int lo, hi;
-    __device__ __forceinline__ Chunk(int words, int p, int P)
-        : lo(static_cast<int>(static_cast<int64_t>(words) * p / P)),
-          hi(static_cast<int>(static_cast<int64_t>(words) * (p + 1) / P)) {}
-};
-
 // This CTA's share: the maxima of the thread's words by position mod 8 (`edge`:
 // of a row's first and last word where they are not whole) and, with SUM, the
 // running maximum and sum of exp((z - m) / T).
@@ -188,12 +181,11 @@ __device__ __forceinline__ void scan_chunk(const RowWords<T>& w, Chunk ch, float
         if (u < 0) edge = m;
         else top[u] = max_nan(top[u], m);
         if constexpr (SUM) {
-            ms.raise(m, c);
-            if (ms.m > -INFINITY) {
-                float e[kRowVec<T>];
-                word_exp<T>(x, ms.m, c, e);
-#pragma unroll
-                for (int i = 0; i < kRowVec<T>; ++i) ms.s += e[i];
+            if (!ms.covers(m)) ms.raise(m, c);
+            if (ms.ref.m > -INFINITY) {
+                uint64_t e[kRowVec<T> / 2];
+                word_weights<T>(x, ms.ref, c, e);
+                ms.s2 = add2(ms.s2, sum_pairs<T>(e));
             }
         }
     });
@@ -219,8 +211,8 @@ __device__ __forceinline__ void push_groups(SelShared& sh, int p, int P, float (
     for (int u = 0; u < 8; ++u) all = max_nan(all, top[u]);
     // NaN above everything, as in the keys
     const uint32_t first = block_reduce(ordered(all), MaxOp(), 0u, reinterpret_cast<uint32_t*>(sh.redf));
-    const float M = block_reduce(ms.m, MaxOp(), -INFINITY, sh.redf);
-    const float S = block_reduce(ms.at(M, c), AddOp(), 0.f, sh.redf);
+    const Ref ref(block_reduce(ms.ref.m, MaxOp(), -INFINITY, sh.redf), c);
+    const float S = block_reduce(ms.at(ref, c), AddOp(), 0.f, sh.redf);
     if (P > 1) cluster_wait();   // every CTA of the cluster has started
     SelShared* to = P > 1 ? cl.map_shared_rank(&sh, 0) : &sh;
 #pragma unroll
@@ -228,7 +220,7 @@ __device__ __forceinline__ void push_groups(SelShared& sh, int p, int P, float (
         if (u < per) to->group[(p * per + u) * kSelThreads + tid] = ordered(top[u]);
     if (tid == 0) {
         to->part_j[p] = static_cast<int>(first);
-        to->part_m[p] = M;
+        to->part_m[p] = ref.m;
         to->part_s[p] = S;
     }
     if (P > 1) cl.sync();
@@ -239,14 +231,15 @@ __device__ __forceinline__ float unordered(uint32_t o) {
     return o == 0xffffffffu ? NAN : __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
 }
 
-// What the parts say of the row: its maximum (NaN if there is one) and, relative
-// to it, the sum.
+// What the parts say of the row: its maximum (NaN if there is one) and the sum of
+// weights relative to it (Ref), if it is finite.
 __device__ __forceinline__ void row_stats(const SelShared& sh, int P, float c, float& m, float& s) {
     uint32_t first = 0u;
     for (int p = 0; p < P; ++p) first = max(first, static_cast<uint32_t>(sh.part_j[p]));
     m = unordered(first);
     s = 0.f;
-    for (int p = 0; p < P; ++p) s += sh.part_m[p] > -INFINITY ? sh.part_s[p] * exp2_fast((sh.part_m[p] - m) * c) : 0.f;
+    const Ref ref(m, c);
+    for (int p = 0; p < P; ++p) s += sh.part_m[p] > -INFINITY ? sh.part_s[p] * Ref(sh.part_m[p], c).rescale(ref, c) : 0.f;
 }
 
 // The first n <= kSelList keys of sh.list into descending order.
@@ -281,7 +274,7 @@ __device__ void sort_list(SelShared& sh, int n) {
 
 // Rank 0: the K largest entries of the row into sh.list, in descending order.
 template <class T>
-__device__ void sort_top(SelShared& sh, const RowWords<T>& w, int P, int K) {
+__device__ void sort_top(SelShared& sh, const RowWords<T>& w, int log_P, int K) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint32_t g[8];
 #pragma unroll
@@ -315,8 +308,8 @@ __device__ void sort_top(SelShared& sh, const RowWords<T>& w, int P, int K) {
     for (int i = 0; i < 8; ++i)
         if (g[i] >= t) sh.chosen[atomicAdd(&sh.n_chosen, 1)] = static_cast<uint16_t>(i * kSelThreads + tid);
     __syncthreads();
-    const int per = 8 / P, chosen = sh.n_chosen;
-    const int rounds = ((w.words + P - 1) / P + kSelThreads * per - 1) / (kSelThreads * per);   // words of a group
+    const int per = 8 >> log_P, chosen = sh.n_chosen;
+    const int rounds = (((w.words - 1) >> log_P) + kSelThreads * per) / (kSelThreads * per);   // words of a group, or more
     const uint64_t floor = static_cast<uint64_t>(t) << 48;
     const auto take = [&](uint4 x, int j0) {
         float v[kRowVec<T>];
@@ -340,7 +333,7 @@ __device__ void sort_top(SelShared& sh, const RowWords<T>& w, int P, int K) {
             at[u] = -1;
             if (i < chosen * rounds) {
                 const int q = sh.chosen[i / rounds], p = q / (kSelThreads * per), r = q % (kSelThreads * per);
-                const Chunk ch(w.words, p, P);
+                const Chunk ch(w.words, p, log_P);
                 const int word = ch.lo + r % kSelThreads + (r / kSelThreads + (i % rounds) * per) * kSelThreads;
                 if (word < ch.hi && w.whole(word)) {
                     at[u] = word;
@@ -379,7 +372,7 @@ __device__ void sort_top(SelShared& sh, const RowWords<T>& w, int P, int K) {
 struct TopArgs {
     const void* z;
     DwaLogitsDims d;
-    int K, P;
+    int K, P, log_P;
     float c, temperature;
     void* values;
     int32_t* indices;
@@ -392,24 +385,24 @@ __global__ void __launch_bounds__(kSelThreads, 4) top_logits_kernel(TopArgs a) {
     const int P = a.P, tid = threadIdx.x;
     if (P > 1) cluster_arrive_relaxed();
     pdl_enter();
-    const int64_t r = blockIdx.x / P;
-    const int p = blockIdx.x % P;
+    const uint32_t r = blockIdx.x >> a.log_P;
+    const int p = blockIdx.x & (P - 1);
     const RowWords<T> w(static_cast<const T*>(a.z) + row_offset(a.d, r), a.d.V);
     float top[8], edge;
     MaxSum ms;
-    scan_chunk<T, true>(w, Chunk(w.words, p, P), a.c, top, edge, ms);
+    scan_chunk<T, true>(w, Chunk(w.words, p, a.log_P), a.c, top, edge, ms);
     push_groups(sh, p, P, top, edge, ms, a.c);
     if (p != 0) return;
     if (tid == 0) {
         float m, s;
         row_stats(sh, P, a.c, m, s);
-        a.lse[r] = m != m || isinf(m) ? m : m / a.temperature + logf(s);
+        a.lse[r] = m != m || isinf(m) ? m : static_cast<float>(0.6931471805599453 * (Ref(m, a.c).a(a.c) + log2f(s)));
     }
-    sort_top(sh, w, P, a.K);
+    sort_top(sh, w, a.log_P, a.K);
     for (int k = tid; k < a.K; k += kSelThreads) {
         const unsigned long long key = sh.list[k];
-        static_cast<T*>(a.values)[r * a.K + k] = Elem<T>::from_f(unordered(static_cast<uint32_t>(key >> 32)));
-        a.indices[r * a.K + k] = key_index(key);
+        static_cast<T*>(a.values)[static_cast<int64_t>(r) * a.K + k] = Elem<T>::from_f(unordered(static_cast<uint32_t>(key >> 32)));
+        a.indices[static_cast<int64_t>(r) * a.K + k] = key_index(key);
     }
 }
 
@@ -422,7 +415,7 @@ struct SampleArgs {
     const float* noise;
     int64_t noise_stride;
     DwaSampleParams p;
-    int P;
+    int P, log_P;
     int32_t* tokens;
     float* logprobs;
 };
@@ -432,7 +425,7 @@ struct Request {
     float T, top_p, min_p;
     int k;   // entries that stay
     bool greedy;
-    __device__ __forceinline__ Request(const DwaSampleParams& q, int64_t r, int V) {
+    __device__ __forceinline__ Request(const DwaSampleParams& q, uint32_t r, int V) {
         T = q.temperature_rows ? q.temperature_rows[r] : q.temperature;
         k = q.top_k_rows ? q.top_k_rows[r] : q.top_k;
         top_p = q.top_p_rows ? q.top_p_rows[r] : q.top_p;
@@ -455,7 +448,7 @@ __device__ __forceinline__ unsigned long long race_key(float score, int j) {
 }
 
 template <class T>
-__device__ __forceinline__ void write_token(const SampleArgs& a, const RowWords<T>& w, int64_t r, const Request& q,
+__device__ __forceinline__ void write_token(const SampleArgs& a, const RowWords<T>& w, uint32_t r, const Request& q,
                                             float m, unsigned long long best, double kept) {
     const int j = best ? key_index(best) : -1;
     a.tokens[r] = j;
@@ -718,7 +711,7 @@ __device__ void sample_wide(SelShared& sh, const SampleArgs& a, const RowWords<T
 // mass that top_p is a part of, or negative for that of these entries.  False if
 // entries beyond the n may be kept too (then nothing is written).
 template <class T>
-__device__ bool sample_listed(SelShared& sh, const SampleArgs& a, const RowWords<T>& w, int64_t r, const Request& q,
+__device__ bool sample_listed(SelShared& sh, const SampleArgs& a, const RowWords<T>& w, uint32_t r, const Request& q,
                               const float* noise, float m, int n, double total, bool complete) {
     constexpr int MOST = DWA_MAX_TOP / kSelThreads;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -788,18 +781,23 @@ __device__ __forceinline__ void race_chunk(const RowWords<T>& w, Chunk ch, float
     w.template each<2>(ch.lo, ch.hi, threadIdx.x, kSelThreads, [&](uint4 x, int j0, int) {
         const float m = word_max<T>(x);
         top = max_nan(top, m);
-        if (m > ms.m) {
-            const float f = exp2_fast((ms.m - m) * c);
-            best = f > 0.f ? best * f : 0.f;
+        if (!ms.covers(m)) {
+            const Ref old = ms.ref;
             ms.raise(m, c);
+            if (old.m > -INFINITY && ms.ref.m > old.m) {
+                const float f = old.rescale(ms.ref, c);
+                best = f > 0.f ? best * f : 0.f;
+            }
+            if (ms.ref.m == -INFINITY) return;
         }
-        if (ms.m == -INFINITY) return;
         float e[VEC], score[VEC];
-        word_exp<T>(x, ms.m, c, e);
+        uint64_t e2[VEC / 2];
+        word_weights<T>(x, ms.ref, c, e2);
+        ms.s2 = add2(ms.s2, sum_pairs<T>(e2));
+        unpair_word<T>(e2, e);
         float lead = -1.f;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            ms.s += e[i];
             score[i] = -1.f;
             if (e[i] > 0.f) score[i] = __fdividef(e[i], noise[j0 + i]);   // e > 0 only inside the row
             lead = fmaxf(lead, score[i]);
@@ -822,13 +820,13 @@ __global__ void __launch_bounds__(kSelThreads, 4) sample_kernel(SampleArgs a) {
     const int P = a.P, tid = threadIdx.x;
     if (P > 1) cluster_arrive_relaxed();
     pdl_enter();
-    const int64_t r = blockIdx.x / P;
-    const int p = blockIdx.x % P, V = a.d.V;
+    const uint32_t r = blockIdx.x >> a.log_P;
+    const int p = blockIdx.x & (P - 1), V = a.d.V;
     const RowWords<T> w(static_cast<const T*>(a.z) + row_offset(a.d, r), V);
     const Request q(a.p, r, V);
-    const float* noise = a.noise + r * a.noise_stride;
+    const float* noise = a.noise + static_cast<int64_t>(r) * a.noise_stride;
     const float c = kLog2e / q.T;
-    const Chunk ch(w.words, p, P);
+    const Chunk ch(w.words, p, a.log_P);
     const bool limited = q.top_p < 1.f || q.min_p > 0.f;
     const bool whole = q.k == V && !limited, list = !whole && q.k <= DWA_MAX_TOP;
     MaxSum ms;
@@ -838,16 +836,16 @@ __global__ void __launch_bounds__(kSelThreads, 4) sample_kernel(SampleArgs a) {
         float top, best;
         int j;
         race_chunk(w, ch, c, noise, ms, top, best, j);
-        const float M = block_reduce(ms.m, MaxOp(), -INFINITY, sh.redf);
-        const float S = block_reduce(ms.at(M, c), AddOp(), 0.f, sh.redf);
+        const Ref ref(block_reduce(ms.ref.m, MaxOp(), -INFINITY, sh.redf), c);
+        const float S = block_reduce(ms.at(ref, c), AddOp(), 0.f, sh.redf);
         const uint32_t first = block_reduce(ordered(top), MaxOp(), 0u, reinterpret_cast<uint32_t*>(sh.redf));
         const unsigned long long won =
-            block_reduce(j >= 0 ? race_key(best * exp2_fast((ms.m - M) * c), j) : 0ull, MaxOp(), 0ull, sh.red64);
+            block_reduce(j >= 0 ? race_key(best * ms.ref.rescale(ref, c), j) : 0ull, MaxOp(), 0ull, sh.red64);
         if (P > 1) cluster_wait();
         SelShared* to = cg::this_cluster().map_shared_rank(&sh, 0);
         if (tid == 0) {
             to->part_j[p] = static_cast<int>(first);
-            to->part_m[p] = M;
+            to->part_m[p] = ref.m;
             to->part_s[p] = S;
             to->part_lo[p] = won;
         }
@@ -860,11 +858,12 @@ __global__ void __launch_bounds__(kSelThreads, 4) sample_kernel(SampleArgs a) {
                 for (int i = 0; i < P; ++i) {
                     unsigned long long x = sh.part_lo[i];
                     if (!x) continue;
-                    x = race_key(__uint_as_float(static_cast<uint32_t>(x >> 32)) * exp2_fast((sh.part_m[i] - m) * c),
+                    x = race_key(__uint_as_float(static_cast<uint32_t>(x >> 32)) * Ref(sh.part_m[i], c).rescale(Ref(m, c), c),
                                  key_index(x));
                     best_of = x > best_of ? x : best_of;
                 }
-                write_token(a, w, r, q, m, best_of, s);
+                // the sum is relative to a, the entry to m
+                write_token(a, w, r, q, m, best_of, s * exp2(Ref(m, c).a(c) - static_cast<double>(m) * c));
             }
         }
     } else {
@@ -878,8 +877,9 @@ __global__ void __launch_bounds__(kSelThreads, 4) sample_kernel(SampleArgs a) {
             // a mass relative to +inf, or of the k largest of many, is not at hand
             if (m > -INFINITY && (list || (m < INFINITY && (masses || q.top_p >= 1.f) && limited))) {
                 const int n = list ? q.k : kTryTop;
-                sort_top(sh, w, P, n);
-                done = sample_listed(sh, a, w, r, q, noise, m, n, masses ? s : -1., list);
+                sort_top(sh, w, a.log_P, n);
+                done = sample_listed(sh, a, w, r, q, noise, m, n,
+                                     masses ? s * exp2(Ref(m, c).a(c) - static_cast<double>(m) * c) : -1., list);
             }
         }
         if (list && p != 0) return;
@@ -900,12 +900,12 @@ __global__ void __launch_bounds__(kSelThreads, 4) sample_kernel(SampleArgs a) {
 
 // CTAs per row: while the launch has room on the GPU (four CTAs an SM) and each
 // CTA at least a word a thread.
-static int ctas_per_row(const DwaLogitsDims& d) {
+static int log_ctas_per_row(const DwaLogitsDims& d) {
     const int64_t room = 4 * static_cast<int64_t>(tc::sm_count());
     const int words = d.V / (16 / static_cast<int>(dtype_bytes(d.dtype)));
-    int P = kSelMaxCluster;
-    while (P > 1 && (d.rows * P > room || words < P * kSelThreads)) P /= 2;
-    return P;
+    int l = 3;
+    while (l > 0 && (d.rows << l > room || words < kSelThreads << l)) --l;
+    return l;
 }
 
 template <class K, class A>
@@ -931,7 +931,8 @@ extern "C" int dwa_top_logits(void* stream, const DwaLogitsDims* dims, const voi
     if (reinterpret_cast<uintptr_t>(logits) % dtype_bytes(dims->dtype) ||
         reinterpret_cast<uintptr_t>(values) % dtype_bytes(dims->dtype))
         return fail(DWA_ERR_INVALID_ARG, "top_logits: a pointer is not aligned to its element");
-    const TopArgs a = {logits, *dims, K, ctas_per_row(*dims), kLog2e / temperature, temperature, values, indices, lse};
+    const int log_P = log_ctas_per_row(*dims);
+    const TopArgs a = {logits, *dims, K, 1 << log_P, log_P, kLog2e / temperature, temperature, values, indices, lse};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dims->dtype == DWA_BF16) DWA_TIMED("top_logits", st, (launch_rows(top_logits_kernel<__nv_bfloat16>, a, st)));
     else DWA_TIMED("top_logits", st, (launch_rows(top_logits_kernel<float>, a, st)));
@@ -952,7 +953,8 @@ extern "C" int dwa_sample_tokens(void* stream, const DwaLogitsDims* dims, const 
         return fail(DWA_ERR_INVALID_ARG, "sample_tokens: a required pointer is NULL");
     if (reinterpret_cast<uintptr_t>(logits) % dtype_bytes(dims->dtype) || reinterpret_cast<uintptr_t>(noise) % 4)
         return fail(DWA_ERR_INVALID_ARG, "sample_tokens: a pointer is not aligned to its element");
-    const SampleArgs a = {logits, *dims, noise, noise_stride, *params, ctas_per_row(*dims), tokens, logprobs};
+    const int log_P = log_ctas_per_row(*dims);
+    const SampleArgs a = {logits, *dims, noise, noise_stride, *params, 1 << log_P, log_P, tokens, logprobs};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dims->dtype == DWA_BF16) DWA_TIMED("sample", st, (launch_rows(sample_kernel<__nv_bfloat16>, a, st)));
     else DWA_TIMED("sample", st, (launch_rows(sample_kernel<float>, a, st)));

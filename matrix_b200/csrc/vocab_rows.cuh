@@ -18,8 +18,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 template <class T> constexpr int kRowVec = 16 / static_cast<int>(sizeof(T));
 
-__device__ __forceinline__ int64_t row_offset(const DwaLogitsDims& d, int64_t r) {
-    return (r / d.rows_inner) * d.stride_outer + (r % d.rows_inner) * d.stride_inner;
+__device__ __forceinline__ int64_t row_offset(const DwaLogitsDims& d, uint32_t r) {   // rows < 2^28
+    if (d.rows_inner >= d.rows) return r * d.stride_inner;
+    const uint32_t inner = static_cast<uint32_t>(d.rows_inner), q = r / inner;
+    return q * d.stride_outer + (r - q * inner) * d.stride_inner;
 }
 
 template <class T>
@@ -83,6 +85,28 @@ __device__ __forceinline__ float word_max(uint4 w) {
     }
 }
 
+// Weights of one row or part of it, relative to a reference m (its largest value
+// so far): w(v) = exp2(v c - a) with a = m c rounded to fp32, one multiply-add and
+// one exp2 each.  The rounding of a scales all weights alike, so shares of their
+// sum do not see it, and logarithms are taken relative to a, not to m.  Where a
+// would overflow (rows at the ends of the type) w(v) = exp2((v - m) c).
+struct Ref {
+    float m = -INFINITY, neg_a = 0.f;
+    bool is_plain = true;
+    __device__ __forceinline__ Ref() {}
+    __device__ __forceinline__ Ref(float m_, float c)
+        : m(m_), neg_a(m_ == -INFINITY ? 0.f : -(m_ * c)), is_plain(fabsf(neg_a) < 1e37f) {}
+    __device__ __forceinline__ bool plain() const { return is_plain; }
+    __device__ __forceinline__ float weight(float v, float c) const {
+        return exp2_fast(plain() ? fmaf(v, c, neg_a) : (v - m) * c);
+    }
+    // the factor that makes weights relative to this one relative to `to` (both m > -inf)
+    __device__ __forceinline__ float rescale(const Ref& to, float c) const {
+        return exp2_fast(plain() && to.plain() ? to.neg_a - neg_a : (m - to.m) * c);
+    }
+    __device__ __forceinline__ double a(float c) const { return plain() ? -static_cast<double>(neg_a) : static_cast<double>(m) * c; }
+};
+
 // Pairs of floats in one 64-bit register: one instruction for two lanes.
 __device__ __forceinline__ uint64_t pair(float a, float b) {
     uint64_t r;
@@ -102,20 +126,44 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
 
-// e[i] = exp2((v[i] - m) * c) of one word
+// The weights of one word, in pairs.
 template <class T>
-__device__ __forceinline__ void word_exp(uint4 w, float m, float c, float* e) {
+__device__ __forceinline__ void word_weights(uint4 w, const Ref& ref, float c, uint64_t* e) {
     float v[kRowVec<T>];
     unpack<T>(w, v);
-    const uint64_t nm = pair(-m, -m), cc = pair(c, c);
+    uint64_t x[kRowVec<T> / 2];
+    const uint64_t cc = pair(c, c);
+    if (ref.plain()) {
+        const uint64_t na = pair(ref.neg_a, ref.neg_a);
 #pragma unroll
-    for (int i = 0; i < kRowVec<T>; i += 2) {
-        float a, b;
-        unpair(mul2(add2(pair(v[i], v[i + 1]), nm), cc), a, b);
-        e[i] = exp2_fast(a);
-        e[i + 1] = exp2_fast(b);
+        for (int i = 0; i < kRowVec<T> / 2; ++i) x[i] = fma2(pair(v[2 * i], v[2 * i + 1]), cc, na);
+    } else {
+        const uint64_t nm = pair(-ref.m, -ref.m);
+#pragma unroll
+        for (int i = 0; i < kRowVec<T> / 2; ++i) x[i] = mul2(add2(pair(v[2 * i], v[2 * i + 1]), nm), cc);
     }
+#pragma unroll
+    for (int i = 0; i < kRowVec<T> / 2; ++i) {
+        float p, q;
+        unpair(x[i], p, q);
+        e[i] = pair(exp2_fast(p), exp2_fast(q));
+    }
+}
+template <class T>
+__device__ __forceinline__ uint64_t sum_pairs(const uint64_t* e) {
+    if constexpr (kRowVec<T> == 8) return add2(add2(e[0], e[1]), add2(e[2], e[3]));
+    else return add2(e[0], e[1]);
+}
+template <class T>
+__device__ __forceinline__ void unpair_word(const uint64_t* e, float* o) {
+#pragma unroll
+    for (int i = 0; i < kRowVec<T> / 2; ++i) unpair(e[i], o[2 * i], o[2 * i + 1]);
 }
 
 // The words of one row.
@@ -133,6 +181,12 @@ struct RowWords {
     }
     __device__ __forceinline__ int first(int g) const { return g * kRowVec<T> - shift; }
     __device__ __forceinline__ bool whole(int g) const { return g >= full_lo && g < full_hi; }
+    // the i with tid + i n a whole word of [lo, hi): [first, last), counted from lo
+    __device__ __forceinline__ void own_whole(int lo, int hi, int tid, int n, int& from, int& to) const {
+        const int a = lo > full_lo ? lo : full_lo, b = hi < full_hi ? hi : full_hi;
+        from = a > lo + tid ? 1 : 0;   // a is lo or lo + 1
+        to = b > lo + tid ? (b - lo - tid + n - 1) / n : 0;
+    }
     __device__ __forceinline__ uint4 word(int g) const { return *reinterpret_cast<const uint4*>(row + first(g)); }
     // f(word, its first index) for a row's first and last word where they are not
     // whole (threads 0 and 1); -inf stands outside the row
@@ -174,6 +228,26 @@ struct RowWords {
     }
 };
 
+// The words [words p / P, words (p + 1) / P) of CTA p of the P = 2^log_P <= 8
+// that share a row (words < 2^28).
+struct Chunk {
+    int lo, hi;
+    __device__ __forceinline__ Chunk(int words, int p, int log_P)
+        : lo(words * p >> log_P), hi(words * (p + 1) >> log_P) {}
+};
+
+// One 16-byte word from global to shared memory, in the background.
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+                 "l"(from)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>   // until at most N of this thread's groups are on their way
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Block-wide reduction in a fixed order; every thread gets the result.  `red`
 // holds 33 values; consecutive calls may share it.
 template <class V, class Op>
@@ -201,17 +275,32 @@ struct AddOp {
     template <class V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
 };
 
-// The running maximum and sum of exp2((v - m) * c): one pass over the data.
+// The running reference and sum of weights: one pass over the data.  The
+// reference is not the largest value itself: it is raised only where a weight
+// would pass 2^20, so that hardly any word but the first does.
 struct MaxSum {
-    float m = -INFINITY, s = 0.f;
-    __device__ __forceinline__ void raise(float to, float c) {   // m becomes `to` if that is larger
-        if (to > m) {
-            s *= exp2_fast((m - to) * c);   // m = -inf: s is 0 and stays 0
-            m = to;
+    Ref ref;
+    float limit = -INFINITY;   // what the reference stands for at most
+    uint64_t s2 = 0;           // two sums
+    __device__ __forceinline__ bool covers(float top) const { return top <= limit; }   // false for NaN
+    __device__ __forceinline__ void raise(float to, float c) {
+        if (to > limit) {
+            const Ref r(to, c);
+            if (ref.m > -INFINITY) {
+                const float f = ref.rescale(r, c);
+                s2 = mul2(s2, pair(f, f));
+            }
+            ref = r;
+            limit = to + 20.f / c;
         }
     }
-    // the sum once the maximum of all is M
-    __device__ __forceinline__ float at(float M, float c) const { return m > -INFINITY ? s * exp2_fast((m - M) * c) : s; }
+    __device__ __forceinline__ void poison() { s2 = pair(NAN, NAN); }
+    // the sum relative to `all`
+    __device__ __forceinline__ float at(const Ref& all, float c) const {
+        float a, b;
+        unpair(s2, a, b);
+        return ref.m > -INFINITY ? (a + b) * ref.rescale(all, c) : a + b;
+    }
 };
 
 int check_logits(const DwaLogitsDims* d, const char* what);   // distill.cu

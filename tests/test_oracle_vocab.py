@@ -110,7 +110,7 @@ def _dims(**kw):
 
 @pytest.mark.parametrize("bad,code", [(dict(dtype=7), -1), (dict(V=0), -1), (dict(rows=-1), -1),
                                       (dict(rows_inner=0), -1), (dict(stride_inner=-64), -1),
-                                      (dict(stride_outer=-1), -1), (dict(V=(1 << 20) + 1), -2),
+                                      (dict(stride_outer=-1), -1), (dict(V=393217), -2),
                                       (dict(rows=1 << 31), -2)])
 def test_bad_logits_are_refused(lib, bad, code):
     from matrix_b200 import _lib
