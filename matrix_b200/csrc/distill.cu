@@ -83,9 +83,7 @@ __device__ __forceinline__ void log2_parts(float x, float& whole, float& rest) {
     rest = fabsf(l) < INFINITY ? log2f(ldexpf(x, -static_cast<int>(whole))) : l;
 }
 // log(x) with the relative precision of fp32 also where x is 1 - y with a small y.
-__device__ __forceinline__ double log_of_rest(double x, double y) {
-    return x > 0.5 ? log1pf(static_cast<float>(-y)) : logf(static_cast<float>(x));
-}
+__device__ __forceinline__ float log_of_rest(float x, float y) { return x > 0.5f ? log1pf(-y) : logf(x); }
 
 // dL/dx of a listed entry from its logits.
 __device__ __forceinline__ float listed_grad(const RowState& s, const DistillArgs& a, float zk, float tk) {
@@ -137,45 +135,42 @@ struct GradWriter {
     }
 };
 
-// What one warp of a row's CTAs hands to all of them.
-struct DistillPart {
-    double P, L, S_l;  // sum p; forward: sum p (log p - x), reverse: sum w (x - log p), x = log2(e) z / T ln 2; sum w
-    float m, S_u;      // reference; sum of the weights w of unlisted entries
-    int bad;
+// What the warps of a row's CTAs hand to all of them, a part each: a reference,
+// the sum of the weights w of unlisted entries, and over listed entries the sum of
+// w and, with x = log2(e) z / T ln 2, forward of p (log p - x), reverse of
+// w (x - log p).
+struct DistillParts {
+    double L[kDistillMaxCluster * kDistillWarps], S_l[kDistillMaxCluster * kDistillWarps];
+    float S_u[kDistillMaxCluster * kDistillWarps], m[kDistillMaxCluster * kDistillWarps];
+    int bad[kDistillMaxCluster];
 };
 
-__device__ __forceinline__ double warp_sum_d(double v) {
+__device__ __forceinline__ void warp_sum_d(double& u, double& v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    for (int o = 16; o > 0; o >>= 1) {
+        u += __shfl_xor_sync(0xffffffffu, u, o);
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
 }
 
-// A row's state from its parts, and its loss: one warp.
-__device__ __forceinline__ double finish_row(RowState& s, const DistillPart* part, const DistillArgs& a, int valid) {
-    const int lane = threadIdx.x & 31;
-    double P = 0., S_u = 0., S_l = 0., L = 0.;
-    float m = -INFINITY;
-    int bad = 0;
-    for (int i = lane; i < a.P * kDistillWarps; i += 32) {
-        m = fmaxf(m, part[i].m);
-        bad |= part[i].bad;
-    }
-    s.m = warp_max(m);
-    bad = __any_sync(0xffffffffu, bad);
+// A row's state from its parts, and its loss: one warp.  P: the sum of the
+// teacher's probabilities.
+__device__ __forceinline__ double finish_row(RowState& s, const DistillParts& part, const DistillArgs& a, int valid,
+                                             double P) {
+    const int lane = threadIdx.x & 31, parts = a.P * kDistillWarps;
+    const bool one = lane < parts, two = lane + 32 < parts;
+    const float m0 = one ? part.m[lane] : -INFINITY, m1 = two ? part.m[lane + 32] : -INFINITY;
+    s.m = warp_max(fmaxf(m0, m1));
+    const bool bad = __any_sync(0xffffffffu, lane < a.P && part.bad[lane]);
     const Ref ref(s.m, a.c);
-    for (int i = lane; i < a.P * kDistillWarps; i += 32) {
-        const DistillPart& x = part[i];
-        // a part without anything above -inf: its sums are 0 (NaN with a NaN)
-        const double f = x.m > -INFINITY ? Ref(x.m, a.c).rescale(ref, a.c) : 1.f;
-        P += x.P;
-        S_u += f * x.S_u;
-        S_l += f * x.S_l;
-        L += a.o.reverse ? f * x.L : x.L;
-    }
-    P = warp_sum_d(P);
-    S_u = warp_sum_d(S_u);
-    S_l = warp_sum_d(S_l);
-    L = warp_sum_d(L);
+    // a part without anything above -inf: its sums are 0 (NaN with a NaN)
+    const float f0 = m0 > -INFINITY ? Ref(m0, a.c).rescale(ref, a.c) : 1.f;
+    const float f1 = m1 > -INFINITY ? Ref(m1, a.c).rescale(ref, a.c) : 1.f;
+    const float S_u = warp_sum((one ? f0 * part.S_u[lane] : 0.f) + (two ? f1 * part.S_u[lane + 32] : 0.f));
+    double S_l = (one ? f0 * part.S_l[lane] : 0.) + (two ? f1 * part.S_l[lane + 32] : 0.);
+    const double g0 = a.o.reverse ? f0 : 1.f, g1 = a.o.reverse ? f1 : 1.f;
+    double L = (one ? g0 * part.L[lane] : 0.) + (two ? g1 * part.L[lane + 32] : 0.);
+    warp_sum_d(S_l, L);
     const double S = S_u + S_l;
     s.S = static_cast<float>(S);
     log2_parts(s.S, s.log2_S_int, s.log2_S);
@@ -185,14 +180,15 @@ __device__ __forceinline__ double finish_row(RowState& s, const DistillPart* par
     else L += P != 0. ? P * log_S : 0.;
     s.of_tail = 1.f;
     if (a.t_lse && valid < a.d.V) {
-        const double p_t = fmax(1. - P, static_cast<double>(kTailFloor)), q_t = S_u / S;
-        if (q_t == 0.) {
+        const float p_t = fmaxf(static_cast<float>(1. - P), kTailFloor), q_t = S_u / s.S;
+        if (q_t == 0.f) {
             if (!a.o.reverse && p_t > kTailNone) L = INFINITY;
             s.of_tail = 0.f;
         } else {
-            const double r_t = log_of_rest(q_t, S_l / S) - log_of_rest(p_t, P);
+            const double r_t = static_cast<double>(log_of_rest(q_t, static_cast<float>(S_l) / s.S)) -
+                               log_of_rest(p_t, static_cast<float>(P));
             L += a.o.reverse ? q_t * r_t : -p_t * r_t;
-            s.of_tail = static_cast<float>(a.o.reverse ? r_t - L : 1. - p_t / q_t);
+            s.of_tail = a.o.reverse ? static_cast<float>(r_t - L) : 1.f - p_t / q_t;
         }
     }
     const bool nothing = valid == 0 || (!a.t_lse && s.t_hi == -INFINITY);
@@ -204,11 +200,11 @@ __device__ __forceinline__ double finish_row(RowState& s, const DistillPart* par
 // A cluster of P CTAs per row: the loss, the state for a backward (a.state) and,
 // with GRAD, the gradient of weight * L.
 template <class T, bool GRAD>
-__global__ void __launch_bounds__(kDistillThreads, 4) distill_fwd_kernel(const __grid_constant__ DistillArgs a) {
+__global__ void __launch_bounds__(kDistillThreads, 3) distill_fwd_kernel(const __grid_constant__ DistillArgs a) {
     namespace cg = cooperative_groups;
-    constexpr int VEC = kRowVec<T>;
+    constexpr int VEC = kRowVec<T>, MOST = DWA_MAX_TOP / kDistillThreads;
     extern __shared__ __align__(16) uint4 data[];
-    __shared__ DistillPart part[kDistillMaxCluster * kDistillWarps];
+    __shared__ DistillParts part;
     __shared__ double redd[33];
     __shared__ float redf[33];
     __shared__ RowState row_state;
@@ -217,31 +213,28 @@ __global__ void __launch_bounds__(kDistillThreads, 4) distill_fwd_kernel(const _
     const uint32_t r = blockIdx.x >> a.log_P;
     const int p = blockIdx.x & (a.P - 1);
     uint32_t* bits = reinterpret_cast<uint32_t*>(data + a.room);
-    float* tk = reinterpret_cast<float*>(bits + (a.room * VEC + 127) / 128 * 4);
-    int* at = reinterpret_cast<int*>(tk + K);   // a listed entry's place in the chunk, -1 elsewhere
     if (a.P > 1) cluster_arrive_relaxed();
     if (tid == 0) bad = valid = 0;
     pdl_enter();
+    // the teacher's loads first, then the chunk's copies, which they would wait behind
+    const int64_t rK = static_cast<int64_t>(r) * K;
+    int j[MOST];
+    float t[MOST];
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+        const int k = tid + i * kDistillThreads;
+        j[i] = -1;
+        t[i] = -INFINITY;
+        if (k < K) {
+            j[i] = a.idx[rK + k];
+            t[i] = load_elem(a.t, rK + k, a.o.teacher_dtype);
+        }
+    }
+    const float weight = a.weights ? a.weights[r] : 1.f, t_lse = a.t_lse ? a.t_lse[r] : 0.f;
     const RowWords<T> w(static_cast<const T*>(a.z) + row_offset(a.d, r), V);
     const Chunk ch(w.words, p, a.log_P);
     const int n = ch.hi - ch.lo;
     T* g = GRAD ? static_cast<T*>(a.g) + static_cast<int64_t>(r) * V : nullptr;
-    const int32_t* idx = a.idx + static_cast<int64_t>(r) * K;
-    const float weight = a.weights ? a.weights[r] : 1.f;
-    if (weight == 0.f) {   // a row left out: its logits and teacher are not looked at
-        RowState s = {};
-        s.kind = kRowZero;
-        if (p == 0 && tid == 0) {
-            a.loss[r] = 0.f;
-            if (a.state) a.state[r] = s;
-        }
-        if constexpr (GRAD) {
-            const GradWriter<T> write(w, g, s, a, 0.f);
-            for (int i = ch.lo + tid; i < ch.hi; i += kDistillThreads) write(make_uint4(0u, 0u, 0u, 0u), w.first(i));
-        }
-        if (a.P > 1) cluster_wait();
-        return;
-    }
     // the chunk, in pieces: every thread copies the words that it will look at
     int from, to;
     w.own_whole(ch.lo, ch.hi, tid, kDistillThreads, from, to);
@@ -255,44 +248,63 @@ __global__ void __launch_bounds__(kDistillThreads, 4) distill_fwd_kernel(const _
         for (int k = piece(i); k < end; ++k) copy_async(own_words + k * kDistillThreads, src + k * kDistillThreads);
         copy_commit();
     }
-    // meanwhile the teacher
     for (int i = tid; i < (n * VEC + 127) / 128; i += kDistillThreads)
         reinterpret_cast<uint4*>(bits)[i] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
-    int mine = 0;
-    float t_top = -INFINITY;
-    for (int k = tid; k < K; k += kDistillThreads) {
-        const int j = idx[k];
-        float t = -INFINITY;
-        int place = -1;
-        if (j >= V) {
-            bad = 1;
-        } else if (j >= 0) {
-            t = load_elem(a.t, static_cast<int64_t>(r) * K + k, a.o.teacher_dtype);
-            ++mine;
-            const int b = j + w.shift - ch.lo * VEC;
-            if (b >= 0 && b < n * VEC) {
-                place = b;
-                if (atomicOr(&bits[b >> 5], 1u << (b & 31)) & (1u << (b & 31))) bad = 1;
-            }
+    RowState s = {};
+    if (weight == 0.f) {   // a row left out, whatever it holds
+        s.kind = kRowZero;
+        if (p == 0 && tid == 0) {
+            a.loss[r] = 0.f;
+            if (a.state) a.state[r] = s;
         }
-        tk[k] = t;
-        at[k] = place;
-        t_top = fmaxf(t_top, t);
+        copy_wait<0>();
+        if constexpr (GRAD) {
+            const GradWriter<T> write(w, g, s, a, 0.f);
+            for (int i = ch.lo + tid; i < ch.hi; i += kDistillThreads) write(make_uint4(0u, 0u, 0u, 0u), w.first(i));
+        }
+        if (a.P > 1) cluster_wait();
+        return;
+    }
+    // the teacher: every CTA all of it, the places of the entries in its chunk
+    int mine = 0, at[MOST];
+    float t_top = -INFINITY, prob[MOST];
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+        at[i] = -1;
+        if (j[i] >= V) bad = 1;
+        if (j[i] < 0 || j[i] >= V) {
+            t[i] = -INFINITY;
+            continue;
+        }
+        ++mine;
+        const int b = j[i] + w.shift - ch.lo * VEC;
+        if (b >= 0 && b < n * VEC) {
+            at[i] = b;
+            if (atomicOr(&bits[b >> 5], 1u << (b & 31)) & (1u << (b & 31))) bad = 1;
+        }
+        t_top = fmaxf(t_top, t[i]);
     }
     if (mine) atomicAdd(&valid, mine);
-    RowState s = {};
     if (a.t_lse) {
-        s.t_lo = a.t_lse[r];
-        __syncthreads();
+        s.t_lo = t_lse;
     } else {
         s.t_hi = block_reduce(t_top, MaxOp(), -INFINITY, redf);
         double sum = 0.;
-        for (int k = tid; k < K; k += kDistillThreads)
-            if (tk[k] > -INFINITY) sum += expf(static_cast<float>((static_cast<double>(tk[k]) - s.t_hi) * a.inv_T));
+#pragma unroll
+        for (int i = 0; i < MOST; ++i)
+            if (t[i] > -INFINITY) sum += expf(static_cast<float>((static_cast<double>(t[i]) - s.t_hi) * a.inv_T));
         s.t_lo = logf(static_cast<float>(block_reduce(sum, AddOp(), 0., redd)));
     }
-    // one pass: the chunk's maximum, and the sum over unlisted entries
+    const auto log_p = [&](float x) { return (static_cast<double>(x) - s.t_hi) * a.inv_T - s.t_lo; };
+    double P = 0.;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+        prob[i] = t[i] == -INFINITY ? 0.f : expf(static_cast<float>(log_p(t[i])));
+        if (tid + i * kDistillThreads < K) P += prob[i];
+    }
+    P = block_reduce(P, AddOp(), 0., redd);   // its barriers also order the bitmap
+    // one pass: the sum of the weights of unlisted entries
     MaxSum ms;
     const uint8_t* byte = reinterpret_cast<const uint8_t*>(bits);
     const auto add_word = [&](uint4 x, int k) {
@@ -334,53 +346,55 @@ __global__ void __launch_bounds__(kDistillThreads, 4) distill_fwd_kernel(const _
     copy_wait<0>();
     add(3);
     __syncthreads();   // the listed entries may be other threads' words
-    const Ref ref(warp_max(ms.ref.m), a.c);   // the warp's
-    DistillPart own = {0., 0., 0., ref.m, warp_sum(ms.at(ref, a.c)), bad};
-    // the warp's share of the chunk's listed entries
-    float z_top = ref.m;
-    for (int k = tid; k < K; k += kDistillThreads)
-        if (at[k] >= 0) z_top = fmaxf(z_top, Elem<T>::to_f(reinterpret_cast<const T*>(data)[at[k]]));
-    const Ref all(warp_max(z_top), a.c);
-    if (ref.m > -INFINITY) own.S_u *= ref.rescale(all, a.c);
-    own.m = all.m;
+    // the warp's part: what it summed, and its listed entries of this chunk
+    float z[MOST], top = ms.ref.m;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+        z[i] = -INFINITY;
+        if (at[i] >= 0) z[i] = Elem<T>::to_f(reinterpret_cast<const T*>(data)[at[i]]);
+        top = fmaxf(top, z[i]);
+    }
+    const Ref ref(warp_max(top), a.c);
+    const float S_u = warp_sum(ms.at(ref, a.c));
+    double S_l = 0., L = 0.;
     if (warp * 32 < K) {
-        for (int k = tid; k < K; k += kDistillThreads) {
-            if (at[k] < 0) continue;
-            const float z = Elem<T>::to_f(reinterpret_cast<const T*>(data)[at[k]]);
-            const double lp = (static_cast<double>(tk[k]) - s.t_hi) * a.inv_T - s.t_lo, x = kLn2 * a.c * z;
-            const float e = z == -INFINITY ? 0.f : all.weight(z, a.c);   // the reference may be -inf too
-            const float prob = tk[k] == -INFINITY ? 0.f : expf(static_cast<float>(lp));
-            own.S_l += e;
-            own.P += prob;
-            if (a.o.reverse) own.L += e != 0.f ? e * (x - lp) : 0.;
-            else own.L += prob != 0.f ? prob * (lp - x) : 0.;
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) {
+            if (at[i] < 0) continue;
+            const double lp = log_p(t[i]), x = kLn2 * a.c * z[i];
+            const float e = z[i] == -INFINITY ? 0.f : ref.weight(z[i], a.c);   // the reference may be -inf too
+            S_l += e;
+            if (a.o.reverse) L += e != 0.f ? e * (x - lp) : 0.;
+            else L += prob[i] != 0.f ? prob[i] * (lp - x) : 0.;
         }
-        own.S_l = warp_sum_d(own.S_l);
-        own.P = warp_sum_d(own.P);
-        own.L = warp_sum_d(own.L);
+        warp_sum_d(S_l, L);
     }
-    if (a.P > 1) {
-        cluster_wait();   // every CTA of the cluster has started
-        if (lane < a.P) *cg::this_cluster().map_shared_rank(&part[p * kDistillWarps + warp], lane) = own;
-        cg::this_cluster().sync();
-    } else {
-        if (lane == 0) part[warp] = own;
-        __syncthreads();
+    if (a.P > 1) cluster_wait();   // every CTA of the cluster has started
+    if (lane < a.P) {              // lane q: to CTA q
+        DistillParts& to_q = *cg::this_cluster().map_shared_rank(&part, lane);
+        const int i = p * kDistillWarps + warp;
+        to_q.m[i] = ref.m;
+        to_q.S_u[i] = S_u;
+        to_q.S_l[i] = S_l;
+        to_q.L[i] = L;
+        if (warp == 0) to_q.bad[p] = bad;
     }
+    if (a.P > 1) cg::this_cluster().sync();
+    else __syncthreads();
     if (!GRAD && p != 0) return;
     if (warp == 0) {
-        const double L = finish_row(s, part, a, valid);
+        const double loss = finish_row(s, part, a, valid, P);
         if (lane == 0) row_state = s;
         if (p == 0 && lane == 0) {
             if (s.kind == kRowBad) raise_status(a.status, DWA_STATUS_BAD_TOKEN);
-            a.loss[r] = static_cast<float>(L * weight);
+            a.loss[r] = static_cast<float>(loss * weight);
             if (a.state) a.state[r] = s;
         }
     }
     if constexpr (GRAD) {
         __syncthreads();
         s = row_state;
-        const float scale = weight / a.o.temperature;
+        const float scale = weight * static_cast<float>(a.inv_T);
         const GradWriter<T> write(w, g, s, a, scale);
         if (write.fast) {
             uint4* const to_g = reinterpret_cast<uint4*>(g + w.first(ch.lo + tid));
@@ -392,11 +406,9 @@ __global__ void __launch_bounds__(kDistillThreads, 4) distill_fwd_kernel(const _
         }
         if (s.kind != kRowPlain) return;
         __syncthreads();
-        for (int k = tid; k < K; k += kDistillThreads) {
-            if (at[k] < 0) continue;
-            const float z = Elem<T>::to_f(reinterpret_cast<const T*>(data)[at[k]]);
-            g[at[k] + w.first(ch.lo)] = Elem<T>::from_f(listed_grad(s, a, z, tk[k]) * scale);
-        }
+#pragma unroll
+        for (int i = 0; i < MOST; ++i)
+            if (at[i] >= 0) g[j[i]] = Elem<T>::from_f(listed_grad(s, a, z[i], t[i]) * scale);
     }
 }
 
@@ -420,7 +432,7 @@ __global__ void __launch_bounds__(kDistillThreads) distill_bwd_kernel(const __gr
             if (here(idx[k])) zk[k] = Elem<T>::to_f(w.row[idx[k]]);
         __syncthreads();
     }
-    const float scale = (a.weights ? a.weights[r] : 1.f) * a.g_loss[r] / a.o.temperature;
+    const float scale = (a.weights ? a.weights[r] : 1.f) * a.g_loss[r] * static_cast<float>(a.inv_T);
     T* g = static_cast<T*>(a.g) + static_cast<int64_t>(r) * V;
     const GradWriter<T> write(w, g, s, a, scale);
     if (write.fast) {
@@ -501,8 +513,7 @@ static int launch_fwd(cudaStream_t st, DistillArgs a) {
     a.log_P = log_ctas_per_row(a.d);
     a.P = 1 << a.log_P;
     a.room = (a.d.V + 2 * VEC - 2) / VEC / a.P + 1;
-    const size_t sh = static_cast<size_t>(a.room) * 16 + (static_cast<size_t>(a.room) * VEC + 127) / 128 * 16 +
-                      static_cast<size_t>(a.o.K) * 8;
+    const size_t sh = static_cast<size_t>(a.room) * 16 + (static_cast<size_t>(a.room) * VEC + 127) / 128 * 16;
     if (int rc = allow_smem(distill_fwd_kernel<T, GRAD>, sh)) return rc;
     DWA_TIMED("distill_fwd", st, (launch_pdl_cluster(distill_fwd_kernel<T, GRAD>, dim3(static_cast<unsigned>(a.d.rows * a.P)),
                                                      dim3(kDistillThreads), sh, st, dim3(a.P), a)));
