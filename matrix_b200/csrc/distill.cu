@@ -33,9 +33,11 @@ namespace dwa {
 
 extern std::atomic<uint64_t> g_launches_total;
 
-constexpr int kDistillThreads = 256;
-constexpr int kDistillWarps = kDistillThreads / 32;
+constexpr int kDistillThreads = 256;             // a CTA of a cluster that holds a row
+constexpr int kStreamThreads = 512;              // a CTA that reads a row twice
+constexpr int kRing = 5;                         // stages of two words a thread that such a CTA has in flight
 constexpr int kDistillMaxCluster = 8;
+constexpr int kDistillMaxParts = 64;             // warps that share a row
 constexpr int kDistillPieces = 4;                // pieces in which a chunk arrives
 constexpr int kDistillChunkBytes = 72 * 1024;    // three CTAs an SM
 constexpr float kTailFloor = 5.9604645e-8f;      // 2^-24: what an fp32 log-sum-exp can tell from no tail
@@ -140,8 +142,8 @@ struct GradWriter {
 // w and, with x = log2(e) z / T ln 2, forward of p (log p - x), reverse of
 // w (x - log p).
 struct DistillParts {
-    double L[kDistillMaxCluster * kDistillWarps], S_l[kDistillMaxCluster * kDistillWarps];
-    float S_u[kDistillMaxCluster * kDistillWarps], m[kDistillMaxCluster * kDistillWarps];
+    double L[kDistillMaxParts], S_l[kDistillMaxParts];
+    float S_u[kDistillMaxParts], m[kDistillMaxParts];
     int bad[kDistillMaxCluster];
 };
 
@@ -156,8 +158,8 @@ __device__ __forceinline__ void warp_sum_d(double& u, double& v) {
 // A row's state from its parts, and its loss: one warp.  P: the sum of the
 // teacher's probabilities.
 __device__ __forceinline__ double finish_row(RowState& s, const DistillParts& part, const DistillArgs& a, int valid,
-                                             double P) {
-    const int lane = threadIdx.x & 31, parts = a.P * kDistillWarps;
+                                             double P, int parts) {
+    const int lane = threadIdx.x & 31;
     const bool one = lane < parts, two = lane + 32 < parts;
     const float m0 = one ? part.m[lane] : -INFINITY, m1 = two ? part.m[lane + 32] : -INFINITY;
     s.m = warp_max(fmaxf(m0, m1));
@@ -197,12 +199,53 @@ __device__ __forceinline__ double finish_row(RowState& s, const DistillParts& pa
     return bad ? NAN : nothing ? 0. : L;
 }
 
-// A cluster of P CTAs per row: the loss, the state for a backward (a.state) and,
-// with GRAD, the gradient of weight * L.
-template <class T, bool GRAD>
-__global__ void __launch_bounds__(kDistillThreads, 3) distill_fwd_kernel(const __grid_constant__ DistillArgs a) {
+// A thread's words of a row on their way through shared memory, kRing stages of
+// two words ahead, each pass right behind the one before.  Only the thread that
+// copies a word reads it, so nothing but its own copies is waited for.
+template <int NT>
+struct WordRing {
+    uint4* const slots;        // this thread's: 2 kRing of them, NT words apart
+    const uint4* const src;    // its words, NT apart
+    const int from, to;
+    int left, next, put = 0, get = 0;
+
+    __device__ __forceinline__ WordRing(uint4* slots_, const uint4* src_, int from_, int to_, int passes)
+        : slots(slots_), src(src_), from(from_), to(to_), left(passes), next(from_) {}
+    __device__ __forceinline__ void issue() {
+        if (next >= to && left > 0) {
+            --left;
+            next = from;
+        }
+        if (left > 0 && next < to) {
+            copy_async(slots + put * 2 * NT, src + next * NT);
+            if (next + 1 < to) copy_async(slots + (put * 2 + 1) * NT, src + (next + 1) * NT);
+            next += 2;
+        }
+        put = put + 1 == kRing ? 0 : put + 1;
+        copy_commit();
+    }
+    template <class F>
+    __device__ __forceinline__ void pass(F f) {   // f(word, its number) for all of them
+        for (int k = from; k < to; k += 2) {
+            copy_wait<kRing - 1>();
+            const uint4* x = slots + get * 2 * NT;
+            f(x[0], k);
+            if (k + 1 < to) f(x[NT], k + 1);
+            get = get + 1 == kRing ? 0 : get + 1;
+            issue();
+        }
+    }
+};
+
+// The loss of a row, the state for a backward (a.state) and, with GRAD, the
+// gradient of weight * L.  HOLD: a cluster of P CTAs holds the row in shared
+// memory; else one CTA reads it, and for the gradient once more out of L2.
+template <class T, bool GRAD, bool HOLD>
+__global__ void __launch_bounds__(HOLD ? kDistillThreads : kStreamThreads, HOLD ? 3 : 2)
+    distill_fwd_kernel(const __grid_constant__ DistillArgs a) {
     namespace cg = cooperative_groups;
-    constexpr int VEC = kRowVec<T>, MOST = DWA_MAX_TOP / kDistillThreads;
+    constexpr int NT = HOLD ? kDistillThreads : kStreamThreads, WARPS = NT / 32;
+    constexpr int VEC = kRowVec<T>, MOST = DWA_MAX_TOP / NT;
     extern __shared__ __align__(16) uint4 data[];
     __shared__ DistillParts part;
     __shared__ double redd[33];
@@ -212,7 +255,7 @@ __global__ void __launch_bounds__(kDistillThreads, 3) distill_fwd_kernel(const _
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.o.K, V = a.d.V;
     const uint32_t r = blockIdx.x >> a.log_P;
     const int p = blockIdx.x & (a.P - 1);
-    uint32_t* bits = reinterpret_cast<uint32_t*>(data + a.room);
+    uint32_t* bits = reinterpret_cast<uint32_t*>(data + (HOLD ? a.room : 2 * kRing * NT));
     if (a.P > 1) cluster_arrive_relaxed();
     if (tid == 0) bad = valid = 0;
     pdl_enter();
@@ -222,7 +265,7 @@ __global__ void __launch_bounds__(kDistillThreads, 3) distill_fwd_kernel(const _
     float t[MOST];
 #pragma unroll
     for (int i = 0; i < MOST; ++i) {
-        const int k = tid + i * kDistillThreads;
+        const int k = tid + i * NT;
         j[i] = -1;
         t[i] = -INFINITY;
         if (k < K) {
@@ -237,18 +280,27 @@ __global__ void __launch_bounds__(kDistillThreads, 3) distill_fwd_kernel(const _
     T* g = GRAD ? static_cast<T*>(a.g) + static_cast<int64_t>(r) * V : nullptr;
     // the chunk, in pieces: every thread copies the words that it will look at
     int from, to;
-    w.own_whole(ch.lo, ch.hi, tid, kDistillThreads, from, to);
+    w.own_whole(ch.lo, ch.hi, tid, NT, from, to);
     uint4* const own_words = data + tid;
+    float z[MOST];   // the listed entries' logits
     const auto piece = [&](int i) { return from + (to - from) * i / kDistillPieces; };
     const uint4* const src = reinterpret_cast<const uint4*>(w.row + w.first(ch.lo + tid));
+    WordRing<NT> ring(own_words, src, from, to, GRAD ? 2 : 1);
+    if constexpr (HOLD) {
 #pragma unroll
-    for (int i = 0; i < kDistillPieces; ++i) {
-        const int end = piece(i + 1);
+        for (int i = 0; i < kDistillPieces; ++i) {
+            const int end = piece(i + 1);
 #pragma unroll 4
-        for (int k = piece(i); k < end; ++k) copy_async(own_words + k * kDistillThreads, src + k * kDistillThreads);
-        copy_commit();
+            for (int k = piece(i); k < end; ++k) copy_async(own_words + k * NT, src + k * NT);
+            copy_commit();
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kRing; ++i) ring.issue();
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) z[i] = j[i] >= 0 && j[i] < V ? Elem<T>::to_f(w.row[j[i]]) : -INFINITY;
     }
-    for (int i = tid; i < (n * VEC + 127) / 128; i += kDistillThreads)
+    for (int i = tid; i < (n * VEC + 127) / 128; i += NT)
         reinterpret_cast<uint4*>(bits)[i] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
     RowState s = {};
@@ -261,7 +313,7 @@ __global__ void __launch_bounds__(kDistillThreads, 3) distill_fwd_kernel(const _
         copy_wait<0>();
         if constexpr (GRAD) {
             const GradWriter<T> write(w, g, s, a, 0.f);
-            for (int i = ch.lo + tid; i < ch.hi; i += kDistillThreads) write(make_uint4(0u, 0u, 0u, 0u), w.first(i));
+            for (int i = ch.lo + tid; i < ch.hi; i += NT) write(make_uint4(0u, 0u, 0u, 0u), w.first(i));
         }
         if (a.P > 1) cluster_wait();
         return;
@@ -301,7 +353,7 @@ __global__ void __launch_bounds__(kDistillThreads, 3) distill_fwd_kernel(const _
 #pragma unroll
     for (int i = 0; i < MOST; ++i) {
         prob[i] = t[i] == -INFINITY ? 0.f : expf(static_cast<float>(log_p(t[i])));
-        if (tid + i * kDistillThreads < K) P += prob[i];
+        if (tid + i * NT < K) P += prob[i];
     }
     P = block_reduce(P, AddOp(), 0., redd);   // its barriers also order the bitmap
     // one pass: the sum of the weights of unlisted entries
@@ -326,34 +378,37 @@ __global__ void __launch_bounds__(kDistillThreads, 3) distill_fwd_kernel(const _
         }
         ms.s2 = add2(ms.s2, sum_pairs<T>(e));
     };
-    const auto add = [&](int i) {
-        const int end = piece(i + 1);
-#pragma unroll 2
-        for (int k = piece(i); k < end; ++k) add_word(own_words[k * kDistillThreads], tid + k * kDistillThreads);
-    };
     w.edges(ch.lo, ch.hi, tid, [&](uint4 x, int j0) {
         const int k = (j0 + w.shift) / VEC - ch.lo;
-        data[k] = x;
+        if constexpr (HOLD) data[k] = x;
         add_word(x, k);
     });
-    static_assert(kDistillPieces == 4, "one wait a piece");
-    copy_wait<3>();
-    add(0);
-    copy_wait<2>();
-    add(1);
-    copy_wait<1>();
-    add(2);
-    copy_wait<0>();
-    add(3);
-    __syncthreads();   // the listed entries may be other threads' words
-    // the warp's part: what it summed, and its listed entries of this chunk
-    float z[MOST], top = ms.ref.m;
+    if constexpr (HOLD) {
+        const auto add = [&](int i) {
+            const int end = piece(i + 1);
+#pragma unroll 2
+            for (int k = piece(i); k < end; ++k) add_word(own_words[k * NT], tid + k * NT);
+        };
+        static_assert(kDistillPieces == 4, "one wait a piece");
+        copy_wait<3>();
+        add(0);
+        copy_wait<2>();
+        add(1);
+        copy_wait<1>();
+        add(2);
+        copy_wait<0>();
+        add(3);
+        __syncthreads();   // the listed entries may be other threads' words
 #pragma unroll
-    for (int i = 0; i < MOST; ++i) {
-        z[i] = -INFINITY;
-        if (at[i] >= 0) z[i] = Elem<T>::to_f(reinterpret_cast<const T*>(data)[at[i]]);
-        top = fmaxf(top, z[i]);
+        for (int i = 0; i < MOST; ++i)
+            z[i] = at[i] >= 0 ? Elem<T>::to_f(reinterpret_cast<const T*>(data)[at[i]]) : -INFINITY;
+    } else {
+        ring.pass([&](uint4 x, int k) { add_word(x, tid + k * NT); });
     }
+    // the warp's part: what it summed, and its listed entries of this chunk
+    float top = ms.ref.m;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) top = fmaxf(top, z[i]);
     const Ref ref(warp_max(top), a.c);
     const float S_u = warp_sum(ms.at(ref, a.c));
     double S_l = 0., L = 0.;
@@ -372,7 +427,7 @@ __global__ void __launch_bounds__(kDistillThreads, 3) distill_fwd_kernel(const _
     if (a.P > 1) cluster_wait();   // every CTA of the cluster has started
     if (lane < a.P) {              // lane q: to CTA q
         DistillParts& to_q = *cg::this_cluster().map_shared_rank(&part, lane);
-        const int i = p * kDistillWarps + warp;
+        const int i = p * WARPS + warp;
         to_q.m[i] = ref.m;
         to_q.S_u[i] = S_u;
         to_q.S_l[i] = S_l;
@@ -383,7 +438,7 @@ __global__ void __launch_bounds__(kDistillThreads, 3) distill_fwd_kernel(const _
     else __syncthreads();
     if (!GRAD && p != 0) return;
     if (warp == 0) {
-        const double loss = finish_row(s, part, a, valid, P);
+        const double loss = finish_row(s, part, a, valid, P, a.P * WARPS);
         if (lane == 0) row_state = s;
         if (p == 0 && lane == 0) {
             if (s.kind == kRowBad) raise_status(a.status, DWA_STATUS_BAD_TOKEN);
@@ -398,11 +453,20 @@ __global__ void __launch_bounds__(kDistillThreads, 3) distill_fwd_kernel(const _
         const GradWriter<T> write(w, g, s, a, scale);
         if (write.fast) {
             uint4* const to_g = reinterpret_cast<uint4*>(g + w.first(ch.lo + tid));
+            if constexpr (HOLD) {
 #pragma unroll 4
-            for (int k = from; k < to; ++k) write.whole(own_words[k * kDistillThreads], to_g + k * kDistillThreads);
+                for (int k = from; k < to; ++k) write.whole(own_words[k * NT], to_g + k * NT);
+            } else {
+                ring.pass([&](uint4 x, int k) { write.whole(x, to_g + k * NT); });
+            }
             w.edges(ch.lo, ch.hi, tid, write);
         } else {
-            for (int k = tid; k < n; k += kDistillThreads) write(data[k], w.first(ch.lo + k));
+            if constexpr (HOLD) {
+                for (int k = tid; k < n; k += NT) write(data[k], w.first(ch.lo + k));
+            } else {
+                ring.pass([&](uint4 x, int k) { write(x, w.first(tid + k * NT)); });
+                w.edges(ch.lo, ch.hi, tid, write);
+            }
         }
         if (s.kind != kRowPlain) return;
         __syncthreads();
@@ -495,9 +559,9 @@ static int allow_smem(K kernel, size_t bytes) {
     return DWA_OK;
 }
 
-// CTAs per row: enough that a chunk leaves room for three CTAs an SM (or fits at
-// all), more while the launch is short of two CTAs an SM and chunks stay above
-// 16 KB.
+// CTAs per row that hold it: enough that a chunk leaves room for three CTAs an SM
+// (or fits at all), more while the launch is short of two CTAs an SM and chunks
+// stay above 16 KB.
 static int log_ctas_per_row(const DwaLogitsDims& d) {
     const int64_t bytes = static_cast<int64_t>(d.V) * dtype_bytes(d.dtype);
     int l = 0;
@@ -507,19 +571,26 @@ static int log_ctas_per_row(const DwaLogitsDims& d) {
     return l;
 }
 
-template <class T, bool GRAD>
-static int launch_fwd(cudaStream_t st, DistillArgs a) {
-    constexpr int VEC = kRowVec<T>;
-    a.log_P = log_ctas_per_row(a.d);
+template <class T, bool GRAD, bool HOLD>
+static int launch_fwd_as(cudaStream_t st, DistillArgs a) {
+    constexpr int VEC = kRowVec<T>, NT = HOLD ? kDistillThreads : kStreamThreads;
+    a.log_P = HOLD ? log_ctas_per_row(a.d) : 0;
     a.P = 1 << a.log_P;
     a.room = (a.d.V + 2 * VEC - 2) / VEC / a.P + 1;
-    const size_t sh = static_cast<size_t>(a.room) * 16 + (static_cast<size_t>(a.room) * VEC + 127) / 128 * 16;
-    if (int rc = allow_smem(distill_fwd_kernel<T, GRAD>, sh)) return rc;
-    DWA_TIMED("distill_fwd", st, (launch_pdl_cluster(distill_fwd_kernel<T, GRAD>, dim3(static_cast<unsigned>(a.d.rows * a.P)),
-                                                     dim3(kDistillThreads), sh, st, dim3(a.P), a)));
+    const size_t sh = static_cast<size_t>(HOLD ? a.room : 2 * kRing * NT) * 16 + (static_cast<size_t>(a.room) * VEC + 127) / 128 * 16;
+    if (int rc = allow_smem(distill_fwd_kernel<T, GRAD, HOLD>, sh)) return rc;
+    DWA_TIMED("distill_fwd", st,
+              (launch_pdl_cluster(distill_fwd_kernel<T, GRAD, HOLD>, dim3(static_cast<unsigned>(a.d.rows * a.P)), dim3(NT),
+                                  sh, st, dim3(a.P), a)));
     DWA_LAUNCH_CHECK("distill_fwd_kernel");
     ++g_launches_total;
     return DWA_OK;
+}
+
+template <class T, bool GRAD>
+static int launch_fwd(cudaStream_t st, const DistillArgs& a) {
+    if (a.d.rows >= 2 * tc::sm_count()) return launch_fwd_as<T, GRAD, false>(st, a);
+    return launch_fwd_as<T, GRAD, true>(st, a);
 }
 
 }  // namespace dwa
