@@ -15,15 +15,20 @@
 // entries set apart.
 //
 // Bound: HBM.  The loss has to read the row once, the gradient to write it once;
-// everything else is K entries a row.  A cluster of P CTAs holds a row in its
-// shared memory (chunks of at most 72 KB, so that three CTAs share an SM and one
-// loads while another writes), so the gradient reads nothing again.  One pass
-// over the chunk keeps a running maximum and the sum of exp((z - max) / T) over
-// the UNLISTED entries alone (a bitmap of the chunk tells which, one byte per
-// 16-byte word of bf16): q_t as total minus listed would lose all its digits
-// where the listed entries hold nearly everything.  Row sums are kept in fp32;
-// what is left of a row (K terms and a few logarithms) is done in fp64, where
-// differences of logarithms keep the digits that fp32 would round away.
+// everything else is K entries a row.  The sum of weights runs over the UNLISTED
+// entries alone (a bitmap of the row tells which, one byte per 16-byte word of
+// bf16): q_t as total minus listed would lose all its digits where the listed
+// entries hold nearly everything.  Row sums are kept in fp32; what is left of a
+// row (K terms and a few logarithms) is done in fp64, where differences of
+// logarithms keep the digits that fp32 would round away.
+//
+// Where the rows fill the GPU, a CTA takes a row and, for the gradient, reads it a
+// second time out of L2 (rows in flight: 148 x 2 x 256 KB at most); else a cluster
+// of CTAs holds the row in shared memory, which puts more SMs on a row.  Measured
+// on a B200, 4096 x 131072 bf16: the loss 192 us (5.6 TB/s), with the gradient 456
+// us (4.7 TB/s of the 2.1 GB that it has to move; 521 us as two kernels, of which
+// the backward runs at 6.5 TB/s); 600 us when clusters of four hold each row,
+// because the CTAs of a cluster wait for the slowest.
 
 #include <atomic>
 
@@ -33,27 +38,33 @@ namespace dwa {
 
 extern std::atomic<uint64_t> g_launches_total;
 
-constexpr int kDistillThreads = 256;             // a CTA of a cluster that holds a row
-constexpr int kStreamThreads = 512;              // a CTA that reads a row twice
-constexpr int kRing = 5;                         // stages of two words a thread that such a CTA has in flight
+constexpr int kDistillThreads = 256;             // a CTA of the backward
+constexpr int kHoldThreads = 256;                // a CTA of a cluster that holds a row
+constexpr int kRing = 4;                         // stages of two words that a thread of a streaming CTA has in flight
 constexpr int kDistillMaxCluster = 8;
 constexpr int kDistillMaxParts = 64;             // warps that share a row
-constexpr int kDistillPieces = 4;                // pieces in which a chunk arrives
+constexpr int kHoldPieces = 2;                   // pieces in which a held chunk arrives
 constexpr int kDistillChunkBytes = 72 * 1024;    // three CTAs an SM
 constexpr float kTailFloor = 5.9604645e-8f;      // 2^-24: what an fp32 log-sum-exp can tell from no tail
 constexpr float kTailNone = 1.52587890625e-5f;   // 2^-16: a teacher's tail that may be its rounding alone
+
+constexpr double kLn2 = 0.6931471805599453;
 
 enum : int { kRowPlain = 0, kRowZero = 1, kRowBad = 2 };
 
 // What the backward needs of a row.
 struct RowState {
     float m, S;        // a reference and the sum of the student's weights relative to it (Ref)
-    float log2_S;      // log2 S less its rounding to an integer, and
-    float log2_S_int;  // that integer
+    float twos, rest;  // log S = twos log 2 + rest
     float of_tail;     // dL/dx of an unlisted entry over its q
     float L;           // the loss before its weight
     float t_hi, t_lo;  // log p_k = (t_k - t_hi) / T - t_lo
     float kind;        // kRowPlain, kRowZero (nothing to learn) or kRowBad
+    // log q = log2(e) z / T ln 2 - log_S
+    __device__ __forceinline__ double log_S(const Ref& ref, float c) const { return kLn2 * (ref.a(c) + twos) + rest; }
+    __device__ __forceinline__ double log_p(float t, double inv_T) const {
+        return (static_cast<double>(t) - t_hi) * inv_T - t_lo;
+    }
 };
 static_assert(sizeof(RowState) == DWA_DISTILL_STATE_FLOATS * sizeof(float), "layout of the saved row state");
 
@@ -76,26 +87,45 @@ struct DistillArgs {
     int room;      // words of the largest chunk
 };
 
-constexpr double kLn2 = 0.6931471805599453;
-
-// log2(x) as an integer and a rest in [-0.5, 0.5], which fp32 holds to 2^-25.
-__device__ __forceinline__ void log2_parts(float x, float& whole, float& rest) {
-    const float l = log2f(x);
-    whole = rintf(l);
-    rest = fabsf(l) < INFINITY ? log2f(ldexpf(x, -static_cast<int>(whole))) : l;
+// log((1 + s) / (1 - s)) for |s| <= 1/3, by its series.
+__device__ __forceinline__ float log_ratio(float s) {
+    const float q = s * s;
+    float r = 1.f / 15.f;
+    r = fmaf(r, q, 1.f / 13.f);
+    r = fmaf(r, q, 1.f / 11.f);
+    r = fmaf(r, q, 1.f / 9.f);
+    r = fmaf(r, q, 1.f / 7.f);
+    r = fmaf(r, q, 1.f / 5.f);
+    r = fmaf(r, q, 1.f / 3.f);
+    return 2.f * fmaf(r * q, s, s);
 }
-// log(x) with the relative precision of fp32 also where x is 1 - y with a small y.
-__device__ __forceinline__ float log_of_rest(float x, float y) { return x > 0.5f ? log1pf(-y) : logf(x); }
+// log(x) of a positive finite x as a multiple of log 2 and a rest, which fp32 holds
+// to 2^-24 of at most 0.41.
+__device__ __forceinline__ void log_parts(float x, float& twos, float& rest) {
+    if (!(x >= 1.17549435e-38f && x < INFINITY)) {   // zero, denormal, infinite or NaN
+        twos = 0.f;
+        rest = logf(x);
+        return;
+    }
+    const uint32_t u = __float_as_uint(x) - 0x3f400000u;   // the mantissa in [0.75, 1.5)
+    const float m = __uint_as_float((u & 0x007fffffu) + 0x3f400000u);
+    twos = static_cast<float>(static_cast<int32_t>(u) >> 23);
+    rest = log_ratio(__fdividef(m - 1.f, m + 1.f));
+}
+// log(x), x = 1 - y, with the relative precision of fp32 also where y is small.
+__device__ __forceinline__ float log_of_rest(float x, float y) {
+    return x > 0.5f ? log_ratio(__fdividef(-y, 2.f - y)) : logf(x);
+}
 
-// dL/dx of a listed entry from its logits.
-__device__ __forceinline__ float listed_grad(const RowState& s, const DistillArgs& a, float zk, float tk) {
+// dL/dx of a listed entry from its logit, the teacher's probability and its
+// logarithm.
+__device__ __forceinline__ float listed_grad(const RowState& s, const DistillArgs& a, float zk, float prob, double log_p) {
     const Ref ref(s.m, a.c);
     const float q = ref.weight(zk, a.c) / s.S;
-    const double lp = (static_cast<double>(tk) - s.t_hi) * a.inv_T - s.t_lo;
-    if (!a.o.reverse) return q - (tk == -INFINITY ? 0.f : expf(static_cast<float>(lp)));
+    if (!a.o.reverse) return q - prob;
     if (q == 0.f) return 0.f;
-    const double x = static_cast<double>(zk) * a.c, r = kLn2 * (x - ref.a(a.c) - s.log2_S_int - s.log2_S) - lp - s.L;
-    return fabs(r) > 1e-14 * (fabs(x) + fabs(lp)) ? q * static_cast<float>(r) : 0.f;   // else the terms' rounding
+    const double x = kLn2 * a.c * zk, r = x - s.log_S(ref, a.c) - log_p - s.L;
+    return fabs(r) > 1e-14 * (fabs(x) + fabs(log_p)) ? q * static_cast<float>(r) : 0.f;   // else the terms' rounding
 }
 
 // The unlisted entries' gradient of one row, word by word.
@@ -103,26 +133,25 @@ template <class T>
 struct GradWriter {
     T* g;          // the row's gradient
     int V;
-    bool fast;     // a plain row, and g has the phase of the logits
+    bool fast;     // a plain row with a plain reference, and g has the phase of the logits
     int kind;
     Ref ref;
     float c, unl;
 
     __device__ __forceinline__ GradWriter(const RowWords<T>& w, T* g_, const RowState& s, const DistillArgs& a, float scale)
         : g(g_), V(w.V), kind(static_cast<int>(s.kind)), ref(s.m, a.c), c(a.c) {
-        fast = kind == kRowPlain && (reinterpret_cast<uintptr_t>(g) - reinterpret_cast<uintptr_t>(w.row)) % 16 == 0;
+        fast = kind == kRowPlain && ref.plain() && (reinterpret_cast<uintptr_t>(g) - reinterpret_cast<uintptr_t>(w.row)) % 16 == 0;
         unl = kind == kRowPlain ? s.of_tail * scale / s.S : kind == kRowZero ? 0.f : NAN;
     }
     // any word
     __device__ __forceinline__ void operator()(uint4 x, int j0) const {
         constexpr int VEC = kRowVec<T>;
-        uint64_t e[VEC / 2];
-        float o[VEC];
-        word_weights<T>(x, ref, c, e);
-        unpair_word<T>(e, o);
+        float v[VEC];
+        unpack<T>(x, v);
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
-            if (j0 + i >= 0 && j0 + i < V) g[j0 + i] = Elem<T>::from_f(kind == kRowPlain ? o[i] * unl : unl);
+            if (j0 + i >= 0 && j0 + i < V)
+                g[j0 + i] = Elem<T>::from_f(kind == kRowPlain ? ref.weight(v[i], c) * unl : unl);
     }
     // a whole word of a fast row
     __device__ __forceinline__ void whole(uint4 x, uint4* to) const {
@@ -141,10 +170,16 @@ struct GradWriter {
 // the sum of the weights w of unlisted entries, and over listed entries the sum of
 // w and, with x = log2(e) z / T ln 2, forward of p (log p - x), reverse of
 // w (x - log p).
-struct DistillParts {
+struct DistillShared {
     double L[kDistillMaxParts], S_l[kDistillMaxParts];
     float S_u[kDistillMaxParts], m[kDistillMaxParts];
     int bad[kDistillMaxCluster];
+    double P[32];         // of this CTA's warps: the sum of the teacher's probabilities,
+    int valid[32];        // listed entries
+    double redd[33];
+    float redf[33];
+    RowState state;
+    int own_bad;
 };
 
 __device__ __forceinline__ void warp_sum_d(double& u, double& v) {
@@ -155,39 +190,151 @@ __device__ __forceinline__ void warp_sum_d(double& u, double& v) {
     }
 }
 
-// A row's state from its parts, and its loss: one warp.  P: the sum of the
-// teacher's probabilities.
-__device__ __forceinline__ double finish_row(RowState& s, const DistillParts& part, const DistillArgs& a, int valid,
-                                             double P, int parts) {
-    const int lane = threadIdx.x & 31;
+// The listed entries of a row that a thread looks after: tid, tid + NT, ...
+template <int NT>
+struct Listed {
+    static constexpr int MOST = DWA_MAX_TOP / NT;
+    int j[MOST], at[MOST];    // index (negative: unused), place in the chunk (-1 elsewhere)
+    float t[MOST], z[MOST], prob[MOST];
+
+    __device__ __forceinline__ void fetch(const DistillArgs& a, uint32_t r) {
+        const int64_t row = static_cast<int64_t>(r) * a.o.K;
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) {
+            const int k = threadIdx.x + i * NT;
+            j[i] = -1;
+            t[i] = -INFINITY;
+            if (k < a.o.K) {
+                j[i] = a.idx[row + k];
+                t[i] = load_elem(a.t, row + k, a.o.teacher_dtype);
+            }
+        }
+    }
+    // Notes the entries of the chunk in `bits`; the teacher's probabilities; t_hi and
+    // t_lo of the state.
+    template <class T>
+    __device__ __forceinline__ void place(DistillShared& sh, RowState& s, const DistillArgs& a, const RowWords<T>& w,
+                                          Chunk ch, uint32_t* bits, float t_lse) {
+        constexpr int VEC = kRowVec<T>;
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, V = w.V, n = ch.hi - ch.lo;
+        int mine = 0;
+        float t_top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) {
+            at[i] = -1;
+            if (j[i] >= V) {
+                sh.own_bad = 1;
+                j[i] = -1;
+            }
+            if (j[i] < 0) {
+                t[i] = -INFINITY;
+                continue;
+            }
+            ++mine;
+            const int b = j[i] + w.shift - ch.lo * VEC;
+            if (b >= 0 && b < n * VEC) {
+                at[i] = b;
+                if (atomicOr(&bits[b >> 5], 1u << (b & 31)) & (1u << (b & 31))) sh.own_bad = 1;
+            }
+            t_top = fmaxf(t_top, t[i]);
+        }
+        s.t_hi = 0.f;
+        s.t_lo = t_lse;
+        if (!a.t_lse) {
+            s.t_hi = block_reduce(t_top, MaxOp(), -INFINITY, sh.redf);
+            double sum = 0.;
+#pragma unroll
+            for (int i = 0; i < MOST; ++i)
+                if (t[i] > -INFINITY) sum += expf(static_cast<float>((static_cast<double>(t[i]) - s.t_hi) * a.inv_T));
+            s.t_lo = logf(static_cast<float>(block_reduce(sum, AddOp(), 0., sh.redd)));
+        }
+        double P = 0., unused = 0.;
+        if (warp * 32 < a.o.K) {
+#pragma unroll
+            for (int i = 0; i < MOST; ++i) {
+                prob[i] = t[i] == -INFINITY ? 0.f : expf(static_cast<float>(s.log_p(t[i], a.inv_T)));
+                P += prob[i];
+            }
+            warp_sum_d(P, unused);
+            mine = __reduce_add_sync(0xffffffffu, mine);
+        }
+        if (lane == 0) {
+            sh.P[warp] = P;
+            sh.valid[warp] = mine;
+        }
+    }
+    // this warp's part of the row
+    __device__ __forceinline__ void part(const MaxSum& ms, const RowState& s, const DistillArgs& a, Ref& ref, float& S_u,
+                                         double& S_l, double& L) const {
+        float top = ms.ref.m;
+#pragma unroll
+        for (int i = 0; i < MOST; ++i)
+            if (at[i] >= 0) top = fmaxf(top, z[i]);
+        ref = Ref(warp_max(top), a.c);
+        S_u = warp_sum(ms.at(ref, a.c));
+        S_l = L = 0.;
+        if (static_cast<int>(threadIdx.x & ~31u) >= a.o.K) return;
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) {
+            if (at[i] < 0) continue;
+            const double lp = s.log_p(t[i], a.inv_T), x = kLn2 * a.c * z[i];
+            const float e = z[i] == -INFINITY ? 0.f : ref.weight(z[i], a.c);   // the reference may be -inf too
+            S_l += e;
+            if (a.o.reverse) L += e != 0.f ? e * (x - lp) : 0.;
+            else L += prob[i] != 0.f ? prob[i] * (lp - x) : 0.;
+        }
+        warp_sum_d(S_l, L);
+    }
+    // the gradient of the chunk's entries
+    template <class T>
+    __device__ __forceinline__ void write(T* g, const RowState& s, const DistillArgs& a, float scale) const {
+#pragma unroll
+        for (int i = 0; i < MOST; ++i)
+            if (at[i] >= 0) g[j[i]] = Elem<T>::from_f(listed_grad(s, a, z[i], prob[i], s.log_p(t[i], a.inv_T)) * scale);
+    }
+};
+
+// A row's state from its parts, and its loss: one warp.
+__device__ __forceinline__ double finish_row(RowState& s, const DistillShared& sh, const DistillArgs& a, int warps) {
+    const int lane = threadIdx.x & 31, parts = a.P * warps;
     const bool one = lane < parts, two = lane + 32 < parts;
-    const float m0 = one ? part.m[lane] : -INFINITY, m1 = two ? part.m[lane + 32] : -INFINITY;
+    const float m0 = one ? sh.m[lane] : -INFINITY, m1 = two ? sh.m[lane + 32] : -INFINITY;
     s.m = warp_max(fmaxf(m0, m1));
-    const bool bad = __any_sync(0xffffffffu, lane < a.P && part.bad[lane]);
+    const bool bad = __any_sync(0xffffffffu, lane < a.P && sh.bad[lane]);
+    const int valid = __reduce_add_sync(0xffffffffu, lane < warps ? sh.valid[lane] : 0);
     const Ref ref(s.m, a.c);
     // a part without anything above -inf: its sums are 0 (NaN with a NaN)
     const float f0 = m0 > -INFINITY ? Ref(m0, a.c).rescale(ref, a.c) : 1.f;
     const float f1 = m1 > -INFINITY ? Ref(m1, a.c).rescale(ref, a.c) : 1.f;
-    const float S_u = warp_sum((one ? f0 * part.S_u[lane] : 0.f) + (two ? f1 * part.S_u[lane + 32] : 0.f));
-    double S_l = (one ? f0 * part.S_l[lane] : 0.) + (two ? f1 * part.S_l[lane + 32] : 0.);
+    const float S_u = warp_sum((one ? f0 * sh.S_u[lane] : 0.f) + (two ? f1 * sh.S_u[lane + 32] : 0.f));
+    double S_l = (one ? f0 * sh.S_l[lane] : 0.) + (two ? f1 * sh.S_l[lane + 32] : 0.);
     const double g0 = a.o.reverse ? f0 : 1.f, g1 = a.o.reverse ? f1 : 1.f;
-    double L = (one ? g0 * part.L[lane] : 0.) + (two ? g1 * part.L[lane + 32] : 0.);
-    warp_sum_d(S_l, L);
+    double L = (one ? g0 * sh.L[lane] : 0.) + (two ? g1 * sh.L[lane + 32] : 0.), P = lane < warps ? sh.P[lane] : 0.;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        S_l += __shfl_xor_sync(0xffffffffu, S_l, o);
+        L += __shfl_xor_sync(0xffffffffu, L, o);
+        P += __shfl_xor_sync(0xffffffffu, P, o);
+    }
     const double S = S_u + S_l;
     s.S = static_cast<float>(S);
-    log2_parts(s.S, s.log2_S_int, s.log2_S);
-    // log q = x - log_S
-    const double log_S = kLn2 * (ref.a(a.c) + s.log2_S_int + s.log2_S);
-    if (a.o.reverse) L = (L - (S_l != 0. ? S_l * log_S : 0.)) / S;
-    else L += P != 0. ? P * log_S : 0.;
+    log_parts(s.S, s.twos, s.rest);
+    const double log_S = s.log_S(ref, a.c);
+    const float inv = 1.f / s.S;
+    if (a.o.reverse) {
+        const double inv_S = inv * (2. - S * inv);   // one step: to 2^-46
+        L = (L - (S_l != 0. ? S_l * log_S : 0.)) * inv_S;
+    } else {
+        L += P != 0. ? P * log_S : 0.;
+    }
     s.of_tail = 1.f;
     if (a.t_lse && valid < a.d.V) {
-        const float p_t = fmaxf(static_cast<float>(1. - P), kTailFloor), q_t = S_u / s.S;
+        const float p_t = fmaxf(static_cast<float>(1. - P), kTailFloor), q_t = S_u * inv;
         if (q_t == 0.f) {
             if (!a.o.reverse && p_t > kTailNone) L = INFINITY;
             s.of_tail = 0.f;
         } else {
-            const double r_t = static_cast<double>(log_of_rest(q_t, static_cast<float>(S_l) / s.S)) -
+            const double r_t = static_cast<double>(log_of_rest(q_t, static_cast<float>(S_l) * inv)) -
                                log_of_rest(p_t, static_cast<float>(P));
             L += a.o.reverse ? q_t * r_t : -p_t * r_t;
             s.of_tail = a.o.reverse ? static_cast<float>(r_t - L) : 1.f - p_t / q_t;
@@ -199,26 +346,174 @@ __device__ __forceinline__ double finish_row(RowState& s, const DistillParts& pa
     return bad ? NAN : nothing ? 0. : L;
 }
 
-// A thread's words of a row on their way through shared memory, kRing stages of
-// two words ahead, each pass right behind the one before.  Only the thread that
-// copies a word reads it, so nothing but its own copies is waited for.
+// Warp 0: finishes the row, leaves its state in sh and, with `out`, writes its
+// loss and state.
+__device__ __forceinline__ void finish_and_tell(RowState& s, DistillShared& sh, const DistillArgs& a, uint32_t r,
+                                                float weight, int warps, bool out) {
+    double loss = finish_row(s, sh, a, warps);
+    if ((threadIdx.x & 31) != 0) return;
+    if (weight == 0.f) {   // a row left out, whatever it holds
+        loss = 0.;
+        s.kind = kRowZero;
+    }
+    sh.state = s;
+    if (out) {
+        if (s.kind == kRowBad) raise_status(a.status, DWA_STATUS_BAD_TOKEN);
+        a.loss[r] = static_cast<float>(loss * weight);
+        if (a.state) a.state[r] = s;
+    }
+}
+
+// Adds one word but for its entries in `listed`.
+template <class T>
+__device__ __forceinline__ void add_word(MaxSum& ms, uint4 x, uint32_t listed, float c) {
+    constexpr int VEC = kRowVec<T>;
+    const float top = word_max<T>(x);
+    if (!ms.covers(top)) ms.raise(top, c);
+    if (!ms.covers(top)) {   // NaN, nothing above -inf so far, or the ends of the type
+        ms.add_slow<T>(x, listed, c);
+        return;
+    }
+    uint64_t e[VEC / 2];
+    word_weights<T>(x, ms.ref, c, e);
+    if (listed != 0u) {
+        float f[VEC];
+        unpair_word<T>(e, f);
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2)
+            e[i / 2] = pair((listed >> i) & 1u ? 0.f : f[i], (listed >> i) & 2u ? 0.f : f[i + 1]);
+    }
+    ms.s2 = add2(ms.s2, sum_pairs<T>(e));
+}
+
+// The entries of word k that a bitmap holds.
+template <class T>
+__device__ __forceinline__ uint32_t listed_in(const uint32_t* bits, int k) {
+    const uint8_t* byte = reinterpret_cast<const uint8_t*>(bits);
+    return kRowVec<T> == 8 ? byte[k] : (byte[k >> 1] >> (4 * (k & 1))) & 15u;
+}
+
+// Few rows: a cluster of P CTAs holds a row in its shared memory.  The loss, the
+// state for a backward (a.state) and, with GRAD, the gradient of weight * L.
+template <class T, bool GRAD>
+__global__ void __launch_bounds__(kHoldThreads, 3) distill_hold_kernel(const __grid_constant__ DistillArgs a) {
+    namespace cg = cooperative_groups;
+    constexpr int NT = kHoldThreads, WARPS = NT / 32, VEC = kRowVec<T>;
+    extern __shared__ __align__(16) uint4 data[];
+    __shared__ DistillShared sh;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.d.V;
+    const uint32_t r = blockIdx.x >> a.log_P;
+    const int p = blockIdx.x & (a.P - 1);
+    uint32_t* bits = reinterpret_cast<uint32_t*>(data + a.room);
+    if (a.P > 1) cluster_arrive_relaxed();
+    if (tid == 0) sh.own_bad = 0;
+    pdl_enter();
+    // the teacher's loads first, then the chunk's copies, which they would wait behind
+    Listed<NT> l;
+    l.fetch(a, r);
+    const float weight = a.weights ? a.weights[r] : 1.f, t_lse = a.t_lse ? a.t_lse[r] : 0.f;
+    const RowWords<T> w(static_cast<const T*>(a.z) + row_offset(a.d, r), V);
+    const Chunk ch(w.words, p, a.log_P);
+    const int n = ch.hi - ch.lo;
+    // every thread copies the words that it will look at, in pieces
+    int from, to;
+    w.own_whole(ch.lo, ch.hi, tid, NT, from, to);
+    const int count = max(to - from, 0), w0 = tid + from * NT;   // words w0, w0 + NT, ... of the chunk
+    const int per_piece = (count + kHoldPieces - 1) / kHoldPieces;
+    uint4* const own_words = data + w0;
+    const uint4* const src = reinterpret_cast<const uint4*>(w.row + w.first(ch.lo + w0));
+#pragma unroll
+    for (int i = 0; i < kHoldPieces; ++i) {
+        const int end = min((i + 1) * per_piece, count);
+#pragma unroll 4
+        for (int k = i * per_piece; k < end; ++k) copy_async(own_words + k * NT, src + k * NT);
+        copy_commit();
+    }
+    for (int i = tid; i < (n * VEC + 127) / 128; i += NT) reinterpret_cast<uint4*>(bits)[i] = make_uint4(0u, 0u, 0u, 0u);
+    __syncthreads();
+    RowState s = {};
+    l.place(sh, s, a, w, ch, bits, t_lse);
+    __syncthreads();
+    // one pass: the sum of the weights of unlisted entries
+    MaxSum ms;
+    w.edges(ch.lo, ch.hi, tid, [&](uint4 x, int j0) {
+        const int k = (j0 + w.shift) / VEC - ch.lo;
+        data[k] = x;
+        ms.add_slow<T>(x, listed_in<T>(bits, k), a.c);
+    });
+    const auto add_piece = [&](int i) {
+        const int end = min((i + 1) * per_piece, count);
+#pragma unroll 2
+        for (int k = i * per_piece; k < end; ++k) add_word<T>(ms, own_words[k * NT], listed_in<T>(bits, w0 + k * NT), a.c);
+    };
+    static_assert(kHoldPieces == 2, "one wait a piece");
+    copy_wait<1>();
+    add_piece(0);
+    copy_wait<0>();
+    add_piece(1);
+    __syncthreads();   // the listed entries may be other threads' words
+#pragma unroll
+    for (int i = 0; i < l.MOST; ++i)
+        l.z[i] = l.at[i] >= 0 ? Elem<T>::to_f(reinterpret_cast<const T*>(data)[l.at[i]]) : -INFINITY;
+    Ref ref;
+    float S_u;
+    double S_l, L;
+    l.part(ms, s, a, ref, S_u, S_l, L);
+    if (a.P > 1) cluster_wait();   // every CTA of the cluster has started
+    if (lane < a.P) {              // lane q: to CTA q
+        DistillShared& to_q = *cg::this_cluster().map_shared_rank(&sh, lane);
+        const int i = p * WARPS + warp;
+        to_q.m[i] = ref.m;
+        to_q.S_u[i] = S_u;
+        to_q.S_l[i] = S_l;
+        to_q.L[i] = L;
+        if (warp == 0) to_q.bad[p] = sh.own_bad;
+    }
+    if (a.P > 1) cg::this_cluster().sync();
+    else __syncthreads();
+    if (!GRAD && p != 0) return;
+    if (warp == 0) finish_and_tell(s, sh, a, r, weight, WARPS, p == 0);
+    if constexpr (GRAD) {
+        __syncthreads();
+        s = sh.state;
+        T* g = static_cast<T*>(a.g) + static_cast<int64_t>(r) * V;
+        const float scale = weight * static_cast<float>(a.inv_T);
+        const GradWriter<T> write(w, g, s, a, scale);
+        if (write.fast) {
+            uint4* const to_g = reinterpret_cast<uint4*>(g + w.first(ch.lo + w0));
+#pragma unroll 4
+            for (int k = 0; k < count; ++k) write.whole(own_words[k * NT], to_g + k * NT);
+            w.edges(ch.lo, ch.hi, tid, write);
+        } else {
+            for (int k = tid; k < n; k += NT) write(data[k], w.first(ch.lo + k));
+        }
+        if (s.kind != kRowPlain) return;
+        __syncthreads();
+        l.write(g, s, a, scale);
+    }
+}
+
+// A thread's `count` words of a row, NT apart, on their way through a ring of its
+// own in shared memory, kRing stages of two words ahead, each pass right behind the
+// one before.  Only the thread that copies a word reads it, so nothing but its own
+// copies is waited for.
 template <int NT>
 struct WordRing {
-    uint4* const slots;        // this thread's: 2 kRing of them, NT words apart
-    const uint4* const src;    // its words, NT apart
-    const int from, to;
-    int left, next, put = 0, get = 0;
+    uint4* const slots;        // 2 kRing of them, NT apart
+    const uint4* const src;
+    const int count;
+    int left, next = 0, put = 0, get = 0;
 
-    __device__ __forceinline__ WordRing(uint4* slots_, const uint4* src_, int from_, int to_, int passes)
-        : slots(slots_), src(src_), from(from_), to(to_), left(passes), next(from_) {}
+    __device__ __forceinline__ WordRing(uint4* slots_, const uint4* src_, int count_, int passes)
+        : slots(slots_), src(src_), count(count_), left(passes) {}
     __device__ __forceinline__ void issue() {
-        if (next >= to && left > 0) {
+        if (next >= count && left > 0) {
             --left;
-            next = from;
+            next = 0;
         }
-        if (left > 0 && next < to) {
+        if (left > 0 && next < count) {
             copy_async(slots + put * 2 * NT, src + next * NT);
-            if (next + 1 < to) copy_async(slots + (put * 2 + 1) * NT, src + (next + 1) * NT);
+            if (next + 1 < count) copy_async(slots + (put * 2 + 1) * NT, src + (next + 1) * NT);
             next += 2;
         }
         put = put + 1 == kRing ? 0 : put + 1;
@@ -226,253 +521,77 @@ struct WordRing {
     }
     template <class F>
     __device__ __forceinline__ void pass(F f) {   // f(word, its number) for all of them
-        for (int k = from; k < to; k += 2) {
+        for (int k = 0; k < count; k += 2) {
             copy_wait<kRing - 1>();
             const uint4* x = slots + get * 2 * NT;
             f(x[0], k);
-            if (k + 1 < to) f(x[NT], k + 1);
+            if (k + 1 < count) f(x[NT], k + 1);
             get = get + 1 == kRing ? 0 : get + 1;
             issue();
         }
     }
 };
 
-// The loss of a row, the state for a backward (a.state) and, with GRAD, the
-// gradient of weight * L.  HOLD: a cluster of P CTAs holds the row in shared
-// memory; else one CTA reads it, and for the gradient once more out of L2.
-template <class T, bool GRAD, bool HOLD>
-__global__ void __launch_bounds__(HOLD ? kDistillThreads : kStreamThreads, HOLD ? 3 : 2)
-    distill_fwd_kernel(const __grid_constant__ DistillArgs a) {
-    namespace cg = cooperative_groups;
-    constexpr int NT = HOLD ? kDistillThreads : kStreamThreads, WARPS = NT / 32;
-    constexpr int VEC = kRowVec<T>, MOST = DWA_MAX_TOP / NT;
+// Many rows: one CTA per row that, with GRAD, reads it a second time, out of L2.
+template <class T, bool GRAD, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) distill_stream_kernel(const __grid_constant__ DistillArgs a) {
+    constexpr int WARPS = NT / 32, VEC = kRowVec<T>;
     extern __shared__ __align__(16) uint4 data[];
-    __shared__ DistillParts part;
-    __shared__ double redd[33];
-    __shared__ float redf[33];
-    __shared__ RowState row_state;
-    __shared__ int bad, valid;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.o.K, V = a.d.V;
-    const uint32_t r = blockIdx.x >> a.log_P;
-    const int p = blockIdx.x & (a.P - 1);
-    uint32_t* bits = reinterpret_cast<uint32_t*>(data + (HOLD ? a.room : 2 * kRing * NT));
-    if (a.P > 1) cluster_arrive_relaxed();
-    if (tid == 0) bad = valid = 0;
+    __shared__ DistillShared sh;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.d.V;
+    const uint32_t r = blockIdx.x;
+    uint32_t* bits = reinterpret_cast<uint32_t*>(data + 2 * kRing * NT);
+    if (tid == 0) sh.own_bad = 0;
     pdl_enter();
-    // the teacher's loads first, then the chunk's copies, which they would wait behind
-    const int64_t rK = static_cast<int64_t>(r) * K;
-    int j[MOST];
-    float t[MOST];
-#pragma unroll
-    for (int i = 0; i < MOST; ++i) {
-        const int k = tid + i * NT;
-        j[i] = -1;
-        t[i] = -INFINITY;
-        if (k < K) {
-            j[i] = a.idx[rK + k];
-            t[i] = load_elem(a.t, rK + k, a.o.teacher_dtype);
-        }
-    }
+    Listed<NT> l;
+    l.fetch(a, r);
     const float weight = a.weights ? a.weights[r] : 1.f, t_lse = a.t_lse ? a.t_lse[r] : 0.f;
     const RowWords<T> w(static_cast<const T*>(a.z) + row_offset(a.d, r), V);
-    const Chunk ch(w.words, p, a.log_P);
-    const int n = ch.hi - ch.lo;
-    T* g = GRAD ? static_cast<T*>(a.g) + static_cast<int64_t>(r) * V : nullptr;
-    // the chunk, in pieces: every thread copies the words that it will look at
     int from, to;
-    w.own_whole(ch.lo, ch.hi, tid, NT, from, to);
-    uint4* const own_words = data + tid;
-    float z[MOST];   // the listed entries' logits
-    const auto piece = [&](int i) { return from + (to - from) * i / kDistillPieces; };
-    const uint4* const src = reinterpret_cast<const uint4*>(w.row + w.first(ch.lo + tid));
-    WordRing<NT> ring(own_words, src, from, to, GRAD ? 2 : 1);
-    if constexpr (HOLD) {
-#pragma unroll
-        for (int i = 0; i < kDistillPieces; ++i) {
-            const int end = piece(i + 1);
-#pragma unroll 4
-            for (int k = piece(i); k < end; ++k) copy_async(own_words + k * NT, src + k * NT);
-            copy_commit();
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < kRing; ++i) ring.issue();
-#pragma unroll
-        for (int i = 0; i < MOST; ++i) z[i] = j[i] >= 0 && j[i] < V ? Elem<T>::to_f(w.row[j[i]]) : -INFINITY;
-    }
-    for (int i = tid; i < (n * VEC + 127) / 128; i += NT)
-        reinterpret_cast<uint4*>(bits)[i] = make_uint4(0u, 0u, 0u, 0u);
+    w.own_whole(0, w.words, tid, NT, from, to);
+    const int count = max(to - from, 0), w0 = tid + from * NT;   // words w0, w0 + NT, ... of the row
+    WordRing<NT> ring(data + tid, reinterpret_cast<const uint4*>(w.row + w.first(w0)), count, GRAD ? 2 : 1);
+#pragma unroll 1
+    for (int i = 0; i < kRing; ++i) ring.issue();
+    for (int i = tid; i < (w.words * VEC + 127) / 128; i += NT) reinterpret_cast<uint4*>(bits)[i] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
     RowState s = {};
-    if (weight == 0.f) {   // a row left out, whatever it holds
-        s.kind = kRowZero;
-        if (p == 0 && tid == 0) {
-            a.loss[r] = 0.f;
-            if (a.state) a.state[r] = s;
-        }
-        copy_wait<0>();
-        if constexpr (GRAD) {
-            const GradWriter<T> write(w, g, s, a, 0.f);
-            for (int i = ch.lo + tid; i < ch.hi; i += NT) write(make_uint4(0u, 0u, 0u, 0u), w.first(i));
-        }
-        if (a.P > 1) cluster_wait();
-        return;
-    }
-    // the teacher: every CTA all of it, the places of the entries in its chunk
-    int mine = 0, at[MOST];
-    float t_top = -INFINITY, prob[MOST];
+    l.place(sh, s, a, w, Chunk(w.words, 0, 0), bits, t_lse);
 #pragma unroll
-    for (int i = 0; i < MOST; ++i) {
-        at[i] = -1;
-        if (j[i] >= V) bad = 1;
-        if (j[i] < 0 || j[i] >= V) {
-            t[i] = -INFINITY;
-            continue;
-        }
-        ++mine;
-        const int b = j[i] + w.shift - ch.lo * VEC;
-        if (b >= 0 && b < n * VEC) {
-            at[i] = b;
-            if (atomicOr(&bits[b >> 5], 1u << (b & 31)) & (1u << (b & 31))) bad = 1;
-        }
-        t_top = fmaxf(t_top, t[i]);
-    }
-    if (mine) atomicAdd(&valid, mine);
-    if (a.t_lse) {
-        s.t_lo = t_lse;
-    } else {
-        s.t_hi = block_reduce(t_top, MaxOp(), -INFINITY, redf);
-        double sum = 0.;
-#pragma unroll
-        for (int i = 0; i < MOST; ++i)
-            if (t[i] > -INFINITY) sum += expf(static_cast<float>((static_cast<double>(t[i]) - s.t_hi) * a.inv_T));
-        s.t_lo = logf(static_cast<float>(block_reduce(sum, AddOp(), 0., redd)));
-    }
-    const auto log_p = [&](float x) { return (static_cast<double>(x) - s.t_hi) * a.inv_T - s.t_lo; };
-    double P = 0.;
-#pragma unroll
-    for (int i = 0; i < MOST; ++i) {
-        prob[i] = t[i] == -INFINITY ? 0.f : expf(static_cast<float>(log_p(t[i])));
-        if (tid + i * NT < K) P += prob[i];
-    }
-    P = block_reduce(P, AddOp(), 0., redd);   // its barriers also order the bitmap
-    // one pass: the sum of the weights of unlisted entries
+    for (int i = 0; i < l.MOST; ++i) l.z[i] = l.j[i] >= 0 ? Elem<T>::to_f(w.row[l.j[i]]) : -INFINITY;
+    __syncthreads();
     MaxSum ms;
-    const uint8_t* byte = reinterpret_cast<const uint8_t*>(bits);
-    const auto add_word = [&](uint4 x, int k) {
-        const float top = word_max<T>(x);
-        const uint32_t listed = VEC == 8 ? byte[k] : (byte[k >> 1] >> (4 * (k & 1))) & 15u;
-        if (!ms.covers(top)) {
-            ms.raise(top, a.c);
-            if (top != top) ms.poison();
-            if (ms.ref.m == -INFINITY) return;
-        }
-        uint64_t e[VEC / 2];
-        word_weights<T>(x, ms.ref, a.c, e);
-        if (listed != 0u) {
-            float f[VEC];
-            unpair_word<T>(e, f);
-#pragma unroll
-            for (int v = 0; v < VEC; v += 2)
-                e[v / 2] = pair((listed >> v) & 1u ? 0.f : f[v], (listed >> v) & 2u ? 0.f : f[v + 1]);
-        }
-        ms.s2 = add2(ms.s2, sum_pairs<T>(e));
-    };
-    w.edges(ch.lo, ch.hi, tid, [&](uint4 x, int j0) {
-        const int k = (j0 + w.shift) / VEC - ch.lo;
-        if constexpr (HOLD) data[k] = x;
-        add_word(x, k);
-    });
-    if constexpr (HOLD) {
-        const auto add = [&](int i) {
-            const int end = piece(i + 1);
-#pragma unroll 2
-            for (int k = piece(i); k < end; ++k) add_word(own_words[k * NT], tid + k * NT);
-        };
-        static_assert(kDistillPieces == 4, "one wait a piece");
-        copy_wait<3>();
-        add(0);
-        copy_wait<2>();
-        add(1);
-        copy_wait<1>();
-        add(2);
-        copy_wait<0>();
-        add(3);
-        __syncthreads();   // the listed entries may be other threads' words
-#pragma unroll
-        for (int i = 0; i < MOST; ++i)
-            z[i] = at[i] >= 0 ? Elem<T>::to_f(reinterpret_cast<const T*>(data)[at[i]]) : -INFINITY;
-    } else {
-        ring.pass([&](uint4 x, int k) { add_word(x, tid + k * NT); });
+    w.edges(0, w.words, tid, [&](uint4 x, int j0) { ms.add_slow<T>(x, listed_in<T>(bits, (j0 + w.shift) / VEC), a.c); });
+    ring.pass([&](uint4 x, int k) { add_word<T>(ms, x, listed_in<T>(bits, w0 + k * NT), a.c); });
+    Ref ref;
+    float S_u;
+    double S_l, L;
+    l.part(ms, s, a, ref, S_u, S_l, L);
+    if (lane == 0) {
+        sh.m[warp] = ref.m;
+        sh.S_u[warp] = S_u;
+        sh.S_l[warp] = S_l;
+        sh.L[warp] = L;
+        if (warp == 0) sh.bad[0] = sh.own_bad;
     }
-    // the warp's part: what it summed, and its listed entries of this chunk
-    float top = ms.ref.m;
-#pragma unroll
-    for (int i = 0; i < MOST; ++i) top = fmaxf(top, z[i]);
-    const Ref ref(warp_max(top), a.c);
-    const float S_u = warp_sum(ms.at(ref, a.c));
-    double S_l = 0., L = 0.;
-    if (warp * 32 < K) {
-#pragma unroll
-        for (int i = 0; i < MOST; ++i) {
-            if (at[i] < 0) continue;
-            const double lp = log_p(t[i]), x = kLn2 * a.c * z[i];
-            const float e = z[i] == -INFINITY ? 0.f : ref.weight(z[i], a.c);   // the reference may be -inf too
-            S_l += e;
-            if (a.o.reverse) L += e != 0.f ? e * (x - lp) : 0.;
-            else L += prob[i] != 0.f ? prob[i] * (lp - x) : 0.;
-        }
-        warp_sum_d(S_l, L);
-    }
-    if (a.P > 1) cluster_wait();   // every CTA of the cluster has started
-    if (lane < a.P) {              // lane q: to CTA q
-        DistillParts& to_q = *cg::this_cluster().map_shared_rank(&part, lane);
-        const int i = p * WARPS + warp;
-        to_q.m[i] = ref.m;
-        to_q.S_u[i] = S_u;
-        to_q.S_l[i] = S_l;
-        to_q.L[i] = L;
-        if (warp == 0) to_q.bad[p] = bad;
-    }
-    if (a.P > 1) cg::this_cluster().sync();
-    else __syncthreads();
-    if (!GRAD && p != 0) return;
-    if (warp == 0) {
-        const double loss = finish_row(s, part, a, valid, P, a.P * WARPS);
-        if (lane == 0) row_state = s;
-        if (p == 0 && lane == 0) {
-            if (s.kind == kRowBad) raise_status(a.status, DWA_STATUS_BAD_TOKEN);
-            a.loss[r] = static_cast<float>(loss * weight);
-            if (a.state) a.state[r] = s;
-        }
-    }
+    __syncthreads();
+    if (warp == 0) finish_and_tell(s, sh, a, r, weight, WARPS, true);
     if constexpr (GRAD) {
         __syncthreads();
-        s = row_state;
+        s = sh.state;
+        T* g = static_cast<T*>(a.g) + static_cast<int64_t>(r) * V;
         const float scale = weight * static_cast<float>(a.inv_T);
         const GradWriter<T> write(w, g, s, a, scale);
         if (write.fast) {
-            uint4* const to_g = reinterpret_cast<uint4*>(g + w.first(ch.lo + tid));
-            if constexpr (HOLD) {
-#pragma unroll 4
-                for (int k = from; k < to; ++k) write.whole(own_words[k * NT], to_g + k * NT);
-            } else {
-                ring.pass([&](uint4 x, int k) { write.whole(x, to_g + k * NT); });
-            }
-            w.edges(ch.lo, ch.hi, tid, write);
+            uint4* const to_g = reinterpret_cast<uint4*>(g + w.first(w0));
+            ring.pass([&](uint4 x, int k) { write.whole(x, to_g + k * NT); });
         } else {
-            if constexpr (HOLD) {
-                for (int k = tid; k < n; k += NT) write(data[k], w.first(ch.lo + k));
-            } else {
-                ring.pass([&](uint4 x, int k) { write(x, w.first(tid + k * NT)); });
-                w.edges(ch.lo, ch.hi, tid, write);
-            }
+            ring.pass([&](uint4 x, int k) { write(x, w.first(w0 + k * NT)); });
         }
+        w.edges(0, w.words, tid, write);
         if (s.kind != kRowPlain) return;
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < MOST; ++i)
-            if (at[i] >= 0) g[j[i]] = Elem<T>::from_f(listed_grad(s, a, z[i], t[i]) * scale);
+        l.write(g, s, a, scale);
     }
 }
 
@@ -510,8 +629,12 @@ __global__ void __launch_bounds__(kDistillThreads) distill_bwd_kernel(const __gr
     if (!plain) return;
     __syncthreads();
     for (int k = tid; k < K; k += kDistillThreads)
-        if (here(idx[k]))
-            g[idx[k]] = Elem<T>::from_f(listed_grad(s, a, zk[k], load_elem(a.t, static_cast<int64_t>(r) * K + k, a.o.teacher_dtype)) * scale);
+        if (here(idx[k])) {
+            const float t = load_elem(a.t, static_cast<int64_t>(r) * K + k, a.o.teacher_dtype);
+            const double lp = s.log_p(t, a.inv_T);
+            const float prob = t == -INFINITY ? 0.f : expf(static_cast<float>(lp));
+            g[idx[k]] = Elem<T>::from_f(listed_grad(s, a, zk[k], prob, lp) * scale);
+        }
 }
 
 int check_logits(const DwaLogitsDims* d, const char* what) {
@@ -552,10 +675,15 @@ static int check_workspace(const void* ws, size_t bytes) {
 
 static bool misaligned(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % dtype_bytes(dtype) != 0; }
 
-template <class K>
-static int allow_smem(K kernel, size_t bytes) {
-    if (bytes > 48 * 1024)
-        DWA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+// Lets a kernel have `bytes` of dynamic shared memory, once per device and size.
+template <auto KERNEL>
+static int allow_smem(size_t bytes) {
+    static std::atomic<size_t> allowed[64];
+    int dev = 0;
+    DWA_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 64 && allowed[dev].load(std::memory_order_relaxed) >= bytes) return DWA_OK;
+    DWA_CUDA_TRY(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+    if (dev < 64) allowed[dev].store(bytes, std::memory_order_relaxed);
     return DWA_OK;
 }
 
@@ -571,26 +699,45 @@ static int log_ctas_per_row(const DwaLogitsDims& d) {
     return l;
 }
 
-template <class T, bool GRAD, bool HOLD>
-static int launch_fwd_as(cudaStream_t st, DistillArgs a) {
-    constexpr int VEC = kRowVec<T>, NT = HOLD ? kDistillThreads : kStreamThreads;
-    a.log_P = HOLD ? log_ctas_per_row(a.d) : 0;
+template <class T, bool GRAD>
+static int launch_hold(cudaStream_t st, DistillArgs a) {
+    constexpr int VEC = kRowVec<T>, NT = kHoldThreads;
+    a.log_P = log_ctas_per_row(a.d);
     a.P = 1 << a.log_P;
     a.room = (a.d.V + 2 * VEC - 2) / VEC / a.P + 1;
-    const size_t sh = static_cast<size_t>(HOLD ? a.room : 2 * kRing * NT) * 16 + (static_cast<size_t>(a.room) * VEC + 127) / 128 * 16;
-    if (int rc = allow_smem(distill_fwd_kernel<T, GRAD, HOLD>, sh)) return rc;
+    const size_t sh = static_cast<size_t>(a.room) * 16 + (static_cast<size_t>(a.room) * VEC + 127) / 128 * 16;
+    if (int rc = allow_smem<distill_hold_kernel<T, GRAD>>(sh)) return rc;
     DWA_TIMED("distill_fwd", st,
-              (launch_pdl_cluster(distill_fwd_kernel<T, GRAD, HOLD>, dim3(static_cast<unsigned>(a.d.rows * a.P)), dim3(NT),
-                                  sh, st, dim3(a.P), a)));
-    DWA_LAUNCH_CHECK("distill_fwd_kernel");
+              (launch_pdl_cluster(distill_hold_kernel<T, GRAD>, dim3(static_cast<unsigned>(a.d.rows * a.P)), dim3(NT), sh, st,
+                                  dim3(a.P), a)));
+    DWA_LAUNCH_CHECK("distill_hold_kernel");
+    ++g_launches_total;
+    return DWA_OK;
+}
+
+template <class T, bool GRAD, int NT>
+static int launch_stream(cudaStream_t st, DistillArgs a) {
+    constexpr int VEC = kRowVec<T>;
+    a.room = (a.d.V + 2 * VEC - 2) / VEC;
+    const size_t sh = static_cast<size_t>(2 * kRing * NT) * 16 + (static_cast<size_t>(a.room) * VEC + 127) / 128 * 16;
+    if (int rc = allow_smem<distill_stream_kernel<T, GRAD, NT>>(sh)) return rc;
+    DWA_TIMED("distill_fwd", st,
+              (launch_pdl(distill_stream_kernel<T, GRAD, NT>, dim3(static_cast<unsigned>(a.d.rows)), dim3(NT), sh, st, a)));
+    DWA_LAUNCH_CHECK("distill_stream_kernel");
     ++g_launches_total;
     return DWA_OK;
 }
 
 template <class T, bool GRAD>
 static int launch_fwd(cudaStream_t st, const DistillArgs& a) {
-    if (a.d.rows >= 2 * tc::sm_count()) return launch_fwd_as<T, GRAD, false>(st, a);
-    return launch_fwd_as<T, GRAD, true>(st, a);
+    // fewer rows than two a SM: 64 x 131072 takes 17.6 us held by clusters, 36 us streamed
+    if (a.d.rows < 2 * tc::sm_count()) return launch_hold<T, GRAD>(st, a);
+    // four CTAs of 256 threads an SM hide a row's serial steps better (8192 x 32768
+    // with the gradient: 240 us, 327 us with two of 512) as long as their rows stay
+    // in L2 between the passes (4096 x 131072: 492 and 456 us)
+    if constexpr (GRAD)
+        if (static_cast<int64_t>(a.d.V) * sizeof(T) > 128 * 1024) return launch_stream<T, GRAD, 512>(st, a);
+    return launch_stream<T, GRAD, 256>(st, a);
 }
 
 }  // namespace dwa

@@ -181,12 +181,8 @@ __device__ __forceinline__ void scan_chunk(const RowWords<T>& w, Chunk ch, float
         if (u < 0) edge = m;
         else top[u] = max_nan(top[u], m);
         if constexpr (SUM) {
-            if (!ms.covers(m)) ms.raise(m, c);
-            if (ms.ref.m > -INFINITY) {
-                uint64_t e[kRowVec<T> / 2];
-                word_weights<T>(x, ms.ref, c, e);
-                ms.s2 = add2(ms.s2, sum_pairs<T>(e));
-            }
+            if (ms.covers(m)) ms.add_words<T, 1>(&x, c);
+            else ms.add_slow<T>(x, 0u, c);
         }
     });
 }
@@ -781,20 +777,24 @@ __device__ __forceinline__ void race_chunk(const RowWords<T>& w, Chunk ch, float
     w.template each<2>(ch.lo, ch.hi, threadIdx.x, kSelThreads, [&](uint4 x, int j0, int) {
         const float m = word_max<T>(x);
         top = max_nan(top, m);
-        if (!ms.covers(m)) {
+        float e[VEC], score[VEC];
+        if (ms.covers(m)) {
+            uint64_t e2[VEC / 2];
+            word_weights<T>(x, ms.ref, c, e2);
+            ms.s2 = add2(ms.s2, sum_pairs<T>(e2));
+            unpair_word<T>(e2, e);
+        } else {
             const Ref old = ms.ref;
-            ms.raise(m, c);
+            ms.add_slow<T>(x, 0u, c);
             if (old.m > -INFINITY && ms.ref.m > old.m) {
                 const float f = old.rescale(ms.ref, c);
                 best = f > 0.f ? best * f : 0.f;
             }
             if (ms.ref.m == -INFINITY) return;
+            unpack<T>(x, e);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) e[i] = ms.ref.weight(e[i], c);
         }
-        float e[VEC], score[VEC];
-        uint64_t e2[VEC / 2];
-        word_weights<T>(x, ms.ref, c, e2);
-        ms.s2 = add2(ms.s2, sum_pairs<T>(e2));
-        unpair_word<T>(e2, e);
         float lead = -1.f;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {

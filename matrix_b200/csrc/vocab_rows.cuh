@@ -71,19 +71,28 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// The largest value of a word, NaN if one is there.
-template <class T>
-__device__ __forceinline__ float word_max(uint4 w) {
+// The largest value of N words, NaN if one is there.
+template <class T, int N = 1>
+__device__ __forceinline__ float words_max(const uint4* w) {
     if constexpr (sizeof(T) == 2) {
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
-        const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);
+        __nv_bfloat162 m = h[0];
+#pragma unroll
+        for (int i = 1; i < 4 * N; ++i) m = __hmax2_nan(m, h[i]);
         return max_nan(__low2float(m), __high2float(m));
     } else {
-        float v[4];
-        unpack<T>(w, v);
-        return max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3]));
+        float m = __uint_as_float(w[0].x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float v[4];
+            unpack<T>(w[i], v);
+            m = max_nan(m, max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3])));
+        }
+        return m;
     }
 }
+template <class T>
+__device__ __forceinline__ float word_max(uint4 w) { return words_max<T>(&w); }
 
 // Weights of one row or part of it, relative to a reference m (its largest value
 // so far): w(v) = exp2(v c - a) with a = m c rounded to fp32, one multiply-add and
@@ -132,26 +141,16 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     return r;
 }
 
-// The weights of one word, in pairs.
+// The weights of one word, in pairs, relative to a plain reference.
 template <class T>
 __device__ __forceinline__ void word_weights(uint4 w, const Ref& ref, float c, uint64_t* e) {
     float v[kRowVec<T>];
     unpack<T>(w, v);
-    uint64_t x[kRowVec<T> / 2];
-    const uint64_t cc = pair(c, c);
-    if (ref.plain()) {
-        const uint64_t na = pair(ref.neg_a, ref.neg_a);
-#pragma unroll
-        for (int i = 0; i < kRowVec<T> / 2; ++i) x[i] = fma2(pair(v[2 * i], v[2 * i + 1]), cc, na);
-    } else {
-        const uint64_t nm = pair(-ref.m, -ref.m);
-#pragma unroll
-        for (int i = 0; i < kRowVec<T> / 2; ++i) x[i] = mul2(add2(pair(v[2 * i], v[2 * i + 1]), nm), cc);
-    }
+    const uint64_t cc = pair(c, c), na = pair(ref.neg_a, ref.neg_a);
 #pragma unroll
     for (int i = 0; i < kRowVec<T> / 2; ++i) {
         float p, q;
-        unpair(x[i], p, q);
+        unpair(fma2(pair(v[2 * i], v[2 * i + 1]), cc, na), p, q);
         e[i] = pair(exp2_fast(p), exp2_fast(q));
     }
 }
@@ -178,6 +177,11 @@ struct RowWords {
         words = (V + shift + VEC - 1) / VEC;
         full_lo = shift > 0 ? 1 : 0;
         full_hi = (V + shift) / VEC;
+    }
+    // a word that adds nothing: -inf throughout
+    static __device__ __forceinline__ uint4 nothing() {
+        const uint32_t u = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+        return make_uint4(u, u, u, u);
     }
     __device__ __forceinline__ int first(int g) const { return g * kRowVec<T> - shift; }
     __device__ __forceinline__ bool whole(int g) const { return g >= full_lo && g < full_hi; }
@@ -280,21 +284,44 @@ struct AddOp {
 // would pass 2^20, so that hardly any word but the first does.
 struct MaxSum {
     Ref ref;
-    float limit = -INFINITY;   // what the reference stands for at most
+    float limit = -INFINITY;   // what a plain reference stands for at most
     uint64_t s2 = 0;           // two sums
-    __device__ __forceinline__ bool covers(float top) const { return top <= limit; }   // false for NaN
+    // whether words up to `top` may be added by add_words: false for NaN, before
+    // the first value above -inf, and at the ends of the type
+    __device__ __forceinline__ bool covers(float top) const { return top <= limit; }
+    template <class T, int N>
+    __device__ __forceinline__ void add_words(const uint4* x, float c) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            uint64_t e[kRowVec<T> / 2];
+            word_weights<T>(x[i], ref, c, e);
+            s2 = add2(s2, sum_pairs<T>(e));
+        }
+    }
     __device__ __forceinline__ void raise(float to, float c) {
-        if (to > limit) {
+        if (to > limit && to > ref.m) {
             const Ref r(to, c);
             if (ref.m > -INFINITY) {
                 const float f = ref.rescale(r, c);
                 s2 = mul2(s2, pair(f, f));
             }
             ref = r;
-            limit = to + 20.f / c;
+            limit = r.plain() ? to + 20.f / c : -INFINITY;
         }
     }
-    __device__ __forceinline__ void poison() { s2 = pair(NAN, NAN); }
+    // any word; entry i is left out where bit i of `skip` is set
+    template <class T>
+    __device__ __forceinline__ void add_slow(uint4 x, uint32_t skip, float c) {
+        const float top = word_max<T>(x);
+        raise(top, c);
+        if (top != top) s2 = pair(NAN, NAN);
+        if (ref.m == -INFINITY) return;
+        float v[kRowVec<T>], sum = 0.f;
+        unpack<T>(x, v);
+#pragma unroll
+        for (int i = 0; i < kRowVec<T>; ++i) sum += (skip >> i) & 1u ? 0.f : ref.weight(v[i], c);
+        s2 = add2(s2, pair(sum, 0.f));
+    }
     // the sum relative to `all`
     __device__ __forceinline__ float at(const Ref& all, float c) const {
         float a, b;
