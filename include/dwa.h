@@ -620,8 +620,8 @@ DWA_API int dwa_top_logits(void* stream, const DwaLogitsDims* dims, const void* 
  *   state [rows, DWA_DISTILL_STATE_FLOATS] f32 or NULL: what dwa_distill_bwd needs
  *   g_logits [rows, V] in the logits' dtype or NULL: the gradient of sum loss;
  *     may be the memory of contiguous logits
- * dwa_distill_bwd writes the gradient of sum g_loss[r] * loss[r] from the same
- * inputs and the state.  An index >= V, or one listed twice in a row, sets
+ * dwa_distill_bwd writes the gradient of sum g_loss[r * g_loss_stride] * loss[r]
+ * (stride 0: one value for all rows) from the same inputs and the state.  An index >= V, or one listed twice in a row, sets
  * DWA_STATUS_BAD_TOKEN in the workspace's status word and makes the row's loss
  * and gradient NaN. */
 #define DWA_DISTILL_STATE_FLOATS 9
@@ -641,7 +641,7 @@ DWA_API int dwa_distill_fwd(void* stream, const DwaLogitsDims* dims, const DwaDi
 DWA_API int dwa_distill_bwd(void* stream, const DwaLogitsDims* dims, const DwaDistillDims* opts,
                             const void* logits, const void* teacher_logits, const int32_t* teacher_indices,
                             const float* teacher_lse, const float* weights, const float* state,
-                            const float* g_loss, void* g_logits);
+                            const float* g_loss, int g_loss_stride, void* g_logits);
 
 /* One token per row.  noise: row r's V numbers at r * noise_stride, drawn from
  * the exponential distribution (positive).  With w_i = exp((z_i - max z) / T):

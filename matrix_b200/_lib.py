@@ -166,7 +166,7 @@ _SIGNATURES = {
     "dwa_distill_fwd": (C.c_int, [_P, C.POINTER(LogitsDims), C.POINTER(DistillDims), _P, _P, _P, _P, _P, _P, _P, _P,
                                   _P, C.c_size_t]),
     "dwa_distill_bwd": (C.c_int, [_P, C.POINTER(LogitsDims), C.POINTER(DistillDims), _P, _P, _P, _P, _P, _P, _P,
-                                  _P]),
+                                  C.c_int, _P]),
     "dwa_sample_tokens": (C.c_int, [_P, C.POINTER(LogitsDims), C.POINTER(SampleParams), _P, _P, C.c_int64, _P, _P]),
     "dwa_retrieve_merge": (C.c_int, [_P, C.POINTER(RetrieveDims), C.c_int, _P, C.c_int, _P, _P, _P,
                                      _P, _P, _P, C.c_size_t]),

@@ -79,6 +79,7 @@ struct DistillArgs {
     float* loss;
     RowState* state;
     const float* g_loss;
+    int g_loss_stride;
     void* g;
     uint32_t* status;
     float c;       // log2(e) / T
@@ -615,7 +616,7 @@ __global__ void __launch_bounds__(kDistillThreads) distill_bwd_kernel(const __gr
             if (here(idx[k])) zk[k] = Elem<T>::to_f(w.row[idx[k]]);
         __syncthreads();
     }
-    const float scale = (a.weights ? a.weights[r] : 1.f) * a.g_loss[r] * static_cast<float>(a.inv_T);
+    const float scale = (a.weights ? a.weights[r] : 1.f) * a.g_loss[static_cast<int64_t>(r) * a.g_loss_stride] * static_cast<float>(a.inv_T);
     T* g = static_cast<T*>(a.g) + static_cast<int64_t>(r) * V;
     const GradWriter<T> write(w, g, s, a, scale);
     if (write.fast) {
@@ -760,7 +761,7 @@ extern "C" int dwa_distill_fwd(void* stream, const DwaLogitsDims* dims, const Dw
         return fail(DWA_ERR_INVALID_ARG, "distill: a pointer is not aligned to its element");
     if ((rc = check_workspace(workspace, workspace_bytes))) return rc;
     const DistillArgs a = {logits, *dims, *opts, teacher_logits, teacher_indices, teacher_lse, weights, loss,
-                           reinterpret_cast<RowState*>(state), nullptr, g_logits, static_cast<uint32_t*>(workspace),
+                           reinterpret_cast<RowState*>(state), nullptr, 0, g_logits, static_cast<uint32_t*>(workspace),
                            kLog2e / opts->temperature, 1. / opts->temperature, 1, 0, 0};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dims->dtype == DWA_BF16)
@@ -770,7 +771,8 @@ extern "C" int dwa_distill_fwd(void* stream, const DwaLogitsDims* dims, const Dw
 
 extern "C" int dwa_distill_bwd(void* stream, const DwaLogitsDims* dims, const DwaDistillDims* opts, const void* logits,
                                const void* teacher_logits, const int32_t* teacher_indices, const float* teacher_lse,
-                               const float* weights, const float* state, const float* g_loss, void* g_logits) {
+                               const float* weights, const float* state, const float* g_loss, int g_loss_stride,
+                               void* g_logits) {
     int rc = check_distill(dims, opts, teacher_lse);
     if (rc) return rc;
     if (dims->rows == 0) return DWA_OK;
@@ -781,7 +783,7 @@ extern "C" int dwa_distill_bwd(void* stream, const DwaLogitsDims* dims, const Dw
         return fail(DWA_ERR_INVALID_ARG, "distill: a pointer is not aligned to its element");
     const int log_P = log_ctas_per_row(*dims);
     const DistillArgs a = {logits, *dims, *opts, teacher_logits, teacher_indices, teacher_lse, weights, nullptr,
-                           reinterpret_cast<RowState*>(const_cast<float*>(state)), g_loss, g_logits, nullptr,
+                           reinterpret_cast<RowState*>(const_cast<float*>(state)), g_loss, g_loss_stride, g_logits, nullptr,
                            kLog2e / opts->temperature, 1. / opts->temperature, 1 << log_P, log_P, 0};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const size_t sh = static_cast<size_t>(opts->K) * 4;

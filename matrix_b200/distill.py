@@ -31,9 +31,10 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .runtime import dtype_code, logits_view, ptr, require_cuda, stream_of, workspace
+from .runtime import address, call_on, dtype_code, logits_view, require_cuda, workspace
 
 MAX_TOP = _lib.DWA_MAX_TOP
+_WORKSPACE = 256   # dwa_distill_workspace_bytes()
 
 
 def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0):
@@ -47,10 +48,10 @@ def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0):
     values = torch.empty((*lead, k), dtype=logits.dtype, device=dev)
     indices = torch.empty((*lead, k), dtype=torch.int32, device=dev)
     lse = torch.empty(lead, dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        rc = _lib.load().dwa_top_logits(stream_of(dev), dims, ptr(z), int(k), float(temperature), ptr(values),
-                                        ptr(indices), ptr(lse))
-    _lib.check(rc, "dwa_top_logits")
+    rc = call_on(dev, _lib.load().dwa_top_logits, dims, z.data_ptr(), int(k), float(temperature), values.data_ptr(),
+                 indices.data_ptr(), lse.data_ptr())
+    if rc:
+        _lib.check(rc, "dwa_top_logits")
     return values, indices, lse
 
 
@@ -64,19 +65,25 @@ class _Call:
             raise ValueError(f"teacher_logits must be {[*self.lead, 'K']}, got {list(teacher_logits.shape)}")
         if teacher_indices.shape != teacher_logits.shape:
             raise ValueError("teacher_indices must have the shape of teacher_logits")
-        if teacher_indices.dtype not in (torch.int32, torch.int64):
-            raise TypeError("teacher_indices must be int32 or int64")
         if reverse and teacher_lse is None:
             raise ValueError("reverse=True needs teacher_lse: without it the teacher gives unlisted entries no mass")
-        self.t = self._input("teacher_logits", teacher_logits.detach())
-        self.idx = self._input("teacher_indices", teacher_indices).to(torch.int32)
+        if teacher_indices.dtype != torch.int32:
+            if teacher_indices.dtype != torch.int64:
+                raise TypeError("teacher_indices must be int32 or int64")
+            # an index that does not fit is refused as any other beyond the vocabulary
+            teacher_indices = teacher_indices.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+        self.t = self._input("teacher_logits", teacher_logits)
+        self.idx = self._input("teacher_indices", teacher_indices)
         self.lse = self._row("teacher_lse", teacher_lse)
         self.w = self._row("weights", weights)
         self.opts = _lib.DistillDims(teacher_logits.shape[-1], dtype_code(teacher_logits.dtype, "teacher_logits"),
                                      float(temperature), int(bool(reverse)))
 
     def _input(self, name, t):
-        t = t.contiguous()
+        if t.requires_grad:
+            t = t.detach()
+        if not t.is_contiguous():
+            t = t.contiguous()
         require_cuda(name, t, self.dev)
         return t
 
@@ -87,26 +94,33 @@ class _Call:
             raise ValueError(f"{name} must be {list(self.lead)}, got {list(t.shape)}")
         if t.dtype != torch.float32:
             raise TypeError(f"{name} must be float32")
-        return self._input(name, t.detach())
+        return self._input(name, t)
 
     def _common(self):
-        return ptr(self.z), ptr(self.t), ptr(self.idx), ptr(self.lse), ptr(self.w)
+        return (self.dims, self.opts, self.z.data_ptr(), self.t.data_ptr(), self.idx.data_ptr(), address(self.lse),
+                address(self.w))
 
     def forward(self, state=None, g=None):
         lib = _lib.load()
         loss = torch.empty(self.lead, dtype=torch.float32, device=self.dev)
-        ws = workspace(self.dev, "distill", lib.dwa_distill_workspace_bytes())
-        with torch.cuda.device(self.dev):
-            rc = lib.dwa_distill_fwd(stream_of(self.dev), self.dims, self.opts, *self._common(), ptr(loss), ptr(state),
-                                     ptr(g), ptr(ws), ws.numel())
-        _lib.check(rc, "dwa_distill_fwd")
+        ws = workspace(self.dev, "distill", _WORKSPACE)
+        rc = call_on(self.dev, lib.dwa_distill_fwd, *self._common(), loss.data_ptr(), address(state), address(g),
+                     ws.data_ptr(), ws.numel())
+        if rc:
+            _lib.check(rc, "dwa_distill_fwd")
         return loss
 
     def backward(self, state, g_loss, g):
-        with torch.cuda.device(self.dev):
-            rc = _lib.load().dwa_distill_bwd(stream_of(self.dev), self.dims, self.opts, *self._common(), ptr(state),
-                                             ptr(g_loss), ptr(g))
-        _lib.check(rc, "dwa_distill_bwd")
+        stride = 1
+        if not g_loss.is_contiguous():
+            if any(g_loss.stride()):
+                g_loss = g_loss.contiguous()
+            else:   # one value for all rows, as the backward of a sum hands it over
+                stride = 0
+        rc = call_on(self.dev, _lib.load().dwa_distill_bwd, *self._common(), state.data_ptr(), g_loss.data_ptr(), stride,
+                     g.data_ptr())
+        if rc:
+            _lib.check(rc, "dwa_distill_bwd")
         return g
 
 
@@ -149,7 +163,7 @@ class _DistillFunction(torch.autograd.Function):
         call = ctx.call
         call.z, call.t, call.idx, call.lse, call.w, state = ctx.saved_tensors
         g = torch.empty(ctx.like[0], dtype=ctx.like[1], device=call.dev)
-        call.backward(state, g_loss.float().contiguous(), g)
+        call.backward(state, g_loss, g)
         call.z = call.t = call.idx = call.lse = call.w = None
         return g, None
 

@@ -31,6 +31,24 @@ def stream_of(device: torch.device) -> C.c_void_p:
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def call_on(device: torch.device, fn, *args) -> int:
+    """``fn(stream, *args)``, a libdwa entry point, on ``device`` and its current
+    stream.  The short way for calls whose kernels take microseconds: no device
+    context where ``device`` is current, and no stream object."""
+    index = device.index
+    if _raw_stream is not None and torch.cuda.current_device() == index:
+        return fn(_raw_stream(index), *args)
+    with torch.cuda.device(device):
+        return fn(stream_of(device), *args)
+
+
+def address(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
 def require_cuda(name: str, t: torch.Tensor, device: torch.device | None = None) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
@@ -90,15 +108,17 @@ def logits_view(name: str, t: torch.Tensor) -> tuple[torch.Tensor, "_lib.LogitsD
         raise TypeError(f"{name} must be a torch.Tensor")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on a CUDA device (the hot path has no CPU fallback)")
-    if t.dim() < 1 or t.shape[-1] < 1:
+    shape = t.shape
+    if not shape or shape[-1] < 1:
         raise ValueError(f"{name} must be [..., V] with V >= 1")
-    code, V = dtype_code(t.dtype, name), t.shape[-1]
+    code, V = dtype_code(t.dtype, name), shape[-1]
     if t.is_contiguous():
         rows = t.numel() // V
-        return t, _lib.LogitsDims(rows, max(rows, 1), 0, V, V, code)
+        return t, _lib.LogitsDims(rows, rows or 1, 0, V, V, code)
     rows = 1
     levels: list[list[int]] = []   # [size, stride], innermost first
-    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+    strides = t.stride()
+    for size, stride in zip(reversed(shape[:-1]), reversed(strides[:-1])):
         rows *= size
         if size == 1:
             continue
@@ -106,7 +126,7 @@ def logits_view(name: str, t: torch.Tensor) -> tuple[torch.Tensor, "_lib.LogitsD
             levels[-1][0] *= size
         else:
             levels.append([size, stride])
-    if rows == 0 or len(levels) > 2 or (V > 1 and t.stride(-1) != 1):
+    if rows == 0 or len(levels) > 2 or (V > 1 and strides[-1] != 1):
         return logits_view(name, t.contiguous())
     inner = levels[0] if levels else [1, V]
     outer = levels[1][1] if len(levels) == 2 else 0

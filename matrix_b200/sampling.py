@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .runtime import logits_view, ptr, stream_of
+from .runtime import address, call_on, logits_view
 
 
 def _per_row(name, value, lead, dev, dtype):
@@ -26,7 +26,7 @@ def _per_row(name, value, lead, dev, dtype):
         raise ValueError(f"{name} must be a number or {list(lead)}, got {list(value.shape)}")
     if value.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}")
-    return value.contiguous(), 0
+    return (value if value.is_contiguous() else value.contiguous()), 0
 
 
 def sample_tokens(logits: torch.Tensor, noise: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -40,7 +40,7 @@ def sample_tokens(logits: torch.Tensor, noise: torch.Tensor, *, temperature=1.0,
     largest logit (logprob 0).  A row that holds only -inf, or a NaN, gives token
     -1 and logprob NaN.  Each parameter is a number, or a tensor ``[...]`` with
     one per row (float32; ``top_k`` int32)."""
-    z, dims = logits_view("logits", logits.detach())
+    z, dims = logits_view("logits", logits)
     lead, dev = logits.shape[:-1], logits.device
     if not isinstance(noise, torch.Tensor) or noise.device != dev:
         raise ValueError(f"noise must be a tensor on {dev}")
@@ -48,19 +48,21 @@ def sample_tokens(logits: torch.Tensor, noise: torch.Tensor, *, temperature=1.0,
         raise ValueError("noise must have the shape of logits")
     if noise.dtype != torch.float32:
         raise TypeError("noise must be float32")
-    noise, nd = logits_view("noise", noise)
-    if nd.rows_inner < nd.rows:
-        noise, nd = logits_view("noise", noise.contiguous())
+    stride = dims.V
+    if not noise.is_contiguous():
+        noise, nd = logits_view("noise", noise)
+        if nd.rows_inner < nd.rows:
+            noise, nd = logits_view("noise", noise.contiguous())
+        stride = nd.stride_inner
     t, t0 = _per_row("temperature", temperature, lead, dev, torch.float32)
     k, k0 = _per_row("top_k", top_k, lead, dev, torch.int32)
     p, p0 = _per_row("top_p", top_p, lead, dev, torch.float32)
     m, m0 = _per_row("min_p", min_p, lead, dev, torch.float32)
-    params = _lib.SampleParams(*(None if x is None else x.data_ptr() for x in (t, k, p, m)), float(t0), int(k0),
-                               float(p0), float(m0))
+    params = _lib.SampleParams(address(t), address(k), address(p), address(m), t0, int(k0), p0, m0)
     tokens = torch.empty(lead, dtype=torch.int32, device=dev)
     logprobs = torch.empty(lead, dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        rc = _lib.load().dwa_sample_tokens(stream_of(dev), dims, params, ptr(z), ptr(noise), nd.stride_inner,
-                                           ptr(tokens), ptr(logprobs))
-    _lib.check(rc, "dwa_sample_tokens")
+    rc = call_on(dev, _lib.load().dwa_sample_tokens, dims, params, z.data_ptr(), noise.data_ptr(), stride,
+                 tokens.data_ptr(), logprobs.data_ptr())
+    if rc:
+        _lib.check(rc, "dwa_sample_tokens")
     return tokens, logprobs

@@ -117,7 +117,7 @@ def test_bad_logits_are_refused(lib, bad, code):
     d, p = _dims(**bad), C.c_void_p(256)
     assert lib.dwa_top_logits(None, d, p, 1, 1.0, p, p, p) == code
     assert lib.dwa_distill_fwd(None, d, _lib.DistillDims(1, 0, 1.0, 0), p, p, p, None, None, p, None, None, p, 256) == code
-    assert lib.dwa_distill_bwd(None, d, _lib.DistillDims(1, 0, 1.0, 0), p, p, p, None, None, p, p, p) == code
+    assert lib.dwa_distill_bwd(None, d, _lib.DistillDims(1, 0, 1.0, 0), p, p, p, None, None, p, p, 1, p) == code
     assert lib.dwa_sample_tokens(None, d, _lib.SampleParams(), p, p, 64, p, p) == code
     assert _lib.last_error()
 
@@ -130,7 +130,7 @@ def test_bad_top_and_distill_options_are_refused(lib, k, t, code):
     assert lib.dwa_top_logits(None, d, p, k, t, p, p, p) == code
     o = _lib.DistillDims(k, 0, t, 0)
     assert lib.dwa_distill_fwd(None, d, o, p, p, p, None, None, p, None, None, p, 256) == code
-    assert lib.dwa_distill_bwd(None, d, o, p, p, p, None, None, p, p, p) == code
+    assert lib.dwa_distill_bwd(None, d, o, p, p, p, None, None, p, p, 1, p) == code
 
 
 def test_other_refusals(lib):
@@ -149,7 +149,7 @@ def test_other_refusals(lib):
     for args in ((None, p, p), (p, None, p), (p, p, None)):
         assert lib.dwa_distill_fwd(None, d, o, *args, None, None, p, None, None, p, 256) == -1
     assert lib.dwa_distill_fwd(None, d, o, odd, p, p, None, None, p, None, None, p, 256) == -1
-    assert lib.dwa_distill_bwd(None, d, o, p, p, p, None, None, None, p, p) == -1
+    assert lib.dwa_distill_bwd(None, d, o, p, p, p, None, None, None, p, 1, p) == -1
     assert lib.dwa_top_logits(None, d, None, 4, 1.0, p, p, p) == -1
     assert lib.dwa_top_logits(None, d, odd, 4, 1.0, p, p, p) == -1
     s = _lib.SampleParams()
