@@ -660,8 +660,8 @@ static int check_distill(const DwaLogitsDims* d, const DwaDistillDims* o, const 
     if (o->K > DWA_MAX_TOP) return fail(DWA_ERR_UNSUPPORTED, "distill: K > " + std::to_string(DWA_MAX_TOP));
     if (o->teacher_dtype != DWA_F32 && o->teacher_dtype != DWA_BF16)
         return fail(DWA_ERR_INVALID_ARG, "distill: teacher_dtype must be DWA_F32 or DWA_BF16");
-    if (!(o->temperature > 0.f) || o->temperature > 1e30f)
-        return fail(DWA_ERR_INVALID_ARG, "distill: temperature must be positive and finite");
+    if (!(o->temperature >= 1e-30f && o->temperature <= 1e30f))
+        return fail(DWA_ERR_INVALID_ARG, "distill: temperature must be in [1e-30, 1e30]");
     if (o->reverse && !t_lse)
         return fail(DWA_ERR_INVALID_ARG, "distill: the reverse divergence needs the teacher's log-sum-exp");
     return DWA_OK;

@@ -30,8 +30,8 @@ constexpr int kSelList = 2048;                // candidates held
 constexpr int kTryTop = 256;                  // entries sorted first when only a mass or a floor limits the row
 constexpr int kSelMaxCluster = 8;
 constexpr int kBins = 2048;                   // bins of a wide cut: 32 octaves of weight, 64 bins each, at first
-constexpr float kUnit = 262144.f;             // 2^18: a weight is 2^36 units, in two parts of 18 bits
-constexpr int kDrain = 8192;                  // entries after which a bin's 32-bit parts are emptied: 2^13 * 2^18
+constexpr float kFraction = 131072.f;         // 2^17: a weight is counted in parts of its bin's largest
+constexpr int kDrain = 16384;                 // entries after which the 32-bit bins are emptied: 2^14 * 2^17
 
 // A logit as an unsigned integer of the same order.
 __device__ __forceinline__ uint32_t ordered(float z) {
@@ -48,32 +48,18 @@ __device__ __forceinline__ int key_index(uint64_t key) { return static_cast<int>
 // weights far below the largest the same way, and with them a nucleus' edge.
 struct Weigh {
     float m, c, c_lo;
-    __device__ __forceinline__ Weigh(float m_, float T) : m(m_) {
+    __device__ __forceinline__ Weigh(float m_, float T) : m(m_) {   // 1e-30 <= T <= 1e30
         const double cd = 1.4426950408889634 / T;
         c = static_cast<float>(cd);
-        c_lo = isinf(c) ? 0.f : static_cast<float>(cd - c);
+        c_lo = static_cast<float>(cd - c);
     }
-    // log2 of the weight: 0 at the maximum, -inf for what has none
+    // log2 of the weight: 0 at the maximum, below -1e8 for -inf (which 2^x takes to 0)
     __device__ __forceinline__ float log2_of(float z) const {
-        const float d = z - m;
-        return z == m ? 0.f : z == -INFINITY || m == INFINITY ? -INFINITY : fmaf(d, c, d * c_lo);
+        const float d = z == m ? 0.f : fmaxf(z - m, -3.4e38f);
+        return fmaf(d, c, d * c_lo);
     }
     __device__ __forceinline__ float operator()(float z) const { return exp2_fast(log2_of(z)); }
 };
-
-// An entry's measure: 1, or its weight in units of 2^-36 of the largest; in two
-// parts of 18 bits (and one bit more when they round up).
-template <bool MASS>
-__device__ __forceinline__ void measure(float log2_w, uint32_t& hi, uint32_t& lo) {
-    if constexpr (MASS) {
-        const float x = exp2_fast(log2_w) * kUnit;
-        hi = static_cast<uint32_t>(x);
-        lo = static_cast<uint32_t>(rintf((x - static_cast<float>(hi)) * kUnit));
-    } else {
-        hi = 0u;
-        lo = 1u;
-    }
-}
 
 // The `target`-th largest key of a row by one block, eight bits of the key a
 // pass.  hist: 256 values, found: 2 values in shared memory.
@@ -148,11 +134,11 @@ struct SelShared {
     union {
         uint32_t group[kSelGroups];
         unsigned long long hist[256];
-        uint32_t bin[2][kBins];          // high and low part of a bin's measure
+        uint32_t bin[kBins];             // a wide cut's histogram
     };
     union {
         unsigned long long list[kSelList];   // candidates; sorted: the K largest in descending order
-        unsigned long long sum[kBins];       // the bins' measure so far
+        unsigned long long sum[kBins];       // the bins so far
     };
     uint16_t chosen[kSelGroups];
     unsigned long long part_lo[kSelMaxCluster], part_hi[kSelMaxCluster];
@@ -162,9 +148,9 @@ struct SelShared {
     uint32_t warp_count[2][kSelThreads / 32];
     unsigned long long found[2];
     unsigned long long red64[33];
-    double redd[33], scan[kSelThreads / 32 + 1];
+    double redd[33], scan[kSelThreads / 32 + 1], found_at;
     float redf[33];
-    int n_chosen, n_list;
+    int n_chosen, n_list, first, last;
 };
 
 // This CTA's share: the maxima of the thread's words by position mod 8 (`edge`:
@@ -241,21 +227,33 @@ __device__ __forceinline__ void row_stats(const SelShared& sh, int P, float c, f
 // The first n <= kSelList keys of sh.list into descending order.
 __device__ void sort_list(SelShared& sh, int n) {
     const int tid = threadIdx.x;
-    if (n <= kSelThreads) {   // each key to its rank
-        const unsigned long long key = tid < n ? sh.list[tid] : 0ull;
-        int rank = 0;
-        for (int i = 0; i < n; ++i) rank += sh.list[i] > key;
+    if (n <= 2 * kSelThreads) {   // each key to its rank
+        const bool two = n > kSelThreads;
+        const unsigned long long a = tid < n ? sh.list[tid] : 0ull, b = tid + kSelThreads < n ? sh.list[tid + kSelThreads] : 0ull;
+        int ra = 0, rb = 0;
+        if (two) {
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) {
+                const unsigned long long k = sh.list[i];
+                ra += k > a;
+                rb += k > b;
+            }
+        } else {
+#pragma unroll 8
+            for (int i = 0; i < n; ++i) ra += sh.list[i] > a;
+        }
         __syncthreads();
-        if (tid < n) sh.list[rank] = key;
-    } else {                  // bitonic, padded to a power of two
-        int size = 2 * kSelThreads;
+        if (tid < n) sh.list[ra] = a;
+        if (tid + kSelThreads < n) sh.list[rb] = b;
+    } else {                      // bitonic, padded to a power of two
+        int size = 4 * kSelThreads;
         while (size < n) size <<= 1;
         for (int i = n + tid; i < size; i += kSelThreads) sh.list[i] = 0ull;
         for (int k = 2; k <= size; k <<= 1) {
             for (int j = k >> 1; j > 0; j >>= 1) {
                 __syncthreads();
                 for (int i = tid; i < size / 2; i += kSelThreads) {
-                    const int a = (i / j) * 2 * j + i % j, b = a + j;
+                    const int a = 2 * i - (i & (j - 1)), b = a + j;
                     const unsigned long long x = sh.list[a], y = sh.list[b];
                     if ((x < y) == ((a & k) == 0)) {
                         sh.list[a] = y;
@@ -268,9 +266,10 @@ __device__ void sort_list(SelShared& sh, int n) {
     __syncthreads();
 }
 
-// Rank 0: the K largest entries of the row into sh.list, in descending order.
+// Rank 0: the K largest entries of the row, and a few more, into sh.list in any
+// order; their number.
 template <class T>
-__device__ void sort_top(SelShared& sh, const RowWords<T>& w, int log_P, int K) {
+__device__ int collect_top(SelShared& sh, const RowWords<T>& w, int log_P, int K) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint32_t g[8];
 #pragma unroll
@@ -304,33 +303,35 @@ __device__ void sort_top(SelShared& sh, const RowWords<T>& w, int log_P, int K) 
     for (int i = 0; i < 8; ++i)
         if (g[i] >= t) sh.chosen[atomicAdd(&sh.n_chosen, 1)] = static_cast<uint16_t>(i * kSelThreads + tid);
     __syncthreads();
-    const int per = 8 >> log_P, chosen = sh.n_chosen;
-    const int rounds = (((w.words - 1) >> log_P) + kSelThreads * per) / (kSelThreads * per);   // words of a group, or more
-    const uint64_t floor = static_cast<uint64_t>(t) << 48;
+    // a group: words lo + x + (u + i per) NT, i = 0, 1, ..., of chunk p, where its
+    // number is (p per + u) NT + x
+    const int log_per = 3 - log_P, chosen = sh.n_chosen;
+    const int rounds = (((w.words - 1) >> log_P) + (kSelThreads << log_per)) / (kSelThreads << log_per);   // words, or more
+    const int log_rounds = rounds > 1 ? 32 - __clz(rounds - 1) : 0;
+    const float least = unordered(t << 16);   // NaN where even -inf reaches the prefix
     const auto take = [&](uint4 x, int j0) {
         float v[kRowVec<T>];
         unpack<T>(x, v);
 #pragma unroll
         for (int e = 0; e < kRowVec<T>; ++e) {
-            const uint64_t key = entry_key(v[e], j0 + e);
-            if (key >= floor && static_cast<unsigned>(j0 + e) < static_cast<unsigned>(w.V)) {
+            if (!(v[e] < least) && static_cast<unsigned>(j0 + e) < static_cast<unsigned>(w.V)) {
                 const int to = atomicAdd(&sh.n_list, 1);
-                if (to < kSelList) sh.list[to] = key;
+                if (to < kSelList) sh.list[to] = entry_key(v[e], j0 + e);
             }
         }
     };
     constexpr int U = 4;
-    for (int i0 = tid; i0 < chosen * rounds; i0 += U * kSelThreads) {
+    for (int i0 = tid; i0 < chosen << log_rounds; i0 += U * kSelThreads) {
         uint4 x[U];
         int at[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * kSelThreads;
+            const int i = i0 + u * kSelThreads, k = i & ((1 << log_rounds) - 1);
             at[u] = -1;
-            if (i < chosen * rounds) {
-                const int q = sh.chosen[i / rounds], p = q / (kSelThreads * per), r = q % (kSelThreads * per);
-                const Chunk ch(w.words, p, log_P);
-                const int word = ch.lo + r % kSelThreads + (r / kSelThreads + (i % rounds) * per) * kSelThreads;
+            if (i < chosen << log_rounds && k < rounds) {
+                const int q = sh.chosen[i >> log_rounds], r = q / kSelThreads;
+                const Chunk ch(w.words, r >> log_per, log_P);
+                const int word = ch.lo + q % kSelThreads + ((r & ((1 << log_per) - 1)) + (k << log_per)) * kSelThreads;
                 if (word < ch.hi && w.whole(word)) {
                     at[u] = word;
                     x[u] = w.word(word);
@@ -338,9 +339,8 @@ __device__ void sort_top(SelShared& sh, const RowWords<T>& w, int log_P, int K) 
             }
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < U; ++u)
             if (at[u] >= 0) take(x[u], w.first(at[u]));
-        }
     }
     w.edges(0, w.words, tid, take);
     __syncthreads();
@@ -362,7 +362,7 @@ __device__ void sort_top(SelShared& sh, const RowWords<T>& w, int log_P, int K) 
         __syncthreads();
         n = K;
     }
-    sort_list(sh, n);
+    return n;
 }
 
 struct TopArgs {
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kSelThreads, 4) top_logits_kernel(TopArgs a) {
         row_stats(sh, P, a.c, m, s);
         a.lse[r] = m != m || isinf(m) ? m : static_cast<float>(0.6931471805599453 * (Ref(m, a.c).a(a.c) + log2f(s)));
     }
-    sort_top(sh, w, a.log_P, a.K);
+    sort_list(sh, collect_top(sh, w, a.log_P, a.K));
     for (int k = tid; k < a.K; k += kSelThreads) {
         const unsigned long long key = sh.list[k];
         static_cast<T*>(a.values)[static_cast<int64_t>(r) * a.K + k] = Elem<T>::from_f(unordered(static_cast<uint32_t>(key >> 32)));
@@ -430,6 +430,7 @@ struct Request {
         if (k <= 0 || k > V) k = V;
         min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
         top_p = top_p < 1.f ? fmaxf(top_p, 0.f) : 1.f;
+        T = fminf(fmaxf(T, 1e-30f), 1e30f);   // all that tells logits apart, or none
         if (greedy) {
             T = 1.f;
             k = 1;
@@ -476,119 +477,140 @@ __device__ __forceinline__ void tell(SelShared& sh, int P, int p, uint64_t a, ui
 // descending order, reach `target` in number or, with MASS, the part top_p of
 // their mass.  A histogram of the measure finds the bin of the cut and what lies
 // above it; the bin's entries go to rank 0, which sorts them and walks to the
-// cut.  Bins are even in the logarithm of the weight; where one holds more than
-// can be sorted (equal logits), the bins of the next round divide its keys.
-// All sums are whole numbers, so no order of additions shows in the result.
+// cut.  Bins are even in the logarithm of the weight, so that a bin's weights
+// differ by one percent and are counted as whole parts of the largest: sums that
+// no order of additions changes, one 32-bit atomic an entry.  Where a bin holds
+// more than can be sorted (equal logits), the bins of the next round divide its
+// keys.
 template <class T, bool MASS>
 __device__ uint64_t wide_cut(SelShared& sh, const RowWords<T>& w, Chunk ch, int p, int P, const Weigh& weigh,
-                             uint64_t floor, uint64_t target, float top_p) {
+                             uint64_t floor, uint64_t count, float top_p) {
     namespace cg = cooperative_groups;
     cg::cluster_group cl = cg::this_cluster();
     constexpr int VEC = kRowVec<T>, PER = kBins / kSelThreads;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint64_t key_lo = floor, key_hi = ~uint64_t(0);   // the cut lies in here
     int shift = -1;                                   // < 0: bins of the logarithm of the weight
-    for (;;) {
-        const auto bin_of = [&](uint64_t key, float log2_w) {
-            return shift < 0 ? static_cast<int>(fminf(log2_w * -64.f, kBins - 1.f))
-                             : static_cast<int>((key_hi - key) >> shift);
-        };
-        // the histogram of this CTA's share
-        __syncthreads();
-        for (int i = tid; i < kBins; i += kSelThreads) {
-            sh.bin[0][i] = sh.bin[1][i] = 0u;
-            sh.sum[i] = 0ull;
-        }
-        __syncthreads();
-        for (int a = ch.lo; a < ch.hi; a += kDrain / VEC) {
-            const int b = a + kDrain / VEC < ch.hi ? a + kDrain / VEC : ch.hi;
-            w.template each<2>(a, b, tid, kSelThreads, [&](uint4 x, int j0, int) {
-                float v[VEC];
-                unpack<T>(x, v);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const uint64_t key = entry_key(v[i], j0 + i);
-                    if (key < key_lo || key > key_hi || static_cast<unsigned>(j0 + i) >= static_cast<unsigned>(w.V)) continue;
-                    const float l = weigh.log2_of(v[i]);
-                    uint32_t hi, lo;
-                    measure<MASS>(l, hi, lo);
-                    const int at = bin_of(key, l);
-                    if (hi) atomicAdd(&sh.bin[0][at], hi);
-                    if (lo) atomicAdd(&sh.bin[1][at], lo);
-                }
-            });
-            __syncthreads();
-            for (int i = tid; i < kBins; i += kSelThreads) {
-                sh.sum[i] += (static_cast<unsigned long long>(sh.bin[0][i]) << 18) + sh.bin[1][i];
-                sh.bin[0][i] = sh.bin[1][i] = 0u;
-            }
-            __syncthreads();
-        }
-        cl.sync();
-        // rank 0: the bin of the cut
-        if (p == 0) {
-            unsigned long long v[PER], own = 0ull;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) v[i] = 0ull;
-            for (int q = 0; q < P; ++q) {
-                const unsigned long long* from = cl.map_shared_rank(sh.sum, q) + tid * PER;
-#pragma unroll
-                for (int i = 0; i < PER; ++i) v[i] += from[i];
-            }
-#pragma unroll
-            for (int i = 0; i < PER; ++i) own += v[i];
-            unsigned long long incl = own;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned long long up = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += up;
-            }
-            if (lane == 31) sh.red64[warp] = incl;
-            __syncthreads();
-            unsigned long long all = 0ull, acc = incl - own;
-#pragma unroll
-            for (int i = 0; i < kSelThreads / 32; ++i) {
-                if (i < warp) acc += sh.red64[i];
-                all += sh.red64[i];
-            }
-            if (MASS && target == 0) {
-                const double want = ceil(static_cast<double>(top_p) * static_cast<double>(all));
-                target = want < 1. ? 1ull : static_cast<unsigned long long>(want);
-            }
-            if (acc < target && target <= acc + own) {   // one thread
-                int i = 0;
-#pragma unroll
-                for (int k = 0; k < PER - 1; ++k)
-                    if (i == k && acc + v[k] < target) {
-                        acc += v[k];
-                        i = k + 1;
-                    }
-                sh.found[0] = static_cast<unsigned long long>(tid * PER + i);
-                sh.found[1] = acc;
-            }
-            if (tid == 0) sh.n_list = 0;
-            __syncthreads();
-        }
-        tell(sh, P, p, sh.found[0], target, sh.found[1], 0);
-        const int cut_bin = static_cast<int>(sh.told[0]);
-        target = sh.told[1] - sh.told[2];   // what is left to reach inside the bin
-        // its entries to rank 0
-        SelShared* to = cl.map_shared_rank(&sh, 0);
-        unsigned long long least = ~0ull, most = 0ull;
-        w.template each<2>(ch.lo, ch.hi, tid, kSelThreads, [&](uint4 x, int j0, int) {
+    double target = static_cast<double>(count);       // with MASS set by the first round
+    float top_l = 0.f;                                // log2 of the largest weight in question (shift >= 0)
+    // f(z, its index, log2 of its weight, its bin) for the entries in question
+    const auto each_entry = [&](int lo, int hi, auto f) {
+        const bool bounded = key_lo > 0 || shift >= 0;
+        w.template each<2>(lo, hi, tid, kSelThreads, [&](uint4 x, int j0, int u) {
             float v[VEC];
             unpack<T>(x, v);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const unsigned long long key = entry_key(v[i], j0 + i);
-                if (key < key_lo || key > key_hi || static_cast<unsigned>(j0 + i) >= static_cast<unsigned>(w.V) ||
-                    bin_of(key, weigh.log2_of(v[i])) != cut_bin)
-                    continue;
-                least = key < least ? key : least;
-                most = key > most ? key : most;
-                const int at = atomicAdd(&to->n_list, 1);
-                if (at < kSelList) to->list[at] = key;
+                if (u < 0 && static_cast<unsigned>(j0 + i) >= static_cast<unsigned>(w.V)) continue;
+                const float l = weigh.log2_of(v[i]);
+                int bin = static_cast<int>(fminf(l * -64.f, kBins - 1.f));
+                if (bounded) {
+                    const uint64_t key = entry_key(v[i], j0 + i);
+                    if (key < key_lo || key > key_hi) continue;
+                    if (shift >= 0) bin = static_cast<int>((key_hi - key) >> shift);
+                }
+                f(v[i], j0 + i, l, bin);
             }
+        });
+    };
+    // a bin's measure: of a full part of it, in units of the largest weight
+    const auto part_of = [&](int bin) {
+        return !MASS ? 1. : static_cast<double>(exp2f(shift < 0 ? static_cast<float>(bin) * (-1.f / 64.f) : top_l)) / kFraction;
+    };
+    for (;;) {
+        // the histogram of this CTA's share
+        __syncthreads();
+        for (int i = tid; i < kBins; i += kSelThreads) {
+            sh.bin[i] = 0u;
+            sh.sum[i] = 0ull;
+        }
+        __syncthreads();
+        for (int a = ch.lo; a < ch.hi; a += kDrain / VEC) {
+            each_entry(a, a + kDrain / VEC < ch.hi ? a + kDrain / VEC : ch.hi, [&](float, int, float l, int bin) {
+                const float up = shift < 0 ? static_cast<float>(bin) * (1.f / 64.f) : -top_l;
+                atomicAdd(&sh.bin[bin], MASS ? static_cast<uint32_t>(rintf(exp2_fast(l + up) * kFraction)) : 1u);
+            });
+            __syncthreads();
+            for (int i = tid; i < kBins; i += kSelThreads) {
+                sh.sum[i] += sh.bin[i];
+                sh.bin[i] = 0u;
+            }
+            __syncthreads();
+        }
+        if (P > 1) {   // CTA p adds bins kBins p / P ... of all, for rank 0
+            cl.sync();
+            unsigned long long* to = cl.map_shared_rank(sh.sum, 0);
+            const int n = kBins / P;
+            for (int i = p * n + tid; i < (p + 1) * n; i += kSelThreads) {
+                unsigned long long v[kSelMaxCluster], all = 0ull;
+#pragma unroll
+                for (int q = 0; q < kSelMaxCluster; ++q) v[q] = q < P ? cl.map_shared_rank(sh.sum, q)[i] : 0ull;
+#pragma unroll
+                for (int q = 0; q < kSelMaxCluster; ++q) all += v[q];
+                to[i] = all;   // read above by this thread alone
+            }
+            cl.sync();
+        }
+        // rank 0: the bin of the cut
+        if (p == 0) {
+            double v[PER], own = 0.;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                v[i] = static_cast<double>(sh.sum[tid * PER + i]) * part_of(tid * PER + i);
+                own += v[i];
+            }
+            double incl = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double up = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += up;
+            }
+            if (lane == 31) sh.scan[warp] = incl;
+            if (tid == 0) {
+                sh.n_list = 0;
+                sh.first = kSelThreads;
+                sh.last = 0;
+            }
+            __syncthreads();
+            double all = 0., acc = incl - own;
+#pragma unroll
+            for (int i = 0; i < kSelThreads / 32; ++i) {
+                if (i < warp) acc += sh.scan[i];
+                all += sh.scan[i];
+            }
+            if (MASS && shift < 0) target = static_cast<double>(top_p) * all;
+            // the first bin to reach the target, or where rounding leaves none the last that holds something
+            if (own > 0.) {
+                if (acc + own >= target) atomicMin(&sh.first, tid);
+                atomicMax(&sh.last, tid);
+            }
+            __syncthreads();
+            if (tid == (sh.first < kSelThreads ? sh.first : sh.last)) {
+                bool there = false;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    if (there || v[i] == 0.) continue;
+                    sh.found[0] = static_cast<unsigned long long>(tid * PER + i);
+                    sh.found_at = acc;
+                    acc += v[i];
+                    there = acc >= target;
+                }
+            }
+            __syncthreads();
+        }
+        tell(sh, P, p, sh.found[0], __double_as_longlong(target), __double_as_longlong(sh.found_at), 0);
+        const int cut_bin = static_cast<int>(sh.told[0]);
+        target = __longlong_as_double(sh.told[1]) - __longlong_as_double(sh.told[2]);   // left to reach inside the bin
+        // its entries to rank 0
+        SelShared* to = cl.map_shared_rank(&sh, 0);
+        unsigned long long least = ~0ull, most = 0ull;
+        each_entry(ch.lo, ch.hi, [&](float z, int j, float, int bin) {
+            if (bin != cut_bin) return;
+            const unsigned long long key = entry_key(z, j);
+            least = key < least ? key : least;
+            most = key > most ? key : most;
+            const int at = atomicAdd(&to->n_list, 1);
+            if (at < kSelList) to->list[at] = key;
         });
         least = ~block_reduce(~least, MaxOp(), 0ull, sh.red64);
         most = block_reduce(most, MaxOp(), 0ull, sh.red64);
@@ -603,34 +625,35 @@ __device__ uint64_t wide_cut(SelShared& sh, const RowWords<T>& w, Chunk ch, int 
                 sort_list(sh, n);
                 constexpr int MOST = kSelList / kSelThreads;
                 const int per = (n + kSelThreads - 1) / kSelThreads;
-                unsigned long long own = 0ull, u[MOST];
+                double own = 0., u[MOST];
 #pragma unroll
                 for (int i = 0; i < MOST; ++i) {
-                    u[i] = 0ull;
-                    if (i < per && tid * per + i < n) {
-                        uint32_t hi, lo;
-                        measure<MASS>(weigh.log2_of(unordered(static_cast<uint32_t>(sh.list[tid * per + i] >> 32))), hi, lo);
-                        u[i] = (static_cast<unsigned long long>(hi) << 18) + lo;
-                    }
+                    u[i] = 0.;
+                    if (i < per && tid * per + i < n)
+                        u[i] = MASS ? weigh(unordered(static_cast<uint32_t>(sh.list[tid * per + i] >> 32))) : 1.;
                     own += u[i];
                 }
-                unsigned long long incl = own;
+                double incl = own;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
-                    const unsigned long long up = __shfl_up_sync(0xffffffffu, incl, o);
+                    const double up = __shfl_up_sync(0xffffffffu, incl, o);
                     if (lane >= o) incl += up;
                 }
-                if (lane == 31) sh.red64[warp] = incl;
+                if (lane == 31) sh.scan[warp] = incl;
+                if (tid == 0) sh.first = n - 1;   // where rounding leaves the target unreached
                 __syncthreads();
-                unsigned long long acc = incl - own;
-                for (int i = 0; i < warp; ++i) acc += sh.red64[i];
-                if (acc < target && target <= acc + own) {
+                double acc = incl - own;
+                for (int i = 0; i < warp; ++i) acc += sh.scan[i];
+                bool there = false;
 #pragma unroll
-                    for (int i = 0; i < MOST; ++i) {
-                        if (acc < target && acc + u[i] >= target) sh.found[0] = sh.list[tid * per + i];
-                        acc += u[i];
-                    }
+                for (int i = 0; i < MOST; ++i) {
+                    acc += u[i];
+                    if (there || i >= per || tid * per + i >= n || acc < target) continue;
+                    there = true;
+                    atomicMin(&sh.first, tid * per + i);
                 }
+                __syncthreads();
+                if (tid == 0) sh.found[0] = sh.list[sh.first];
                 sh.found[1] = 1ull;
             } else {
                 sh.found[1] = 0ull;
@@ -649,18 +672,39 @@ __device__ uint64_t wide_cut(SelShared& sh, const RowWords<T>& w, Chunk ch, int 
         if (sh.told[1]) return sh.told[0];
         key_lo = sh.told[2];
         key_hi = sh.told[3];
+        top_l = weigh.log2_of(unordered(static_cast<uint32_t>(key_hi >> 32)));
         shift = 0;
         while ((key_hi - key_lo) >> shift >= kBins) ++shift;
+    }
+}
+
+// The numbers of one word's entries; `inside`: all of them lie in the row.
+template <int VEC>
+__device__ __forceinline__ void load_noise(const float* noise, int j0, int V, bool inside, float* e) {
+    const float* p = noise + j0;
+    if (inside && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(p + i);
+            e[i] = x.x;
+            e[i + 1] = x.y;
+            e[i + 2] = x.z;
+            e[i + 3] = x.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) e[i] = static_cast<unsigned>(j0 + i) < static_cast<unsigned>(V) ? p[i] : 1.f;
     }
 }
 
 // The whole cluster, any row with a finite maximum or +inf: the cuts, then the
 // race over what stays.
 template <class T>
-__device__ void sample_wide(SelShared& sh, const SampleArgs& a, const RowWords<T>& w, Chunk ch, int p, int64_t r,
+__device__ void sample_wide(SelShared& sh, const SampleArgs& a, const RowWords<T>& w, Chunk ch, int p, uint32_t r,
                             const Request& q, const float* noise, float m) {
     namespace cg = cooperative_groups;
     cg::cluster_group cl = cg::this_cluster();
+    constexpr int VEC = kRowVec<T>;
     const int tid = threadIdx.x, P = a.P;
     const Weigh weigh(m, q.T);
     uint64_t floor = 0;
@@ -670,17 +714,23 @@ __device__ void sample_wide(SelShared& sh, const SampleArgs& a, const RowWords<T
     const int fj = floor ? key_index(floor) : w.V;
     unsigned long long best = 0ull;
     float kept = 0.f;
-    w.template each<4>(ch.lo, ch.hi, tid, kSelThreads, [&](uint4 x, int j0, int) {
-        float v[kRowVec<T>];
+    w.template each<2>(ch.lo, ch.hi, tid, kSelThreads, [&](uint4 x, int j0, int u) {
+        float v[VEC], e[VEC];
         unpack<T>(x, v);
+        if (!(word_max<T>(x) >= fz)) return;
 #pragma unroll
-        for (int i = 0; i < kRowVec<T>; ++i) {
-            const int j = j0 + i;
-            const float e = weigh(v[i]);
-            if (!(v[i] > fz || (v[i] == fz && j <= fj)) || !(e > 0.f && e >= q.min_p)) continue;
-            kept += e;
-            const float score = __fdividef(e, noise[j]);
-            const unsigned long long key = race_key(score, j);
+        for (int i = 0; i < VEC; ++i) {
+            e[i] = weigh(v[i]);
+            if (!(v[i] > fz || (v[i] == fz && j0 + i <= fj)) || !(e[i] >= q.min_p)) e[i] = 0.f;
+        }
+        float number[VEC];
+        load_noise<VEC>(noise, j0, w.V, u >= 0, number);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            if (!(e[i] > 0.f)) continue;
+            kept += e[i];
+            const float score = __fdividef(e[i], number[i]);
+            const unsigned long long key = race_key(score, j0 + i);
             if (score >= 0.f && key > best) best = key;
         }
     });
@@ -701,6 +751,23 @@ __device__ void sample_wide(SelShared& sh, const SampleArgs& a, const RowWords<T
         }
         write_token(a, w, r, q, m, best, all);
     }
+}
+
+// Rank 0: whether the n collected entries may hold all that stays of a row of
+// which only a mass or a floor limits it: their mass reaches `limit`, or fewer
+// than kTryTop reach the floor.
+__device__ __forceinline__ bool may_hold_all(SelShared& sh, int n, const Request& q, float m, double limit) {
+    const Weigh weigh(m, q.T);
+    double mass = 0.;
+    int above = 0;
+    for (int i = threadIdx.x; i < n; i += kSelThreads) {
+        const float e = weigh(unordered(static_cast<uint32_t>(sh.list[i] >> 32)));
+        mass += e;
+        above += e > 0.f && e >= q.min_p;
+    }
+    mass = block_reduce(mass, AddOp(), 0., sh.redd);
+    above = block_reduce(above, AddOp(), 0, reinterpret_cast<int*>(sh.redf));
+    return mass >= limit || above < kTryTop;
 }
 
 // Rank 0: the draw among the n largest entries, sorted in sh.list.  `total`: the
@@ -774,7 +841,9 @@ __device__ __forceinline__ void race_chunk(const RowWords<T>& w, Chunk ch, float
     top = -INFINITY;
     best = 0.f;
     best_j = -1;
-    w.template each<2>(ch.lo, ch.hi, threadIdx.x, kSelThreads, [&](uint4 x, int j0, int) {
+    w.template each<2>(ch.lo, ch.hi, threadIdx.x, kSelThreads, [&](uint4 x, int j0, int u) {
+        float number[VEC];
+        load_noise<VEC>(noise, j0, w.V, u >= 0, number);
         const float m = word_max<T>(x);
         top = max_nan(top, m);
         float e[VEC], score[VEC];
@@ -798,8 +867,7 @@ __device__ __forceinline__ void race_chunk(const RowWords<T>& w, Chunk ch, float
         float lead = -1.f;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            score[i] = -1.f;
-            if (e[i] > 0.f) score[i] = __fdividef(e[i], noise[j0 + i]);   // e > 0 only inside the row
+            score[i] = e[i] > 0.f ? __fdividef(e[i], number[i]) : -1.f;   // e > 0 only inside the row
             lead = fmaxf(lead, score[i]);
         }
         if (lead > best || best_j < 0) {
@@ -874,12 +942,23 @@ __global__ void __launch_bounds__(kSelThreads, 4) sample_kernel(SampleArgs a) {
         push_groups(sh, p, P, top, edge, ms, c);
         if (p == 0) {
             row_stats(sh, P, c, m, s);
-            // a mass relative to +inf, or of the k largest of many, is not at hand
-            if (m > -INFINITY && (list || (m < INFINITY && (masses || q.top_p >= 1.f) && limited))) {
-                const int n = list ? q.k : kTryTop;
-                sort_top(sh, w, a.log_P, n);
-                done = sample_listed(sh, a, w, r, q, noise, m, n,
-                                     masses ? s * exp2(Ref(m, c).a(c) - static_cast<double>(m) * c) : -1., list);
+            if (list) {
+                if (m > -INFINITY) {
+                    sort_list(sh, collect_top(sh, w, a.log_P, q.k));
+                    done = sample_listed(sh, a, w, r, q, noise, m, q.k, -1., true);
+                }
+            } else if (fabsf(m) < INFINITY && (masses || q.top_p >= 1.f) && limited) {
+                // (a mass relative to +inf, or of the k largest of many, is not at hand)
+                const double total = masses ? s * exp2(Ref(m, c).a(c) - static_cast<double>(m) * c) : 0.;
+                const double limit = masses ? q.top_p * total : INFINITY;
+                if (limit <= kTryTop || q.min_p > 0.f) {   // else more than kTryTop of the largest weight
+                    const int n = collect_top(sh, w, a.log_P, kTryTop);
+                    if (may_hold_all(sh, n, q, m, limit)) {
+                        sort_list(sh, n);
+                        done = sample_listed(sh, a, w, r, q, noise, m, kTryTop, total, false);
+                    }
+                }
+                __syncthreads();
             }
         }
         if (list && p != 0) return;
@@ -924,8 +1003,8 @@ extern "C" int dwa_top_logits(void* stream, const DwaLogitsDims* dims, const voi
     if (rc) return rc;
     if (K <= 0 || K > dims->V) return fail(DWA_ERR_INVALID_ARG, "top_logits: K must be in [1, V]");
     if (K > DWA_MAX_TOP) return fail(DWA_ERR_UNSUPPORTED, "top_logits: K > " + std::to_string(DWA_MAX_TOP));
-    if (!(temperature > 0.f) || temperature > 1e30f)
-        return fail(DWA_ERR_INVALID_ARG, "top_logits: temperature must be positive and finite");
+    if (!(temperature >= 1e-30f && temperature <= 1e30f))
+        return fail(DWA_ERR_INVALID_ARG, "top_logits: temperature must be in [1e-30, 1e30]");
     if (dims->rows == 0) return DWA_OK;
     if (!logits || !values || !indices || !lse) return fail(DWA_ERR_INVALID_ARG, "top_logits: a required pointer is NULL");
     if (reinterpret_cast<uintptr_t>(logits) % dtype_bytes(dims->dtype) ||
