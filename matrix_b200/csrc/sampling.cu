@@ -473,6 +473,67 @@ __device__ __forceinline__ void tell(SelShared& sh, int P, int p, uint64_t a, ui
     cl.sync();
 }
 
+// Rank 0: drops from the n entries of sh.list, one of which reaches `target` in
+// number or mass, most that lie above or below it; n and target follow.  256 bins
+// of the keys, counted like the bins of the whole row.
+template <bool MASS>
+__device__ void narrow_list(SelShared& sh, int& n, const Weigh& weigh, double& target) {
+    constexpr int MOST = kSelList / kSelThreads;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    unsigned long long key[MOST], least = ~0ull, most = 0ull;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+        key[i] = 0ull;
+        if (tid + i * kSelThreads >= n) continue;
+        key[i] = sh.list[tid + i * kSelThreads];
+        least = key[i] < least ? key[i] : least;
+        most = key[i] > most ? key[i] : most;
+    }
+    least = ~block_reduce(~least, MaxOp(), 0ull, sh.red64);
+    most = block_reduce(most, MaxOp(), 0ull, sh.red64);
+    int shift = 0;
+    while ((most - least) >> shift >= kSelThreads) ++shift;
+    const float top_l = MASS ? weigh.log2_of(unordered(static_cast<uint32_t>(most >> 32))) : 0.f;
+    sh.bin[tid] = 0u;
+    if (tid == 0) {
+        sh.first = kSelThreads;
+        sh.last = 0;
+        sh.n_list = 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+        if (tid + i * kSelThreads >= n) continue;
+        const float l = MASS ? weigh.log2_of(unordered(static_cast<uint32_t>(key[i] >> 32))) : 0.f;
+        atomicAdd(&sh.bin[(most - key[i]) >> shift], MASS ? static_cast<uint32_t>(rintf(exp2_fast(l - top_l) * kFraction)) : 1u);
+    }
+    __syncthreads();
+    const double unit = MASS ? static_cast<double>(exp2f(top_l)) / kFraction : 1.;
+    const double own = sh.bin[tid] * unit;
+    double incl = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+    }
+    if (lane == 31) sh.scan[warp] = incl;
+    __syncthreads();
+    for (int i = 0; i < warp; ++i) incl += sh.scan[i];
+    if (own > 0.) {
+        if (incl >= target) atomicMin(&sh.first, tid);
+        atomicMax(&sh.last, tid);
+    }
+    __syncthreads();
+    const int bin = sh.first < kSelThreads ? sh.first : sh.last;
+    if (tid == bin) sh.found_at = incl - own;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i)
+        if (tid + i * kSelThreads < n && static_cast<int>((most - key[i]) >> shift) == bin) sh.list[atomicAdd(&sh.n_list, 1)] = key[i];
+    __syncthreads();
+    n = sh.n_list;
+    target -= sh.found_at;
+}
+
 // The whole cluster: the key at which the entries at or above `floor`, taken in
 // descending order, reach `target` in number or, with MASS, the part top_p of
 // their mass.  A histogram of the measure finds the bin of the cut and what lies
@@ -493,14 +554,16 @@ __device__ uint64_t wide_cut(SelShared& sh, const RowWords<T>& w, Chunk ch, int 
     int shift = -1;                                   // < 0: bins of the logarithm of the weight
     double target = static_cast<double>(count);       // with MASS set by the first round
     float top_l = 0.f;                                // log2 of the largest weight in question (shift >= 0)
-    // f(z, its index, log2 of its weight, its bin) for the entries in question
-    const auto each_entry = [&](int lo, int hi, auto f) {
+    // f(z, its index, log2 of its weight, its bin) for the entries in question that
+    // are not outside [z_lo, z_hi]
+    const auto each_entry = [&](int lo, int hi, float z_lo, float z_hi, auto f) {
         const bool bounded = key_lo > 0 || shift >= 0;
         w.template each<2>(lo, hi, tid, kSelThreads, [&](uint4 x, int j0, int u) {
             float v[VEC];
             unpack<T>(x, v);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
+                if (v[i] < z_lo || v[i] > z_hi) continue;
                 if (u < 0 && static_cast<unsigned>(j0 + i) >= static_cast<unsigned>(w.V)) continue;
                 const float l = weigh.log2_of(v[i]);
                 int bin = static_cast<int>(fminf(l * -64.f, kBins - 1.f));
@@ -526,7 +589,8 @@ __device__ uint64_t wide_cut(SelShared& sh, const RowWords<T>& w, Chunk ch, int 
         }
         __syncthreads();
         for (int a = ch.lo; a < ch.hi; a += kDrain / VEC) {
-            each_entry(a, a + kDrain / VEC < ch.hi ? a + kDrain / VEC : ch.hi, [&](float, int, float l, int bin) {
+            each_entry(a, a + kDrain / VEC < ch.hi ? a + kDrain / VEC : ch.hi, -INFINITY, INFINITY,
+                       [&](float, int, float l, int bin) {
                 const float up = shift < 0 ? static_cast<float>(bin) * (1.f / 64.f) : -top_l;
                 atomicAdd(&sh.bin[bin], MASS ? static_cast<uint32_t>(rintf(exp2_fast(l + up) * kFraction)) : 1u);
             });
@@ -601,10 +665,20 @@ __device__ uint64_t wide_cut(SelShared& sh, const RowWords<T>& w, Chunk ch, int 
         tell(sh, P, p, sh.found[0], __double_as_longlong(target), __double_as_longlong(sh.found_at), 0);
         const int cut_bin = static_cast<int>(sh.told[0]);
         target = __longlong_as_double(sh.told[1]) - __longlong_as_double(sh.told[2]);   // left to reach inside the bin
-        // its entries to rank 0
+        // its entries to rank 0; most others are ruled out by a look at their value
+        // (the bin's, wide enough for the rounding of the logarithm)
+        float z_lo = -INFINITY, z_hi = INFINITY;
+        if (shift < 0) {
+            const float d = 1.f / (64.f * weigh.c), mid = static_cast<float>(cut_bin) * d, slack = 1e-4f * mid + 0.1f * d;
+            z_hi = weigh.m - mid + slack;
+            if (cut_bin < kBins - 1) z_lo = weigh.m - mid - d - slack;
+            const float ulp = fabsf(weigh.m) * 1e-6f;
+            z_hi += ulp;
+            z_lo -= ulp;
+        }
         SelShared* to = cl.map_shared_rank(&sh, 0);
         unsigned long long least = ~0ull, most = 0ull;
-        each_entry(ch.lo, ch.hi, [&](float z, int j, float, int bin) {
+        each_entry(ch.lo, ch.hi, z_lo, z_hi, [&](float z, int j, float, int bin) {
             if (bin != cut_bin) return;
             const unsigned long long key = entry_key(z, j);
             least = key < least ? key : least;
@@ -620,8 +694,9 @@ __device__ uint64_t wide_cut(SelShared& sh, const RowWords<T>& w, Chunk ch, int 
         }
         cl.sync();
         if (p == 0) {
-            const int n = sh.n_list;
+            int n = sh.n_list;
             if (n <= kSelList) {
+                if (n > 64) narrow_list<MASS>(sh, n, weigh, target);
                 sort_list(sh, n);
                 constexpr int MOST = kSelList / kSelThreads;
                 const int per = (n + kSelThreads - 1) / kSelThreads;
@@ -713,7 +788,7 @@ __device__ void sample_wide(SelShared& sh, const SampleArgs& a, const RowWords<T
     const float fz = floor ? unordered(static_cast<uint32_t>(floor >> 32)) : -INFINITY;
     const int fj = floor ? key_index(floor) : w.V;
     unsigned long long best = 0ull;
-    float kept = 0.f;
+    float kept = 0.f, lead = -1.f;   // lead: the score in `best`
     w.template each<2>(ch.lo, ch.hi, tid, kSelThreads, [&](uint4 x, int j0, int u) {
         float v[VEC], e[VEC];
         unpack<T>(x, v);
@@ -723,15 +798,19 @@ __device__ void sample_wide(SelShared& sh, const SampleArgs& a, const RowWords<T
             e[i] = weigh(v[i]);
             if (!(v[i] > fz || (v[i] == fz && j0 + i <= fj)) || !(e[i] >= q.min_p)) e[i] = 0.f;
         }
-        float number[VEC];
+        float number[VEC], of_word = -1.f;
         load_noise<VEC>(noise, j0, w.V, u >= 0, number);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            if (!(e[i] > 0.f)) continue;
             kept += e[i];
-            const float score = __fdividef(e[i], number[i]);
-            const unsigned long long key = race_key(score, j0 + i);
-            if (score >= 0.f && key > best) best = key;
+            e[i] = e[i] > 0.f ? __fdividef(e[i], number[i]) : -1.f;
+            of_word = fmaxf(of_word, e[i]);
+        }
+        if (of_word >= lead && of_word >= 0.f) {   // seldom; equal scores go by the index
+            lead = of_word;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+                if (e[i] >= 0.f && race_key(e[i], j0 + i) > best) best = race_key(e[i], j0 + i);
         }
     });
     best = block_reduce(best, MaxOp(), 0ull, sh.red64);
@@ -978,12 +1057,16 @@ __global__ void __launch_bounds__(kSelThreads, 4) sample_kernel(SampleArgs a) {
 }
 
 // CTAs per row: while the launch has room on the GPU (four CTAs an SM) and each
-// CTA at least a word a thread.
-static int log_ctas_per_row(const DwaLogitsDims& d) {
-    const int64_t room = 4 * static_cast<int64_t>(tc::sm_count());
+// CTA at least a word a thread.  Sampling, whose rows may take several passes,
+// goes on to eight an SM while a CTA has more than 16 words a thread (the mixed
+// batch of 256 x 131072: 130 us with two CTAs a row, 96 us with four).
+static int log_ctas_per_row(const DwaLogitsDims& d, bool sampling) {
+    const int64_t sms = tc::sm_count();
     const int words = d.V / (16 / static_cast<int>(dtype_bytes(d.dtype)));
-    int l = 3;
-    while (l > 0 && (d.rows << l > room || words < kSelThreads << l)) --l;
+    int l = 0;
+    while (l < 3 && words >= kSelThreads << (l + 1) &&
+           (d.rows << (l + 1) <= 4 * sms || (sampling && words >> l > 16 * kSelThreads && d.rows << (l + 1) <= 8 * sms)))
+        ++l;
     return l;
 }
 
@@ -1010,7 +1093,7 @@ extern "C" int dwa_top_logits(void* stream, const DwaLogitsDims* dims, const voi
     if (reinterpret_cast<uintptr_t>(logits) % dtype_bytes(dims->dtype) ||
         reinterpret_cast<uintptr_t>(values) % dtype_bytes(dims->dtype))
         return fail(DWA_ERR_INVALID_ARG, "top_logits: a pointer is not aligned to its element");
-    const int log_P = log_ctas_per_row(*dims);
+    const int log_P = log_ctas_per_row(*dims, false);
     const TopArgs a = {logits, *dims, K, 1 << log_P, log_P, kLog2e / temperature, temperature, values, indices, lse};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dims->dtype == DWA_BF16) DWA_TIMED("top_logits", st, (launch_rows(top_logits_kernel<__nv_bfloat16>, a, st)));
@@ -1032,7 +1115,7 @@ extern "C" int dwa_sample_tokens(void* stream, const DwaLogitsDims* dims, const 
         return fail(DWA_ERR_INVALID_ARG, "sample_tokens: a required pointer is NULL");
     if (reinterpret_cast<uintptr_t>(logits) % dtype_bytes(dims->dtype) || reinterpret_cast<uintptr_t>(noise) % 4)
         return fail(DWA_ERR_INVALID_ARG, "sample_tokens: a pointer is not aligned to its element");
-    const int log_P = log_ctas_per_row(*dims);
+    const int log_P = log_ctas_per_row(*dims, true);
     const SampleArgs a = {logits, *dims, noise, noise_stride, *params, 1 << log_P, log_P, tokens, logprobs};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dims->dtype == DWA_BF16) DWA_TIMED("sample", st, (launch_rows(sample_kernel<__nv_bfloat16>, a, st)));
