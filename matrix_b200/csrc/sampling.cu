@@ -31,6 +31,7 @@ constexpr int kTryTop = 256;                  // entries sorted first when only 
 constexpr int kSelMaxCluster = 8;
 constexpr int kBins = 2048;                   // bins of a wide cut: 32 octaves of weight, 64 bins each, at first
 constexpr float kFraction = 131072.f;         // 2^17: a weight is counted in parts of its bin's largest
+constexpr float kRound = 12582912.f;          // 1.5 2^23: adding it rounds to a whole number in the low bits
 constexpr int kDrain = 16384;                 // entries after which the 32-bit bins are emptied: 2^14 * 2^17
 
 // A logit as an unsigned integer of the same order.
@@ -43,6 +44,13 @@ __device__ __forceinline__ uint64_t entry_key(float z, int j) {
     return static_cast<uint64_t>(ordered(z)) << 32 | (0xffffffffu - static_cast<uint32_t>(j));
 }
 __device__ __forceinline__ int key_index(uint64_t key) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(key)); }
+
+// e / x, for x below 2^-126 or above 2^126 as for 0 or infinity.
+__device__ __forceinline__ float over(float e, float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return e * r;
+}
 
 // An entry's weight.  1 / T in two floats: the rounding of one would move all
 // weights far below the largest the same way, and with them a nucleus' edge.
@@ -59,6 +67,11 @@ struct Weigh {
         return fmaf(d, c, d * c_lo);
     }
     __device__ __forceinline__ float operator()(float z) const { return exp2_fast(log2_of(z)); }
+    // the same where the maximum is finite
+    __device__ __forceinline__ float log2_below(float z) const {
+        const float d = fmaxf(z - m, -3.4e38f);
+        return fmaf(d, c, d * c_lo);
+    }
 };
 
 // The `target`-th largest key of a row by one block, eight bits of the key a
@@ -376,7 +389,7 @@ struct TopArgs {
 };
 
 template <class T>
-__global__ void __launch_bounds__(kSelThreads, 4) top_logits_kernel(TopArgs a) {
+__global__ void __launch_bounds__(kSelThreads, 4) top_logits_kernel(const __grid_constant__ TopArgs a) {
     __shared__ SelShared sh;
     const int P = a.P, tid = threadIdx.x;
     if (P > 1) cluster_arrive_relaxed();
@@ -491,8 +504,7 @@ __device__ void narrow_list(SelShared& sh, int& n, const Weigh& weigh, double& t
     }
     least = ~block_reduce(~least, MaxOp(), 0ull, sh.red64);
     most = block_reduce(most, MaxOp(), 0ull, sh.red64);
-    int shift = 0;
-    while ((most - least) >> shift >= kSelThreads) ++shift;
+    const int shift = max(0, 56 - __clzll(most - least | 1));   // (most - least) >> shift < 256
     const float top_l = MASS ? weigh.log2_of(unordered(static_cast<uint32_t>(most >> 32))) : 0.f;
     sh.bin[tid] = 0u;
     if (tid == 0) {
@@ -554,6 +566,9 @@ __device__ uint64_t wide_cut(SelShared& sh, const RowWords<T>& w, Chunk ch, int 
     int shift = -1;                                   // < 0: bins of the logarithm of the weight
     double target = static_cast<double>(count);       // with MASS set by the first round
     float top_l = 0.f;                                // log2 of the largest weight in question (shift >= 0)
+    const auto bin_of = [](float l) {   // of the logarithm of the weight
+        return __float_as_int(fmaf(fmaxf(l, -31.95f), -64.f, kRound)) - __float_as_int(kRound);
+    };
     // f(z, its index, log2 of its weight, its bin) for the entries in question that
     // are not outside [z_lo, z_hi]
     const auto each_entry = [&](int lo, int hi, float z_lo, float z_hi, auto f) {
@@ -566,7 +581,7 @@ __device__ uint64_t wide_cut(SelShared& sh, const RowWords<T>& w, Chunk ch, int 
                 if (v[i] < z_lo || v[i] > z_hi) continue;
                 if (u < 0 && static_cast<unsigned>(j0 + i) >= static_cast<unsigned>(w.V)) continue;
                 const float l = weigh.log2_of(v[i]);
-                int bin = static_cast<int>(fminf(l * -64.f, kBins - 1.f));
+                int bin = bin_of(l);
                 if (bounded) {
                     const uint64_t key = entry_key(v[i], j0 + i);
                     if (key < key_lo || key > key_hi) continue;
@@ -576,6 +591,8 @@ __device__ uint64_t wide_cut(SelShared& sh, const RowWords<T>& w, Chunk ch, int 
             }
         });
     };
+    const bool finite = weigh.m < INFINITY;
+    bool lean = finite && floor == 0;   // every entry, by the logarithm of its weight
     // a bin's measure: of a full part of it, in units of the largest weight
     const auto part_of = [&](int bin) {
         return !MASS ? 1. : static_cast<double>(exp2f(shift < 0 ? static_cast<float>(bin) * (-1.f / 64.f) : top_l)) / kFraction;
@@ -589,11 +606,38 @@ __device__ uint64_t wide_cut(SelShared& sh, const RowWords<T>& w, Chunk ch, int 
         }
         __syncthreads();
         for (int a = ch.lo; a < ch.hi; a += kDrain / VEC) {
-            each_entry(a, a + kDrain / VEC < ch.hi ? a + kDrain / VEC : ch.hi, -INFINITY, INFINITY,
-                       [&](float, int, float l, int bin) {
+            const int b = a + kDrain / VEC < ch.hi ? a + kDrain / VEC : ch.hi;
+            const auto count_in = [&](float l, int bin) {
                 const float up = shift < 0 ? static_cast<float>(bin) * (1.f / 64.f) : -top_l;
                 atomicAdd(&sh.bin[bin], MASS ? static_cast<uint32_t>(rintf(exp2_fast(l + up) * kFraction)) : 1u);
-            });
+            };
+            if (MASS && lean) {   // the whole row: 2^(l + bin / 64) by its series, |l + bin / 64| <= 1/128
+                w.template each_whole<2>(a, b, tid, kSelThreads, [&](uint4 x, int, int) {
+                    float v[VEC];
+                    unpack<T>(x, v);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        const float l = weigh.log2_below(v[i]), t = fmaf(l, -64.f, kRound);
+                        if (l < -31.9f) {
+                            count_in(l, bin_of(l));
+                            continue;
+                        }
+                        const float d = fmaf(t - kRound, 1.f / 64.f, l);
+                        const float parts = fmaf(fmaf(kFraction * 0.240226507f, d, kFraction * 0.693147181f), d, kFraction + kRound);
+                        atomicAdd(&sh.bin[__float_as_int(t) - __float_as_int(kRound)],
+                                  static_cast<uint32_t>(__float_as_int(parts) - __float_as_int(kRound)));
+                    }
+                });
+                w.edges(a, b, tid, [&](uint4 x, int j0) {
+                    float v[VEC];
+                    unpack<T>(x, v);
+                    for (int i = 0; i < VEC; ++i)
+                        if (static_cast<unsigned>(j0 + i) < static_cast<unsigned>(w.V))
+                            count_in(weigh.log2_below(v[i]), bin_of(weigh.log2_below(v[i])));
+                });
+            } else {
+                each_entry(a, b, -INFINITY, INFINITY, [&](float, int, float l, int bin) { count_in(l, bin); });
+            }
             __syncthreads();
             for (int i = tid; i < kBins; i += kSelThreads) {
                 sh.sum[i] += sh.bin[i];
@@ -669,23 +713,42 @@ __device__ uint64_t wide_cut(SelShared& sh, const RowWords<T>& w, Chunk ch, int 
         // (the bin's, wide enough for the rounding of the logarithm)
         float z_lo = -INFINITY, z_hi = INFINITY;
         if (shift < 0) {
-            const float d = 1.f / (64.f * weigh.c), mid = static_cast<float>(cut_bin) * d, slack = 1e-4f * mid + 0.1f * d;
+            const float d = 1.f / (64.f * weigh.c), mid = static_cast<float>(cut_bin) * d;
+            const float slack = 0.6f * d + 1e-4f * mid + fabsf(weigh.m) * 1e-6f;
             z_hi = weigh.m - mid + slack;
-            if (cut_bin < kBins - 1) z_lo = weigh.m - mid - d - slack;
-            const float ulp = fabsf(weigh.m) * 1e-6f;
-            z_hi += ulp;
-            z_lo -= ulp;
+            if (static_cast<float>(cut_bin) < 31.9f * 64.f) z_lo = weigh.m - mid - slack;
         }
         SelShared* to = cl.map_shared_rank(&sh, 0);
         unsigned long long least = ~0ull, most = 0ull;
-        each_entry(ch.lo, ch.hi, z_lo, z_hi, [&](float z, int j, float, int bin) {
+        const auto take = [&](float z, int j, float, int bin) {
             if (bin != cut_bin) return;
             const unsigned long long key = entry_key(z, j);
             least = key < least ? key : least;
             most = key > most ? key : most;
             const int at = atomicAdd(&to->n_list, 1);
             if (at < kSelList) to->list[at] = key;
-        });
+        };
+        if (lean) {
+            const float mid_of = z_lo;   // -inf in the last bin
+            w.template each<4>(ch.lo, ch.hi, tid, kSelThreads, [&](uint4 x, int j0, int u) {
+                float v[VEC];
+                unpack<T>(x, v);
+                uint32_t in = 0u;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) in |= (v[i] >= mid_of && v[i] <= z_hi ? 1u : 0u) << i;
+                while (in) {
+                    const int i = __ffs(in) - 1;
+                    in &= in - 1u;
+                    const int j = j0 + i;
+                    if (u < 0 && static_cast<unsigned>(j) >= static_cast<unsigned>(w.V)) continue;
+                    const float z = Elem<T>::to_f(w.row[j]);
+                    const float l = weigh.log2_below(z);
+                    take(z, j, l, bin_of(l));
+                }
+            });
+        } else {
+            each_entry(ch.lo, ch.hi, z_lo, z_hi, take);
+        }
         least = ~block_reduce(~least, MaxOp(), 0ull, sh.red64);
         most = block_reduce(most, MaxOp(), 0ull, sh.red64);
         if (tid == 0) {
@@ -747,9 +810,9 @@ __device__ uint64_t wide_cut(SelShared& sh, const RowWords<T>& w, Chunk ch, int 
         if (sh.told[1]) return sh.told[0];
         key_lo = sh.told[2];
         key_hi = sh.told[3];
+        lean = false;
         top_l = weigh.log2_of(unordered(static_cast<uint32_t>(key_hi >> 32)));
-        shift = 0;
-        while ((key_hi - key_lo) >> shift >= kBins) ++shift;
+        shift = max(0, 53 - __clzll(key_hi - key_lo | 1));   // (key_hi - key_lo) >> shift < kBins = 2^11
     }
 }
 
@@ -787,23 +850,26 @@ __device__ void sample_wide(SelShared& sh, const SampleArgs& a, const RowWords<T
     if (q.top_p < 1.f) floor = wide_cut<T, true>(sh, w, ch, p, P, weigh, floor, 0, q.top_p);
     const float fz = floor ? unordered(static_cast<uint32_t>(floor >> 32)) : -INFINITY;
     const int fj = floor ? key_index(floor) : w.V;
+    const bool finite = m < INFINITY;
     unsigned long long best = 0ull;
     float kept = 0.f, lead = -1.f;   // lead: the score in `best`
     w.template each<2>(ch.lo, ch.hi, tid, kSelThreads, [&](uint4 x, int j0, int u) {
         float v[VEC], e[VEC];
         unpack<T>(x, v);
-        if (!(word_max<T>(x) >= fz)) return;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            e[i] = weigh(v[i]);
-            if (!(v[i] > fz || (v[i] == fz && j0 + i <= fj)) || !(e[i] >= q.min_p)) e[i] = 0.f;
-        }
+        const float top = word_max<T>(x);
+        if (!(top >= fz)) return;
         float number[VEC], of_word = -1.f;
         load_noise<VEC>(noise, j0, w.V, u >= 0, number);
+        const int upto = fj - j0;   // equal entries take part up to here
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            e[i] = exp2_fast(finite ? weigh.log2_below(v[i]) : weigh.log2_of(v[i]));
+            if (!(v[i] > fz || (v[i] == fz && i <= upto)) || !(e[i] >= q.min_p)) e[i] = 0.f;
+        }
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             kept += e[i];
-            e[i] = e[i] > 0.f ? __fdividef(e[i], number[i]) : -1.f;
+            e[i] = e[i] > 0.f ? over(e[i], number[i]) : -1.f;
             of_word = fmaxf(of_word, e[i]);
         }
         if (of_word >= lead && of_word >= 0.f) {   // seldom; equal scores go by the index
@@ -946,7 +1012,7 @@ __device__ __forceinline__ void race_chunk(const RowWords<T>& w, Chunk ch, float
         float lead = -1.f;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            score[i] = e[i] > 0.f ? __fdividef(e[i], number[i]) : -1.f;   // e > 0 only inside the row
+            score[i] = e[i] > 0.f ? over(e[i], number[i]) : -1.f;   // e > 0 only inside the row
             lead = fmaxf(lead, score[i]);
         }
         if (lead > best || best_j < 0) {
@@ -961,7 +1027,7 @@ __device__ __forceinline__ void race_chunk(const RowWords<T>& w, Chunk ch, float
 }
 
 template <class T>
-__global__ void __launch_bounds__(kSelThreads, 4) sample_kernel(SampleArgs a) {
+__global__ void __launch_bounds__(kSelThreads, 4) sample_kernel(const __grid_constant__ SampleArgs a) {
     namespace cg = cooperative_groups;
     __shared__ SelShared sh;
     const int P = a.P, tid = threadIdx.x;
