@@ -204,10 +204,32 @@ __device__ __forceinline__ void push_groups(SelShared& sh, int p, int P, float (
     float all = edge;
 #pragma unroll
     for (int u = 0; u < 8; ++u) all = max_nan(all, top[u]);
-    // NaN above everything, as in the keys
-    const uint32_t first = block_reduce(ordered(all), MaxOp(), 0u, reinterpret_cast<uint32_t*>(sh.redf));
-    const Ref ref(block_reduce(ms.ref.m, MaxOp(), -INFINITY, sh.redf), c);
-    const float S = block_reduce(ms.at(ref, c), AddOp(), 0.f, sh.redf);
+    // the warps' maxima (NaN above everything, as in the keys) and sums, then the CTA's
+    const int lane = tid & 31, warp = tid >> 5;
+    const uint32_t of_warp = __reduce_max_sync(0xffffffffu, ordered(all));
+    const Ref ref_w(warp_max(ms.ref.m), c);
+    const float s_w = warp_sum(ms.at(ref_w, c));
+    if (lane == 0) {
+        sh.warp_count[0][warp] = of_warp;
+        sh.redf[warp] = ref_w.m;
+        sh.redf[16 + warp] = s_w;
+    }
+    __syncthreads();
+    uint32_t first = 0u;
+    Ref ref;
+    float S = 0.f;
+    if (tid == 0) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kSelThreads / 32; ++i) {
+            first = max(first, sh.warp_count[0][i]);
+            m = fmaxf(m, sh.redf[i]);
+        }
+        ref = Ref(m, c);
+#pragma unroll
+        for (int i = 0; i < kSelThreads / 32; ++i)
+            S += sh.redf[i] > -INFINITY ? sh.redf[16 + i] * Ref(sh.redf[i], c).rescale(ref, c) : sh.redf[16 + i];
+    }
     if (P > 1) cluster_wait();   // every CTA of the cluster has started
     SelShared* to = P > 1 ? cl.map_shared_rank(&sh, 0) : &sh;
 #pragma unroll
@@ -237,28 +259,69 @@ __device__ __forceinline__ void row_stats(const SelShared& sh, int P, float c, f
     for (int p = 0; p < P; ++p) s += sh.part_m[p] > -INFINITY ? sh.part_s[p] * Ref(sh.part_m[p], c).rescale(ref, c) : 0.f;
 }
 
+__device__ __forceinline__ unsigned long long larger(unsigned long long a, unsigned long long b, bool of_two) {
+    return (a > b) == of_two ? a : b;
+}
+
+// A warp's 64 keys, a at place `lane` and b at lane + 32, into descending order.
+__device__ __forceinline__ void sort_warp(unsigned long long& a, unsigned long long& b) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1) {
+#pragma unroll
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            const bool lower = (lane & j) == 0, down_a = (lane & k) == 0, down_b = ((lane + 32) & k) == 0;
+            a = larger(a, __shfl_xor_sync(0xffffffffu, a, j), lower == down_a);
+            b = larger(b, __shfl_xor_sync(0xffffffffu, b, j), lower == down_b);
+        }
+    }
+    const unsigned long long c = a;
+    a = larger(a, b, true);
+    b = larger(c, b, false);
+#pragma unroll
+    for (int j = 16; j > 0; j >>= 1) {
+        const bool lower = (lane & j) == 0;
+        a = larger(a, __shfl_xor_sync(0xffffffffu, a, j), lower);
+        b = larger(b, __shfl_xor_sync(0xffffffffu, b, j), lower);
+    }
+}
+
 // The first n <= kSelList keys of sh.list into descending order.
 __device__ void sort_list(SelShared& sh, int n) {
-    const int tid = threadIdx.x;
-    if (n <= 2 * kSelThreads) {   // each key to its rank
-        const bool two = n > kSelThreads;
-        const unsigned long long a = tid < n ? sh.list[tid] : 0ull, b = tid + kSelThreads < n ? sh.list[tid + kSelThreads] : 0ull;
-        int ra = 0, rb = 0;
-        if (two) {
-#pragma unroll 4
-            for (int i = 0; i < n; ++i) {
-                const unsigned long long k = sh.list[i];
-                ra += k > a;
-                rb += k > b;
-            }
-        } else {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (n <= 64) {   // each key to its rank
+        const unsigned long long key = tid < n ? sh.list[tid] : 0ull;
+        int rank = 0;
 #pragma unroll 8
-            for (int i = 0; i < n; ++i) ra += sh.list[i] > a;
+        for (int i = 0; i < n; ++i) rank += sh.list[i] > key;
+        __syncthreads();
+        if (tid < n) sh.list[rank] = key;
+    } else if (n <= 2 * kSelThreads) {   // 64 a warp, then each behind the larger keys of the other warps
+        const int base = 64 * warp;
+        unsigned long long key[2] = {base + lane < n ? sh.list[base + lane] : 0ull,
+                                     base + lane + 32 < n ? sh.list[base + lane + 32] : 0ull};
+        sort_warp(key[0], key[1]);
+        sh.list[base + lane] = key[0];
+        sh.list[base + lane + 32] = key[1];
+        __syncthreads();
+        int at[2] = {lane, lane + 32};
+        const int runs = (n + 63) / 64;
+        for (int r = 0; r < runs; ++r) {
+            if (r == warp) continue;
+            const unsigned long long* run = sh.list + 64 * r;
+            int c[2] = {0, 0};
+#pragma unroll
+            for (int step = 32; step > 0; step >>= 1) {
+                c[0] += run[c[0] + step - 1] > key[0] ? step : 0;
+                c[1] += run[c[1] + step - 1] > key[1] ? step : 0;
+            }
+            at[0] += c[0] + (run[c[0]] > key[0]);
+            at[1] += c[1] + (run[c[1]] > key[1]);
         }
         __syncthreads();
-        if (tid < n) sh.list[ra] = a;
-        if (tid + kSelThreads < n) sh.list[rb] = b;
-    } else {                      // bitonic, padded to a power of two
+        if (key[0]) sh.list[at[0]] = key[0];
+        if (key[1]) sh.list[at[1]] = key[1];
+    } else {   // bitonic, padded to a power of two
         int size = 4 * kSelThreads;
         while (size < n) size <<= 1;
         for (int i = n + tid; i < size; i += kSelThreads) sh.list[i] = 0ull;
@@ -378,6 +441,12 @@ __device__ int collect_top(SelShared& sh, const RowWords<T>& w, int log_P, int K
     return n;
 }
 
+// Rank 0: the K largest entries of the row into sh.list, in descending order.
+template <class T>
+__device__ __forceinline__ void sort_top(SelShared& sh, const RowWords<T>& w, int log_P, int K) {
+    sort_list(sh, collect_top(sh, w, log_P, K));
+}
+
 struct TopArgs {
     const void* z;
     DwaLogitsDims d;
@@ -407,7 +476,7 @@ __global__ void __launch_bounds__(kSelThreads, 4) top_logits_kernel(const __grid
         row_stats(sh, P, a.c, m, s);
         a.lse[r] = m != m || isinf(m) ? m : static_cast<float>(0.6931471805599453 * (Ref(m, a.c).a(a.c) + log2f(s)));
     }
-    sort_list(sh, collect_top(sh, w, a.log_P, a.K));
+    sort_top(sh, w, a.log_P, a.K);
     for (int k = tid; k < a.K; k += kSelThreads) {
         const unsigned long long key = sh.list[k];
         static_cast<T*>(a.values)[static_cast<int64_t>(r) * a.K + k] = Elem<T>::from_f(unordered(static_cast<uint32_t>(key >> 32)));
@@ -487,23 +556,20 @@ __device__ __forceinline__ void tell(SelShared& sh, int P, int p, uint64_t a, ui
 }
 
 // Rank 0: drops from the n entries of sh.list, one of which reaches `target` in
-// number or mass, most that lie above or below it; n and target follow.  256 bins
-// of the keys, counted like the bins of the whole row.
+// number or mass, most that lie above or below it; n and target follow.  All lie in
+// [least, most]; 256 bins of the keys, counted like the bins of the whole row.
 template <bool MASS>
-__device__ void narrow_list(SelShared& sh, int& n, const Weigh& weigh, double& target) {
+__device__ void narrow_list(SelShared& sh, int& n, const Weigh& weigh, double& target, unsigned long long least,
+                            unsigned long long most) {
     constexpr int MOST = kSelList / kSelThreads;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    unsigned long long key[MOST], least = ~0ull, most = 0ull;
+    unsigned long long key[MOST];
 #pragma unroll
     for (int i = 0; i < MOST; ++i) {
         key[i] = 0ull;
         if (tid + i * kSelThreads >= n) continue;
         key[i] = sh.list[tid + i * kSelThreads];
-        least = key[i] < least ? key[i] : least;
-        most = key[i] > most ? key[i] : most;
     }
-    least = ~block_reduce(~least, MaxOp(), 0ull, sh.red64);
-    most = block_reduce(most, MaxOp(), 0ull, sh.red64);
     const int shift = max(0, 56 - __clzll(most - least | 1));   // (most - least) >> shift < 256
     const float top_l = MASS ? weigh.log2_of(unordered(static_cast<uint32_t>(most >> 32))) : 0.f;
     sh.bin[tid] = 0u;
@@ -759,7 +825,12 @@ __device__ uint64_t wide_cut(SelShared& sh, const RowWords<T>& w, Chunk ch, int 
         if (p == 0) {
             int n = sh.n_list;
             if (n <= kSelList) {
-                if (n > 64) narrow_list<MASS>(sh, n, weigh, target);
+                unsigned long long key_least = ~0ull, key_most = 0ull;
+                for (int q = 0; q < P; ++q) {
+                    key_least = sh.part_lo[q] < key_least ? sh.part_lo[q] : key_least;
+                    key_most = sh.part_hi[q] > key_most ? sh.part_hi[q] : key_most;
+                }
+                if (n > 64) narrow_list<MASS>(sh, n, weigh, target, key_least, key_most);
                 sort_list(sh, n);
                 constexpr int MOST = kSelList / kSelThreads;
                 const int per = (n + kSelThreads - 1) / kSelThreads;
@@ -1089,7 +1160,7 @@ __global__ void __launch_bounds__(kSelThreads, 4) sample_kernel(const __grid_con
             row_stats(sh, P, c, m, s);
             if (list) {
                 if (m > -INFINITY) {
-                    sort_list(sh, collect_top(sh, w, a.log_P, q.k));
+                    sort_top(sh, w, a.log_P, q.k);
                     done = sample_listed(sh, a, w, r, q, noise, m, q.k, -1., true);
                 }
             } else if (fabsf(m) < INFINITY && (masses || q.top_p >= 1.f) && limited) {
