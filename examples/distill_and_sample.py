@@ -1,0 +1,126 @@
+"""A student with an assembled layer learns a teacher's next tokens, then writes.
+
+The teacher is a table of next-token logits.  Of each of its rows the training
+loop keeps what a cache of a teacher's answers would hold: the K largest logits,
+their tokens and the row's log-sum-exp (``top_logits``), 6 bytes an entry in
+bfloat16 instead of 2 V bytes a row.  The student is the DWA hot path with a
+vocabulary on both ends:
+
+    embedding -> sequence_mean -> retrieval -> pool rows -> pallas_assemble
+              -> RMSNorm -> output matrix -> logits [B, seq, V]
+
+One step is ``distill_loss_and_grad`` on the logits, whose gradient then enters
+autograd at the logits, so neither the student's probabilities nor the teacher's
+row are ever written.  Afterwards the student continues a prompt with
+``sample_tokens``, every sequence with a temperature and a top_p of its own.
+
+    python examples/distill_and_sample.py --steps 60 --vocab 32000
+"""
+
+from __future__ import annotations
+
+import argparse
+import sys
+from pathlib import Path
+
+import torch
+
+sys.path.insert(0, str(Path(__file__).resolve().parent.parent))
+
+from matrix_b200.assembly import compute_key_cache, pallas_assemble      # noqa: E402
+from matrix_b200.config import DWAConfig                                 # noqa: E402
+from matrix_b200.distill import distill_loss_and_grad, top_logits        # noqa: E402
+from matrix_b200.norm import RMSNorm                                     # noqa: E402
+from matrix_b200.retrieval import MultiAspectRetrieval, sequence_mean    # noqa: E402
+from matrix_b200.sampling import sample_tokens                           # noqa: E402
+
+
+class Student(torch.nn.Module):
+    def __init__(self, cfg: DWAConfig, vocab: int, generator: torch.Generator):
+        super().__init__()
+        self.cfg = cfg
+
+        def normal(*shape, scale):
+            return (torch.randn(*shape, generator=generator) * scale).cuda()
+
+        d = cfg.d_A
+        self.retrieval = MultiAspectRetrieval(cfg, generator=generator)
+        self.pool = normal(cfg.N, cfg.D, scale=d ** -0.5)
+        self.keys = compute_key_cache(self.pool, normal(cfg.S, cfg.D, cfg.d_k, scale=cfg.D ** -0.5))
+        self.embed = torch.nn.Parameter(normal(vocab, d, scale=1.0))
+        self.W_base = torch.nn.Parameter(normal(cfg.d_B, d, scale=d ** -0.5))
+        self.b_base = torch.nn.Parameter(torch.zeros(cfg.d_B, device="cuda"))
+        self.gamma = torch.nn.Parameter(torch.tensor(cfg.gamma_init, device="cuda"))
+        self.norm = RMSNorm(cfg.d_B).cuda()
+        self.out = torch.nn.Parameter(normal(vocab, cfg.d_B, scale=cfg.d_B ** -0.5))
+
+    def forward(self, tokens: torch.Tensor) -> torch.Tensor:
+        """``tokens [B, seq]`` -> ``logits [B, seq, V]`` bf16."""
+        cfg = self.cfg
+        h_A = self.embed[tokens.long()]
+        with torch.no_grad():
+            alphas, rows, _ = self.retrieval(sequence_mean(h_A.detach()), self.keys, 5.0, False, want_soft_full=False)
+        h_mid, _ = pallas_assemble(self.pool[rows.long()], alphas, h_A, self.W_base, self.b_base, self.gamma,
+                                   cfg.d_B, cfg.r, cfg.d_A)
+        return self.norm(h_mid).bfloat16() @ self.out.bfloat16().T
+
+
+def run(*, vocab: int = 32000, steps: int = 60, batch: int = 8, seq: int = 64, top: int = 64, new_tokens: int = 16,
+        temperature: float = 2.0, reverse: bool = False, seed: int = 0) -> dict:
+    """Trains and samples; ``{"losses", "tokens", "logprobs", "student", "teacher"}``."""
+    gen = torch.Generator().manual_seed(seed)
+    cfg = DWAConfig(D=2048, N=512, C=16, m=4, d_A=64, d_B=64, r=8, k_max=8, S=2, d_k=32, bf16_pool=False)
+    student = Student(cfg, vocab, gen)
+    u = torch.randn(vocab, 16, generator=gen).cuda()
+    v = torch.randn(vocab, 16, generator=gen).cuda()
+
+    def teacher(tokens):
+        return (u[tokens.long()] @ v.T).bfloat16()
+
+    opt = torch.optim.Adam(student.parameters(), lr=3e-2)
+    corpus = torch.randint(0, vocab, (batch, seq), generator=gen).cuda()
+    values, ids, lse = top_logits(teacher(corpus), top, temperature=temperature)   # the cached teacher
+    weights = torch.full((batch, seq), 1.0 / (batch * seq), device="cuda")         # the loss is their mean
+    losses = []
+    for _ in range(steps):
+        logits = student(corpus)
+        loss, g_logits = distill_loss_and_grad(logits, values, ids, teacher_lse=lse, temperature=temperature,
+                                               reverse=reverse, weights=weights)
+        opt.zero_grad(set_to_none=True)
+        logits.backward(g_logits)
+        opt.step()
+        losses.append(loss.sum())
+
+    heat = torch.linspace(0.5, 1.0, batch, device="cuda")
+    nucleus = torch.linspace(0.5, 0.95, batch, device="cuda")
+    text, logprobs = corpus[:, :1].int(), []
+    with torch.no_grad():
+        for _ in range(new_tokens):
+            last = student(text)[:, -1]                        # [B, V], rows seq * V apart
+            noise = torch.rand(batch, vocab, device="cuda")
+            token, logprob = sample_tokens(last, noise, temperature=heat, top_k=50, top_p=nucleus, min_p=0.02)
+            text = torch.cat([text, token[:, None]], 1)
+            logprobs.append(logprob)
+    return {"losses": torch.stack(losses).cpu(), "tokens": text.cpu(), "logprobs": torch.stack(logprobs, 1).cpu(),
+            "student": student, "teacher": teacher}
+
+
+def main() -> None:
+    ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
+    ap.add_argument("--vocab", type=int, default=32000)
+    ap.add_argument("--steps", type=int, default=60)
+    ap.add_argument("--top", type=int, default=64)
+    ap.add_argument("--temperature", type=float, default=2.0)
+    ap.add_argument("--reverse", action="store_true", help="KL(student | teacher) in place of KL(teacher | student)")
+    a = ap.parse_args()
+    got = run(vocab=a.vocab, steps=a.steps, top=a.top, temperature=a.temperature, reverse=a.reverse)
+    for i in range(0, a.steps, max(1, a.steps // 10)):
+        print(f"step {i:4d}  loss {got['losses'][i]:.4f}")
+    print(f"last       loss {got['losses'][-1]:.4f}")
+    text, lp = got["tokens"], got["logprobs"]
+    for row in range(len(text)):
+        print(f"sequence {row}: {text[row].tolist()}  mean log-probability {lp[row].mean():.3f}")
+
+
+if __name__ == "__main__":
+    main()
