@@ -23,10 +23,12 @@
 // logarithms keep the digits that fp32 would round away.
 //
 // Where the rows fill the GPU, a CTA takes a row and, for the gradient, reads it a
-// second time out of L2 (rows in flight: 148 x 2 x 256 KB at most); else a cluster
-// of CTAs holds the row in shared memory, which puts more SMs on a row.  Measured
-// on a B200, 4096 x 131072 bf16: the loss 192 us (5.6 TB/s), with the gradient 456
-// us (4.7 TB/s of the 2.1 GB that it has to move; 521 us as two kernels, of which
+// second time, backwards: the end is still in shared memory, the rest mostly in L2
+// (rows in flight: 148 x 2 x 256 KB at most).  Read forwards again, two thirds of
+// the second pass came from HBM.  Else a cluster of CTAs holds the row in shared
+// memory, which puts more SMs on a row.  Measured on a B200, 4096 x 131072 bf16:
+// the loss 185 us (5.8 TB/s), with the gradient 413 us (5.2 TB/s of the 2.1 GB that
+// it has to move; 457 us with both passes forwards; 515 us as two kernels, of which
 // the backward runs at 6.5 TB/s); 600 us when clusters of four hold each row,
 // because the CTAs of a cluster wait for the slowest.
 
@@ -40,7 +42,8 @@ extern std::atomic<uint64_t> g_launches_total;
 
 constexpr int kDistillThreads = 256;             // a CTA of the backward
 constexpr int kHoldThreads = 256;                // a CTA of a cluster that holds a row
-constexpr int kRing = 4;                         // stages of two words that a thread of a streaming CTA has in flight
+constexpr int kAhead = 4;                        // stages of two words that a thread of a streaming CTA has in flight
+constexpr int kSmemOfSM = 227 * 1024;
 constexpr int kDistillMaxCluster = 8;
 constexpr int kDistillMaxParts = 64;             // warps that share a row
 constexpr int kHoldPieces = 2;                   // pieces in which a held chunk arrives
@@ -86,6 +89,7 @@ struct DistillArgs {
     double inv_T;
     int P, log_P;  // CTAs per row
     int room;      // words of the largest chunk
+    int ring;      // stages of two words a thread that a streaming CTA keeps
 };
 
 // log((1 + s) / (1 - s)) for |s| <= 1/3, by its series.
@@ -495,40 +499,52 @@ __global__ void __launch_bounds__(kHoldThreads, 3) distill_hold_kernel(const __g
 }
 
 // A thread's `count` words of a row, NT apart, on their way through a ring of its
-// own in shared memory, kRing stages of two words ahead, each pass right behind the
-// one before.  Only the thread that copies a word reads it, so nothing but its own
-// copies is waited for.
+// own in shared memory, in stages of two words: kAhead of them in flight, `room`
+// kept.  The second pass goes backwards, so that it begins with what the first left
+// in the ring, and asks L2 last for what it has not seen for longest.  Only the
+// thread that copies a word reads it, so nothing but its own copies is waited for.
 template <int NT>
 struct WordRing {
-    uint4* const slots;        // 2 kRing of them, NT apart
+    uint4* const slots;        // 2 room of them, NT apart
     const uint4* const src;
-    const int count;
-    int left, next = 0, put = 0, get = 0;
+    const int count, room;
+    int put = 0, get = 0;
 
-    __device__ __forceinline__ WordRing(uint4* slots_, const uint4* src_, int count_, int passes)
-        : slots(slots_), src(src_), count(count_), left(passes) {}
-    __device__ __forceinline__ void issue() {
-        if (next >= count && left > 0) {
-            --left;
-            next = 0;
+    __device__ __forceinline__ WordRing(uint4* slots_, const uint4* src_, int count_, int room_)
+        : slots(slots_), src(src_), count(count_), room(room_) {}
+    __device__ __forceinline__ void issue(int k, int slot) {   // words k and k + 1
+        if (k >= 0 && k < count) {
+            copy_async(slots + slot * 2 * NT, src + k * NT);
+            if (k + 1 < count) copy_async(slots + (slot * 2 + 1) * NT, src + (k + 1) * NT);
         }
-        if (left > 0 && next < count) {
-            copy_async(slots + put * 2 * NT, src + next * NT);
-            if (next + 1 < count) copy_async(slots + (put * 2 + 1) * NT, src + (next + 1) * NT);
-            next += 2;
-        }
-        put = put + 1 == kRing ? 0 : put + 1;
         copy_commit();
     }
+    __device__ __forceinline__ void begin() {
+#pragma unroll 1
+        for (; put < kAhead; ++put) issue(2 * put, put);
+        if (put == room) put = 0;
+    }
     template <class F>
-    __device__ __forceinline__ void pass(F f) {   // f(word, its number) for all of them
+    __device__ __forceinline__ void forth(F f) {   // f(word, its number) for all of them
         for (int k = 0; k < count; k += 2) {
-            copy_wait<kRing - 1>();
+            copy_wait<kAhead - 1>();
             const uint4* x = slots + get * 2 * NT;
             f(x[0], k);
             if (k + 1 < count) f(x[NT], k + 1);
-            get = get + 1 == kRing ? 0 : get + 1;
-            issue();
+            get = get + 1 == room ? 0 : get + 1;
+            issue(k + 2 * kAhead, put);
+            put = put + 1 == room ? 0 : put + 1;
+        }
+    }
+    template <class F>
+    __device__ __forceinline__ void back(F f) {    // after forth: the same, from the last to the first
+        for (int k = (count - 1) & ~1; k >= 0; k -= 2) {
+            copy_wait<kAhead - 1>();
+            get = get == 0 ? room - 1 : get - 1;
+            const uint4* x = slots + get * 2 * NT;
+            if (k + 1 < count) f(x[NT], k + 1);
+            f(x[0], k);
+            issue(k - 2 * room, get);
         }
     }
 };
@@ -541,7 +557,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_stream_kernel(const __g
     __shared__ DistillShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.d.V;
     const uint32_t r = blockIdx.x;
-    uint32_t* bits = reinterpret_cast<uint32_t*>(data + 2 * kRing * NT);
+    uint32_t* bits = reinterpret_cast<uint32_t*>(data + 2 * a.ring * NT);
     if (tid == 0) sh.own_bad = 0;
     pdl_enter();
     Listed<NT> l;
@@ -551,9 +567,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_stream_kernel(const __g
     int from, to;
     w.own_whole(0, w.words, tid, NT, from, to);
     const int count = max(to - from, 0), w0 = tid + from * NT;   // words w0, w0 + NT, ... of the row
-    WordRing<NT> ring(data + tid, reinterpret_cast<const uint4*>(w.row + w.first(w0)), count, GRAD ? 2 : 1);
-#pragma unroll 1
-    for (int i = 0; i < kRing; ++i) ring.issue();
+    WordRing<NT> ring(data + tid, reinterpret_cast<const uint4*>(w.row + w.first(w0)), count, a.ring);
+    ring.begin();
     for (int i = tid; i < (w.words * VEC + 127) / 128; i += NT) reinterpret_cast<uint4*>(bits)[i] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
     RowState s = {};
@@ -563,7 +578,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_stream_kernel(const __g
     __syncthreads();
     MaxSum ms;
     w.edges(0, w.words, tid, [&](uint4 x, int j0) { ms.add_slow<T>(x, listed_in<T>(bits, (j0 + w.shift) / VEC), a.c); });
-    ring.pass([&](uint4 x, int k) { add_word<T>(ms, x, listed_in<T>(bits, w0 + k * NT), a.c); });
+    ring.forth([&](uint4 x, int k) { add_word<T>(ms, x, listed_in<T>(bits, w0 + k * NT), a.c); });
     Ref ref;
     float S_u;
     double S_l, L;
@@ -585,9 +600,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_stream_kernel(const __g
         const GradWriter<T> write(w, g, s, a, scale);
         if (write.fast) {
             uint4* const to_g = reinterpret_cast<uint4*>(g + w.first(w0));
-            ring.pass([&](uint4 x, int k) { write.whole(x, to_g + k * NT); });
+            ring.back([&](uint4 x, int k) { write.whole(x, to_g + k * NT); });
         } else {
-            ring.pass([&](uint4 x, int k) { write(x, w.first(w0 + k * NT)); });
+            ring.back([&](uint4 x, int k) { write(x, w.first(w0 + k * NT)); });
         }
         w.edges(0, w.words, tid, write);
         if (s.kind != kRowPlain) return;
@@ -720,7 +735,13 @@ template <class T, bool GRAD, int NT>
 static int launch_stream(cudaStream_t st, DistillArgs a) {
     constexpr int VEC = kRowVec<T>;
     a.room = (a.d.V + 2 * VEC - 2) / VEC;
-    const size_t sh = static_cast<size_t>(2 * kRing * NT) * 16 + (static_cast<size_t>(a.room) * VEC + 127) / 128 * 16;
+    const int stage = 2 * NT * 16, bits = (a.room * VEC + 127) / 128 * 16;
+    a.ring = kAhead;
+    if (GRAD) {   // what the first pass leaves there, the second need not fetch
+        const int fits = (kSmemOfSM / (1024 / NT) - 1024 - static_cast<int>(sizeof(DistillShared)) - bits) / stage;
+        a.ring = max(kAhead, min(fits, (a.room + 2 * NT - 1) / (2 * NT)));
+    }
+    const size_t sh = static_cast<size_t>(a.ring) * stage + bits;
     if (int rc = allow_smem<distill_stream_kernel<T, GRAD, NT>>(sh)) return rc;
     DWA_TIMED("distill_fwd", st,
               (launch_pdl(distill_stream_kernel<T, GRAD, NT>, dim3(static_cast<unsigned>(a.d.rows)), dim3(NT), sh, st, a)));
@@ -735,7 +756,7 @@ static int launch_fwd(cudaStream_t st, const DistillArgs& a) {
     if (a.d.rows < 2 * tc::sm_count()) return launch_hold<T, GRAD>(st, a);
     // four CTAs of 256 threads an SM hide a row's serial steps better (8192 x 32768
     // with the gradient: 240 us, 327 us with two of 512) as long as their rows stay
-    // in L2 between the passes (4096 x 131072: 492 and 456 us)
+    // in L2 between the passes (4096 x 131072: 462 and 413 us)
     if constexpr (GRAD)
         if (static_cast<int64_t>(a.d.V) * sizeof(T) > 128 * 1024) return launch_stream<T, GRAD, 512>(st, a);
     return launch_stream<T, GRAD, 256>(st, a);
@@ -762,7 +783,7 @@ extern "C" int dwa_distill_fwd(void* stream, const DwaLogitsDims* dims, const Dw
     if ((rc = check_workspace(workspace, workspace_bytes))) return rc;
     const DistillArgs a = {logits, *dims, *opts, teacher_logits, teacher_indices, teacher_lse, weights, loss,
                            reinterpret_cast<RowState*>(state), nullptr, 0, g_logits, static_cast<uint32_t*>(workspace),
-                           kLog2e / opts->temperature, 1. / opts->temperature, 1, 0, 0};
+                           kLog2e / opts->temperature, 1. / opts->temperature, 1, 0, 0, 0};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dims->dtype == DWA_BF16)
         return g_logits ? launch_fwd<__nv_bfloat16, true>(st, a) : launch_fwd<__nv_bfloat16, false>(st, a);
@@ -784,7 +805,7 @@ extern "C" int dwa_distill_bwd(void* stream, const DwaLogitsDims* dims, const Dw
     const int log_P = log_ctas_per_row(*dims);
     const DistillArgs a = {logits, *dims, *opts, teacher_logits, teacher_indices, teacher_lse, weights, nullptr,
                            reinterpret_cast<RowState*>(const_cast<float*>(state)), g_loss, g_loss_stride, g_logits, nullptr,
-                           kLog2e / opts->temperature, 1. / opts->temperature, 1 << log_P, log_P, 0};
+                           kLog2e / opts->temperature, 1. / opts->temperature, 1 << log_P, log_P, 0, 0};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const size_t sh = static_cast<size_t>(opts->K) * 4;
     const dim3 grid(static_cast<unsigned>(dims->rows << log_P));
