@@ -215,11 +215,11 @@ struct Listed {
             }
         }
     }
-    // Notes the entries of the chunk in `bits`; the teacher's probabilities; t_hi and
-    // t_lo of the state.
-    template <class T>
+    // Notes the entries of the chunk in `bits`, entry b in bit bit_of(b); the
+    // teacher's probabilities; t_hi and t_lo of the state.
+    template <class T, class F>
     __device__ __forceinline__ void place(DistillShared& sh, RowState& s, const DistillArgs& a, const RowWords<T>& w,
-                                          Chunk ch, uint32_t* bits, float t_lse) {
+                                          Chunk ch, uint32_t* bits, F bit_of, float t_lse) {
         constexpr int VEC = kRowVec<T>;
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, V = w.V, n = ch.hi - ch.lo;
         int mine = 0;
@@ -239,7 +239,8 @@ struct Listed {
             const int b = j[i] + w.shift - ch.lo * VEC;
             if (b >= 0 && b < n * VEC) {
                 at[i] = b;
-                if (atomicOr(&bits[b >> 5], 1u << (b & 31)) & (1u << (b & 31))) sh.own_bad = 1;
+                const int q = bit_of(b);
+                if (atomicOr(&bits[q >> 5], 1u << (q & 31)) & (1u << (q & 31))) sh.own_bad = 1;
             }
             t_top = fmaxf(t_top, t[i]);
         }
@@ -437,7 +438,7 @@ __global__ void __launch_bounds__(kHoldThreads, 3) distill_hold_kernel(const __g
     for (int i = tid; i < (n * VEC + 127) / 128; i += NT) reinterpret_cast<uint4*>(bits)[i] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
     RowState s = {};
-    l.place(sh, s, a, w, ch, bits, t_lse);
+    l.place(sh, s, a, w, ch, bits, [](int b) { return b; }, t_lse);
     __syncthreads();
     // one pass: the sum of the weights of unlisted entries
     MaxSum ms;
@@ -498,54 +499,169 @@ __global__ void __launch_bounds__(kHoldThreads, 3) distill_hold_kernel(const __g
     }
 }
 
+// 16 bytes to shared memory, in the background, if `there`.
+__device__ __forceinline__ void copy_async_if(bool there, uint32_t to, const void* from) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %2, 0;\n@p cp.async.cg.shared.global [%0], [%1], 16;\n}" ::"r"(to), "l"(from),
+                 "r"(static_cast<int>(there))
+                 : "memory");
+}
+__device__ __forceinline__ uint4 shared_word(uint32_t at) {
+    uint4 x;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
+    return x;
+}
+
 // A thread's `count` words of a row, NT apart, on their way through a ring of its
 // own in shared memory, in stages of two words: kAhead of them in flight, `room`
 // kept.  The second pass goes backwards, so that it begins with what the first left
 // in the ring, and asks L2 last for what it has not seen for longest.  Only the
 // thread that copies a word reads it, so nothing but its own copies is waited for.
+// The passes call two(word k, word k + 1, k) for whole stages, one(word, k) for the
+// last word of an odd count.
 template <int NT>
 struct WordRing {
-    uint4* const slots;        // 2 room of them, NT apart
+    static constexpr uint32_t kNext = NT * 16, kStage = 2 * kNext;
     const uint4* const src;
+    const uint32_t base, end;   // own slots
     const int count, room;
-    int put = 0, get = 0;
+    uint32_t at;                // the stage to look at
 
-    __device__ __forceinline__ WordRing(uint4* slots_, const uint4* src_, int count_, int room_)
-        : slots(slots_), src(src_), count(count_), room(room_) {}
-    __device__ __forceinline__ void issue(int k, int slot) {   // words k and k + 1
-        if (k >= 0 && k < count) {
-            copy_async(slots + slot * 2 * NT, src + k * NT);
-            if (k + 1 < count) copy_async(slots + (slot * 2 + 1) * NT, src + (k + 1) * NT);
-        }
+    __device__ __forceinline__ WordRing(const uint4* slots, const uint4* src_, int count_, int room_)
+        : src(src_), base(static_cast<uint32_t>(__cvta_generic_to_shared(slots))), end(base + room_ * kStage), count(count_),
+          room(room_), at(base) {}
+    // words k and k + 1 of those below n
+    __device__ __forceinline__ void issue(uint32_t to, const uint4* from, bool first, bool second) {
+        copy_async_if(first, to, from);
+        copy_async_if(second, to + kNext, from + NT);
         copy_commit();
     }
     __device__ __forceinline__ void begin() {
-#pragma unroll 1
-        for (; put < kAhead; ++put) issue(2 * put, put);
-        if (put == room) put = 0;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) issue(base + i * kStage, src + 2 * i * NT, 2 * i < count, 2 * i + 1 < count);
     }
-    template <class F>
-    __device__ __forceinline__ void forth(F f) {   // f(word, its number) for all of them
-        for (int k = 0; k < count; k += 2) {
+    // the largest value of the first stage, among the warp's
+    template <class T>
+    __device__ __forceinline__ float first_max() const {
+        copy_wait<kAhead - 1>();
+        float m = -INFINITY;
+        if (count > 1) {
+            const uint4 x[2] = {shared_word(base), shared_word(base + kNext)};
+            m = words_max<T, 2>(x);
+        } else if (count == 1) {
+            m = word_max<T>(shared_word(base));
+        }
+        return warp_max(m);
+    }
+    template <class F, class G>
+    __device__ __forceinline__ void forth(F two, G one) {
+        uint32_t to = base + kAhead * kStage;
+        if (to == end) to = base;
+        const uint4* from = src + 2 * kAhead * NT;
+        int left = count - 2 * kAhead;
+        for (int k = 0; k + 1 < count; k += 2) {
             copy_wait<kAhead - 1>();
-            const uint4* x = slots + get * 2 * NT;
-            f(x[0], k);
-            if (k + 1 < count) f(x[NT], k + 1);
-            get = get + 1 == room ? 0 : get + 1;
-            issue(k + 2 * kAhead, put);
-            put = put + 1 == room ? 0 : put + 1;
+            two(shared_word(at), shared_word(at + kNext), k);
+            issue(to, from, left > 0, left > 1);
+            from += 2 * NT;
+            left -= 2;
+            at += kStage;
+            if (at == end) at = base;
+            to += kStage;
+            if (to == end) to = base;
+        }
+        copy_wait<0>();   // nothing but the last word of an odd count
+        if (count & 1) {
+            one(shared_word(at), count - 1);
+            at += kStage;
+            if (at == end) at = base;
         }
     }
-    template <class F>
-    __device__ __forceinline__ void back(F f) {    // after forth: the same, from the last to the first
-        for (int k = (count - 1) & ~1; k >= 0; k -= 2) {
+    template <class F, class G>
+    __device__ __forceinline__ void back(F two, G one) {   // after forth: from the last to the first
+        int left = ((count + 1) >> 1) - room;              // stages to fetch
+        const uint4* from = src + 2 * (left - 1) * static_cast<int64_t>(NT);
+        const auto step = [&](auto f) {
             copy_wait<kAhead - 1>();
-            get = get == 0 ? room - 1 : get - 1;
-            const uint4* x = slots + get * 2 * NT;
-            if (k + 1 < count) f(x[NT], k + 1);
-            f(x[0], k);
-            issue(k - 2 * room, get);
+            if (at == base) at = end;
+            at -= kStage;
+            f();
+            issue(at, from, left > 0, left > 0);
+            from -= 2 * NT;
+            --left;
+        };
+        if (count & 1) step([&] { one(shared_word(at), count - 1); });
+        for (int k = (count & ~1) - 2; k >= 0; k -= 2) step([&] { two(shared_word(at), shared_word(at + kNext), k); });
+    }
+};
+
+// Where a streaming CTA keeps which entries are listed: a thread's stages one after
+// the other, 2 VEC bits each, after one for its part of the edges; an odd number of
+// 32-bit words a thread, so that a warp's lie in different banks.
+template <class T, int NT>
+struct ListedBits {
+    static constexpr int VEC = kRowVec<T>;
+    const uint8_t* own;
+    int per, shifted;   // 32-bit words a thread; whether word 0 is an edge
+    static __host__ __device__ __forceinline__ int words_of_thread(int words) {
+        return (((words + NT - 1) / NT + 2) * VEC + 31) / 32 | 1;
+    }
+    __device__ __forceinline__ ListedBits(const uint32_t* bits, const RowWords<T>& w)
+        : per(words_of_thread(w.words)), shifted(w.full_lo) {
+        own = reinterpret_cast<const uint8_t*>(bits) + threadIdx.x * per * 4;
+    }
+    // the bit of entry b, counted from the first word's start
+    __device__ __forceinline__ int operator()(int b) const {
+        const int g = b / VEC, t = g % NT, k = g / NT - (t == 0 ? shifted : 0);   // -1: the first edge
+        return t * per * 32 + (k + 2) * VEC + b % VEC;
+    }
+    __device__ __forceinline__ uint32_t stage(int k) const {   // words k, k + 1 of this thread
+        return VEC == 8 ? reinterpret_cast<const uint16_t*>(own)[k / 2 + 1] : own[k / 2 + 1];
+    }
+    __device__ __forceinline__ uint32_t word(const uint32_t* bits, int g) const {   // any word
+        const int q = (*this)(g * VEC);
+        return bits[q >> 5] >> (q & 31) & ((1u << VEC) - 1);
+    }
+};
+
+// A sum with one reference throughout.  No word is looked at before it is added: a
+// sum that leaves [0, 2^60] says afterwards that the reference was too low, or that
+// a NaN or an infinity was there.
+template <class T>
+struct BlindSum {
+    Ref ref;
+    uint64_t s2 = 0;
+    __device__ __forceinline__ BlindSum(float m, float c) : ref(m, c) {}
+    // words that hold listed entries, a bit each, leave them out
+    template <int N>
+    __device__ __forceinline__ void add(const uint4 (&x)[N], uint32_t listed, float c) {
+        constexpr int VEC = kRowVec<T>;
+        uint64_t e[N][VEC / 2];
+#pragma unroll
+        for (int i = 0; i < N; ++i) word_weights<T>(x[i], ref, c, e[i]);
+        if (listed != 0u) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                float f[VEC];
+                unpair_word<T>(e[i], f);
+#pragma unroll
+                for (int v = 0; v < VEC; v += 2)
+                    e[i][v / 2] = pair((listed >> (i * VEC + v)) & 1u ? 0.f : f[v], (listed >> (i * VEC + v)) & 2u ? 0.f : f[v + 1]);
+            }
         }
+        uint64_t sum = sum_pairs<T>(e[0]);
+        if constexpr (N == 2) sum = add2(sum, sum_pairs<T>(e[1]));
+        s2 = add2(s2, sum);
+    }
+    // as a MaxSum; false where it does not hold
+    __device__ __forceinline__ bool into(MaxSum& ms, float c) const {
+        float a, b;
+        unpair(s2, a, b);
+        const float sum = a + b;
+        if (!(ref.m > -INFINITY && ref.plain() && sum <= 1.152921504606846976e18f)) return false;
+        ms.raise(ref.m, c);
+        ms.s2 = s2;
+        if (sum > 2097152.f) ms.raise(ref.m + __log2f(sum) / c, c);
+        return true;
     }
 };
 
@@ -567,18 +683,25 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_stream_kernel(const __g
     int from, to;
     w.own_whole(0, w.words, tid, NT, from, to);
     const int count = max(to - from, 0), w0 = tid + from * NT;   // words w0, w0 + NT, ... of the row
-    WordRing<NT> ring(data + tid, reinterpret_cast<const uint4*>(w.row + w.first(w0)), count, a.ring);
+    const uint4* const own_words = reinterpret_cast<const uint4*>(w.row + w.first(w0));
+    WordRing<NT> ring(data + tid, own_words, count, a.ring);
     ring.begin();
-    for (int i = tid; i < (w.words * VEC + 127) / 128; i += NT) reinterpret_cast<uint4*>(bits)[i] = make_uint4(0u, 0u, 0u, 0u);
+    const ListedBits<T, NT> listed(bits, w);
+    for (int i = tid; i < NT / 4 * listed.per; i += NT) reinterpret_cast<uint4*>(bits)[i] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
     RowState s = {};
-    l.place(sh, s, a, w, Chunk(w.words, 0, 0), bits, t_lse);
+    l.place(sh, s, a, w, Chunk(w.words, 0, 0), bits, listed, t_lse);
 #pragma unroll
     for (int i = 0; i < l.MOST; ++i) l.z[i] = l.j[i] >= 0 ? Elem<T>::to_f(w.row[l.j[i]]) : -INFINITY;
     __syncthreads();
     MaxSum ms;
-    w.edges(0, w.words, tid, [&](uint4 x, int j0) { ms.add_slow<T>(x, listed_in<T>(bits, (j0 + w.shift) / VEC), a.c); });
-    ring.forth([&](uint4 x, int k) { add_word<T>(ms, x, listed_in<T>(bits, w0 + k * NT), a.c); });
+    BlindSum<T> sum(ring.template first_max<T>(), a.c);
+    ring.forth([&](uint4 x, uint4 y, int k) { sum.add({x, y}, listed.stage(k), a.c); },
+               [&](uint4 x, int k) { sum.add({x}, listed.stage(k), a.c); });
+    if (!sum.into(ms, a.c))
+#pragma unroll 1
+        for (int k = 0; k < count; ++k) add_word<T>(ms, own_words[k * NT], listed.word(bits, w0 + k * NT), a.c);
+    w.edges(0, w.words, tid, [&](uint4 x, int j0) { ms.add_slow<T>(x, listed.word(bits, (j0 + w.shift) / VEC), a.c); });
     Ref ref;
     float S_u;
     double S_l, L;
@@ -600,9 +723,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_stream_kernel(const __g
         const GradWriter<T> write(w, g, s, a, scale);
         if (write.fast) {
             uint4* const to_g = reinterpret_cast<uint4*>(g + w.first(w0));
-            ring.back([&](uint4 x, int k) { write.whole(x, to_g + k * NT); });
+            const auto one = [&](uint4 x, int k) { write.whole(x, to_g + k * NT); };
+            ring.back([&](uint4 x, uint4 y, int k) { one(x, k), one(y, k + 1); }, one);
         } else {
-            ring.back([&](uint4 x, int k) { write(x, w.first(w0 + k * NT)); });
+            const auto one = [&](uint4 x, int k) { write(x, w.first(w0 + k * NT)); };
+            ring.back([&](uint4 x, uint4 y, int k) { one(y, k + 1), one(x, k); }, one);
         }
         w.edges(0, w.words, tid, write);
         if (s.kind != kRowPlain) return;
@@ -735,7 +860,7 @@ template <class T, bool GRAD, int NT>
 static int launch_stream(cudaStream_t st, DistillArgs a) {
     constexpr int VEC = kRowVec<T>;
     a.room = (a.d.V + 2 * VEC - 2) / VEC;
-    const int stage = 2 * NT * 16, bits = (a.room * VEC + 127) / 128 * 16;
+    const int stage = 2 * NT * 16, bits = ListedBits<T, NT>::words_of_thread(a.room) * NT * 4;
     a.ring = kAhead;
     if (GRAD) {   // what the first pass leaves there, the second need not fetch
         const int fits = (kSmemOfSM / (1024 / NT) - 1024 - static_cast<int>(sizeof(DistillShared)) - bits) / stage;
