@@ -27,10 +27,11 @@
 // (rows in flight: 148 x 2 x 256 KB at most).  Read forwards again, two thirds of
 // the second pass came from HBM.  Else a cluster of CTAs holds the row in shared
 // memory, which puts more SMs on a row.  Measured on a B200, 4096 x 131072 bf16:
-// the loss 185 us (5.8 TB/s), with the gradient 413 us (5.2 TB/s of the 2.1 GB that
-// it has to move; 457 us with both passes forwards; 515 us as two kernels, of which
-// the backward runs at 6.5 TB/s); 600 us when clusters of four hold each row,
-// because the CTAs of a cluster wait for the slowest.
+// the loss 159 us (6.8 TB/s), with the gradient 375 us (5.7 TB/s of the 2.1 GB that
+// it has to move, and 9% more reads than that; 407 us without hints to L2, 457 us
+// with both passes forwards; 490 us as two kernels, of which the backward runs at
+// 6.5 TB/s); 600 us when clusters of four hold each row, because the CTAs of a
+// cluster wait for the slowest.
 
 #include <atomic>
 
@@ -499,11 +500,29 @@ __global__ void __launch_bounds__(kHoldThreads, 3) distill_hold_kernel(const __g
     }
 }
 
-// 16 bytes to shared memory, in the background, if `there`.
-__device__ __forceinline__ void copy_async_if(bool there, uint32_t to, const void* from) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %2, 0;\n@p cp.async.cg.shared.global [%0], [%1], 16;\n}" ::"r"(to), "l"(from),
-                 "r"(static_cast<int>(there))
-                 : "memory");
+// 16 bytes to shared memory, in the background, if `there`; with HINT L2 keeps them
+// by `policy`.
+template <bool HINT>
+__device__ __forceinline__ void copy_async_if(bool there, uint32_t to, const void* from, uint64_t policy) {
+    if constexpr (HINT)
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.b32 p, %2, 0;\n@p cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %3;\n}" ::"r"(to),
+            "l"(from), "r"(static_cast<int>(there)), "l"(policy)
+            : "memory");
+    else
+        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %2, 0;\n@p cp.async.cg.shared.global [%0], [%1], 16;\n}" ::"r"(to),
+                     "l"(from), "r"(static_cast<int>(there))
+                     : "memory");
+}
+__device__ __forceinline__ uint64_t keep_policy() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ uint64_t drop_policy() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
 }
 __device__ __forceinline__ uint4 shared_word(uint32_t at) {
     uint4 x;
@@ -516,26 +535,29 @@ __device__ __forceinline__ uint4 shared_word(uint32_t at) {
 // kept.  The second pass goes backwards, so that it begins with what the first left
 // in the ring, and asks L2 last for what it has not seen for longest.  Only the
 // thread that copies a word reads it, so nothing but its own copies is waited for.
-// The passes call two(word k, word k + 1, k) for whole stages, one(word, k) for the
-// last word of an odd count.
-template <int NT>
+// With TWICE, L2 is told to keep what the second pass has to fetch from it, and to
+// drop the rest.  The passes call two(word k, word k + 1, k) for whole stages,
+// one(word, k) for the last word of an odd count.
+template <int NT, bool TWICE>
 struct WordRing {
     static constexpr uint32_t kNext = NT * 16, kStage = 2 * kNext;
     const uint4* const src;
     const uint32_t base, end;   // own slots
     const int count, room;
     uint32_t at;                // the stage to look at
+    uint64_t policy = 0;
 
     __device__ __forceinline__ WordRing(const uint4* slots, const uint4* src_, int count_, int room_)
         : src(src_), base(static_cast<uint32_t>(__cvta_generic_to_shared(slots))), end(base + room_ * kStage), count(count_),
           room(room_), at(base) {}
     // words k and k + 1 of those below n
     __device__ __forceinline__ void issue(uint32_t to, const uint4* from, bool first, bool second) {
-        copy_async_if(first, to, from);
-        copy_async_if(second, to + kNext, from + NT);
+        copy_async_if<TWICE>(first, to, from, policy);
+        copy_async_if<TWICE>(second, to + kNext, from + NT, policy);
         copy_commit();
     }
     __device__ __forceinline__ void begin() {
+        if (TWICE) policy = keep_policy();
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) issue(base + i * kStage, src + 2 * i * NT, 2 * i < count, 2 * i + 1 < count);
     }
@@ -558,9 +580,11 @@ struct WordRing {
         if (to == end) to = base;
         const uint4* from = src + 2 * kAhead * NT;
         int left = count - 2 * kAhead;
+        const uint64_t drop = TWICE ? drop_policy() : 0;
         for (int k = 0; k + 1 < count; k += 2) {
             copy_wait<kAhead - 1>();
             two(shared_word(at), shared_word(at + kNext), k);
+            if (TWICE && left <= 2 * room) policy = drop;   // stays in the ring
             issue(to, from, left > 0, left > 1);
             from += 2 * NT;
             left -= 2;
@@ -580,6 +604,7 @@ struct WordRing {
     __device__ __forceinline__ void back(F two, G one) {   // after forth: from the last to the first
         int left = ((count + 1) >> 1) - room;              // stages to fetch
         const uint4* from = src + 2 * (left - 1) * static_cast<int64_t>(NT);
+        if (TWICE) policy = drop_policy();
         const auto step = [&](auto f) {
             copy_wait<kAhead - 1>();
             if (at == base) at = end;
@@ -665,8 +690,9 @@ struct BlindSum {
     }
 };
 
-// Many rows: one CTA per row that, with GRAD, reads it a second time, out of L2.
-template <class T, bool GRAD, int NT>
+// Many rows: one CTA per row that, with GRAD, reads it a second time; FROM_L2 where
+// most of it has left the ring by then.
+template <class T, bool GRAD, int NT, bool FROM_L2>
 __global__ void __launch_bounds__(NT, 1024 / NT) distill_stream_kernel(const __grid_constant__ DistillArgs a) {
     constexpr int WARPS = NT / 32, VEC = kRowVec<T>;
     extern __shared__ __align__(16) uint4 data[];
@@ -684,7 +710,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_stream_kernel(const __g
     w.own_whole(0, w.words, tid, NT, from, to);
     const int count = max(to - from, 0), w0 = tid + from * NT;   // words w0, w0 + NT, ... of the row
     const uint4* const own_words = reinterpret_cast<const uint4*>(w.row + w.first(w0));
-    WordRing<NT> ring(data + tid, own_words, count, a.ring);
+    WordRing<NT, FROM_L2> ring(data + tid, own_words, count, a.ring);
     ring.begin();
     const ListedBits<T, NT> listed(bits, w);
     for (int i = tid; i < NT / 4 * listed.per; i += NT) reinterpret_cast<uint4*>(bits)[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -856,7 +882,7 @@ static int launch_hold(cudaStream_t st, DistillArgs a) {
     return DWA_OK;
 }
 
-template <class T, bool GRAD, int NT>
+template <class T, bool GRAD, int NT, bool FROM_L2>
 static int launch_stream(cudaStream_t st, DistillArgs a) {
     constexpr int VEC = kRowVec<T>;
     a.room = (a.d.V + 2 * VEC - 2) / VEC;
@@ -867,9 +893,9 @@ static int launch_stream(cudaStream_t st, DistillArgs a) {
         a.ring = max(kAhead, min(fits, (a.room + 2 * NT - 1) / (2 * NT)));
     }
     const size_t sh = static_cast<size_t>(a.ring) * stage + bits;
-    if (int rc = allow_smem<distill_stream_kernel<T, GRAD, NT>>(sh)) return rc;
+    if (int rc = allow_smem<distill_stream_kernel<T, GRAD, NT, FROM_L2>>(sh)) return rc;
     DWA_TIMED("distill_fwd", st,
-              (launch_pdl(distill_stream_kernel<T, GRAD, NT>, dim3(static_cast<unsigned>(a.d.rows)), dim3(NT), sh, st, a)));
+              (launch_pdl(distill_stream_kernel<T, GRAD, NT, FROM_L2>, dim3(static_cast<unsigned>(a.d.rows)), dim3(NT), sh, st, a)));
     DWA_LAUNCH_CHECK("distill_stream_kernel");
     ++g_launches_total;
     return DWA_OK;
@@ -879,12 +905,18 @@ template <class T, bool GRAD>
 static int launch_fwd(cudaStream_t st, const DistillArgs& a) {
     // fewer rows than two a SM: 64 x 131072 takes 17.6 us held by clusters, 36 us streamed
     if (a.d.rows < 2 * tc::sm_count()) return launch_hold<T, GRAD>(st, a);
-    // four CTAs of 256 threads an SM hide a row's serial steps better (8192 x 32768
-    // with the gradient: 240 us, 327 us with two of 512) as long as their rows stay
-    // in L2 between the passes (4096 x 131072: 462 and 413 us)
-    if constexpr (GRAD)
-        if (static_cast<int64_t>(a.d.V) * sizeof(T) > 128 * 1024) return launch_stream<T, GRAD, 512>(st, a);
-    return launch_stream<T, GRAD, 256>(st, a);
+    // Four CTAs of 256 threads an SM hide a row's serial steps better than two of 512
+    // (bf16 with the gradient, 8192 x 32768: 210 and 272 us; 3276 x 81920: 196 and 208)
+    // until four rows are too much for L2 to hold between the passes (2684 x 100352:
+    // 209 and 200; 2048 x 131072: 225 and 195).  Hints to L2 pay where less than half
+    // of a row stays in the ring (without and with, 4096 x 65536: 209 and 188; 4000 x
+    // 40000: 125 and 129; fp32, 4000 x 20000: 108 and 120).
+    if constexpr (GRAD) {
+        const int64_t bytes = static_cast<int64_t>(a.d.V) * sizeof(T);
+        if (bytes > 180 * 1024) return launch_stream<T, GRAD, 512, true>(st, a);
+        if (bytes > 96 * 1024) return launch_stream<T, GRAD, 256, true>(st, a);
+    }
+    return launch_stream<T, GRAD, 256, false>(st, a);
 }
 
 }  // namespace dwa
