@@ -29,8 +29,8 @@
 // memory, which puts more SMs on a row.  Measured on a B200, 4096 x 131072 bf16:
 // the loss 159 us (6.8 TB/s), with the gradient 375 us (5.7 TB/s of the 2.1 GB that
 // it has to move, and 9% more reads than that; 407 us without hints to L2, 457 us
-// with both passes forwards; 490 us as two kernels, of which the backward runs at
-// 6.5 TB/s); 600 us when clusters of four hold each row, because the CTAs of a
+// with both passes forwards; 541 us as two kernels, the loss and its backward, of
+// which the backward runs at 6.5 TB/s); 600 us when clusters of four hold each row, because the CTAs of a
 // cluster wait for the slowest.
 
 #include <atomic>
@@ -762,15 +762,17 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_stream_kernel(const __g
     }
 }
 
-// The gradient from a saved state: P CTAs per row, each its words.  g may be the
-// logits' own memory: a listed entry is read before its word is written.
+// The gradient from a saved state: P CTAs per row, each its words.  The last rows
+// come first, for L2 holds them where the loss was taken just before (both
+// directions of 2040 x 50304 bf16: 121 us with the first rows first, 110 so).  g may
+// be the logits' own memory: a listed entry is read before its word is written.
 template <class T>
 __global__ void __launch_bounds__(kDistillThreads) distill_bwd_kernel(const __grid_constant__ DistillArgs a) {
     pdl_enter();
     constexpr int VEC = kRowVec<T>;
     extern __shared__ float zk[];
     const int tid = threadIdx.x, K = a.o.K, V = a.d.V;
-    const uint32_t r = blockIdx.x >> a.log_P;
+    const uint32_t r = (gridDim.x - 1 - blockIdx.x) >> a.log_P;
     const RowWords<T> w(static_cast<const T*>(a.z) + row_offset(a.d, r), V);
     const Chunk ch(w.words, blockIdx.x & (a.P - 1), a.log_P);
     const int32_t* idx = a.idx + static_cast<int64_t>(r) * K;
