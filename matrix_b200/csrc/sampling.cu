@@ -27,6 +27,7 @@ extern std::atomic<uint64_t> g_launches_total;
 constexpr int kSelThreads = 256;
 constexpr int kSelGroups = 8 * kSelThreads;   // groups of words whose maxima are compared
 constexpr int kSelList = 2048;                // candidates held
+constexpr int kTopRing = 3;                   // stages of two words that a thread of top_logits has in flight
 constexpr int kTryTop = 256;                  // entries sorted first when only a mass or a floor limits the row
 constexpr int kSelMaxCluster = 8;
 constexpr int kBins = 2048;                   // bins of a wide cut: 32 octaves of weight, 64 bins each, at first
@@ -166,6 +167,28 @@ struct SelShared {
     int n_chosen, n_list, first, last;
 };
 
+// The largest entry of some words (NaN if one is there); of bf16 in two lanes.
+template <class T>
+struct WordTop {
+    std::conditional_t<sizeof(T) == 2, __nv_bfloat162, float> m;
+    __device__ __forceinline__ WordTop() {
+        if constexpr (sizeof(T) == 2) m = __nv_bfloat162{__ushort_as_bfloat16(0xff80), __ushort_as_bfloat16(0xff80)};
+        else m = -INFINITY;
+    }
+    __device__ __forceinline__ void add(uint4 x) {
+        if constexpr (sizeof(T) == 2) {
+            const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&x);
+            m = __hmax2_nan(__hmax2_nan(m, __hmax2_nan(h[0], h[1])), __hmax2_nan(h[2], h[3]));
+        } else {
+            m = max_nan(m, word_max<T>(x));
+        }
+    }
+    __device__ __forceinline__ float value() const {
+        if constexpr (sizeof(T) == 2) return max_nan(__low2float(m), __high2float(m));
+        else return m;
+    }
+};
+
 // This CTA's share: the maxima of the thread's words by position mod 8 (`edge`:
 // of a row's first and last word where they are not whole) and, with SUM, the
 // running maximum and sum of exp((z - m) / T).
@@ -183,6 +206,39 @@ __device__ __forceinline__ void scan_chunk(const RowWords<T>& w, Chunk ch, float
             if (ms.covers(m)) ms.add_words<T, 1>(&x, c);
             else ms.add_slow<T>(x, 0u, c);
         }
+    });
+}
+
+// The same for long chunks, whose words stream through shared memory.
+template <class T>
+__device__ __forceinline__ void stream_chunk(const RowWords<T>& w, Chunk ch, float c, uint4* slots, float (&top)[8],
+                                             float& edge, MaxSum& ms) {
+    int first, last;
+    w.own_whole(ch.lo, ch.hi, threadIdx.x, kSelThreads, first, last);
+    const int count = max(last - first, 0);
+    const uint4* const own = reinterpret_cast<const uint4*>(w.row + w.first(ch.lo + threadIdx.x + first * kSelThreads));
+    WordRing<kSelThreads, kTopRing, false> ring(slots + threadIdx.x, own, count, kTopRing);
+    ring.begin();
+    WordTop<T> tops[8];
+    BlindSum<T> sum(ring.template first_max<T>(), c);
+    ring.template forth_by_eight<T>([&](uint4 x, uint4 y, int u) {
+        tops[u].add(x);
+        tops[u + 1].add(y);
+        sum.add({x, y}, 0u, c);
+    });
+#pragma unroll
+    for (int u = 0; u < 8; ++u) top[u] = first ? tops[(u + 7) % 8].value() : tops[u].value();
+    if (!sum.into(ms, c))
+#pragma unroll 1
+        for (int k = 0; k < count; ++k) {
+            const uint4 x = own[k * kSelThreads];
+            if (ms.covers(word_max<T>(x))) ms.add_words<T, 1>(&x, c);
+            else ms.add_slow<T>(x, 0u, c);
+        }
+    edge = -INFINITY;
+    w.edges(ch.lo, ch.hi, threadIdx.x, [&](uint4 x, int) {
+        edge = word_max<T>(x);
+        ms.add_slow<T>(x, 0u, c);
     });
 }
 
@@ -350,17 +406,34 @@ __device__ int collect_top(SelShared& sh, const RowWords<T>& w, int log_P, int K
     uint32_t g[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) g[i] = sh.group[i * kSelThreads + tid] >> 16;
-    // the largest 16-bit prefix that at least K maxima reach, two bits a round
-    uint32_t t = 0u;
+    // a 16-bit prefix t that at least K maxima reach, and hardly more (an eighth, but
+    // for equal ones): their range in four a round, about four rounds of a row of
+    // like entries
+    uint32_t t = g[0], above = g[0];   // fewer than K exceed `above`
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        t = min(t, g[i]);
+        above = max(above, g[i]);
+    }
+    t = __reduce_min_sync(0xffffffffu, t);
+    above = __reduce_max_sync(0xffffffffu, above);
+    if (lane == 0) sh.warp_count[1][warp] = t << 16 | above;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSelThreads / 32; ++i) {
+        t = min(t, sh.warp_count[1][i] >> 16);
+        above = max(above, sh.warp_count[1][i] & 0xffffu);
+    }
+    int reach = kSelGroups;
 #pragma unroll 1
-    for (int s = 14; s >= 0; s -= 2) {
+    for (int round = 0; t < above && reach > K + K / 8 + 8; ++round) {
+        const uint32_t step = (above - t + 4) / 4, t1 = t + step, t2 = t1 + step, t3 = t2 + step;
         uint32_t cnt = 0u;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            cnt += (g[i] >= (t | 1u << s) ? 1u : 0u) + (g[i] >= (t | 2u << s) ? 1u << 10 : 0u) +
-                   (g[i] >= (t | 3u << s) ? 1u << 20 : 0u);
+            cnt += (g[i] >= t1 ? 1u : 0u) + (g[i] >= t2 ? 1u << 10 : 0u) + (g[i] >= t3 ? 1u << 20 : 0u);
         cnt = __reduce_add_sync(0xffffffffu, cnt);
-        uint32_t* wc = sh.warp_count[(s >> 1) & 1];
+        uint32_t* wc = sh.warp_count[round & 1];
         if (lane == 0) wc[warp] = cnt;
         __syncthreads();
         int c1 = 0, c2 = 0, c3 = 0;
@@ -371,7 +444,20 @@ __device__ int collect_top(SelShared& sh, const RowWords<T>& w, int log_P, int K
             c2 += v >> 10 & 1023u;
             c3 += v >> 20;
         }
-        t |= (c3 >= K ? 3u : c2 >= K ? 2u : c1 >= K ? 1u : 0u) << s;
+        if (c3 >= K) {
+            t = t3;
+            reach = c3;
+        } else if (c2 >= K) {
+            above = min(above, t3 - 1);
+            t = t2;
+            reach = c2;
+        } else if (c1 >= K) {
+            above = min(above, t2 - 1);
+            t = t1;
+            reach = c1;
+        } else {
+            above = t1 - 1;
+        }
     }
     if (tid == 0) sh.n_chosen = sh.n_list = 0;
     __syncthreads();
@@ -468,7 +554,8 @@ __global__ void __launch_bounds__(kSelThreads, 4) top_logits_kernel(const __grid
     const RowWords<T> w(static_cast<const T*>(a.z) + row_offset(a.d, r), a.d.V);
     float top[8], edge;
     MaxSum ms;
-    scan_chunk<T, true>(w, Chunk(w.words, p, a.log_P), a.c, top, edge, ms);
+    extern __shared__ __align__(16) uint4 slots[];
+    stream_chunk<T>(w, Chunk(w.words, p, a.log_P), a.c, slots, top, edge, ms);
     push_groups(sh, p, P, top, edge, ms, a.c);
     if (p != 0) return;
     if (tid == 0) {
@@ -1208,9 +1295,19 @@ static int log_ctas_per_row(const DwaLogitsDims& d, bool sampling) {
 }
 
 template <class K, class A>
-static cudaError_t launch_rows(K kernel, const A& a, cudaStream_t st) {
+static cudaError_t launch_rows(K kernel, size_t smem, const A& a, cudaStream_t st) {
     const dim3 grid(static_cast<unsigned>(a.d.rows * a.P));
-    return launch_pdl_cluster(kernel, grid, dim3(kSelThreads), 0, st, dim3(a.P), a);
+    return launch_pdl_cluster(kernel, grid, dim3(kSelThreads), smem, st, dim3(a.P), a);
+}
+
+template <class T>
+static int launch_top(cudaStream_t st, const TopArgs& a) {
+    constexpr size_t ring = 2 * kTopRing * kSelThreads * 16;
+    if (int rc = allow_smem<top_logits_kernel<T>>(ring)) return rc;
+    DWA_TIMED("top_logits", st, (launch_rows(top_logits_kernel<T>, ring, a, st)));
+    DWA_LAUNCH_CHECK("top_logits_kernel");
+    ++g_launches_total;
+    return DWA_OK;
 }
 
 }  // namespace dwa
@@ -1233,11 +1330,7 @@ extern "C" int dwa_top_logits(void* stream, const DwaLogitsDims* dims, const voi
     const int log_P = log_ctas_per_row(*dims, false);
     const TopArgs a = {logits, *dims, K, 1 << log_P, log_P, kLog2e / temperature, temperature, values, indices, lse};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dims->dtype == DWA_BF16) DWA_TIMED("top_logits", st, (launch_rows(top_logits_kernel<__nv_bfloat16>, a, st)));
-    else DWA_TIMED("top_logits", st, (launch_rows(top_logits_kernel<float>, a, st)));
-    DWA_LAUNCH_CHECK("top_logits_kernel");
-    ++g_launches_total;
-    return DWA_OK;
+    return dims->dtype == DWA_BF16 ? launch_top<__nv_bfloat16>(st, a) : launch_top<float>(st, a);
 }
 
 extern "C" int dwa_sample_tokens(void* stream, const DwaLogitsDims* dims, const DwaSampleParams* params,
@@ -1255,8 +1348,8 @@ extern "C" int dwa_sample_tokens(void* stream, const DwaLogitsDims* dims, const 
     const int log_P = log_ctas_per_row(*dims, true);
     const SampleArgs a = {logits, *dims, noise, noise_stride, *params, 1 << log_P, log_P, tokens, logprobs};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dims->dtype == DWA_BF16) DWA_TIMED("sample", st, (launch_rows(sample_kernel<__nv_bfloat16>, a, st)));
-    else DWA_TIMED("sample", st, (launch_rows(sample_kernel<float>, a, st)));
+    if (dims->dtype == DWA_BF16) DWA_TIMED("sample", st, (launch_rows(sample_kernel<__nv_bfloat16>, 0, a, st)));
+    else DWA_TIMED("sample", st, (launch_rows(sample_kernel<float>, 0, a, st)));
     DWA_LAUNCH_CHECK("sample_kernel");
     ++g_launches_total;
     return DWA_OK;

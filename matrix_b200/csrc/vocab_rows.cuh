@@ -330,6 +330,207 @@ struct MaxSum {
     }
 };
 
+// 16 bytes to shared memory, in the background, if `there`; with HINT L2 keeps them
+// by `policy`.
+template <bool HINT>
+__device__ __forceinline__ void copy_async_if(bool there, uint32_t to, const void* from, uint64_t policy) {
+    if constexpr (HINT)
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.b32 p, %2, 0;\n@p cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %3;\n}" ::"r"(to),
+            "l"(from), "r"(static_cast<int>(there)), "l"(policy)
+            : "memory");
+    else
+        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %2, 0;\n@p cp.async.cg.shared.global [%0], [%1], 16;\n}" ::"r"(to),
+                     "l"(from), "r"(static_cast<int>(there))
+                     : "memory");
+}
+__device__ __forceinline__ uint64_t keep_policy() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ uint64_t drop_policy() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ uint4 shared_word(uint32_t at) {
+    uint4 x;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
+    return x;
+}
+
+// A thread's `count` words of a row, NT apart, on their way through a ring of its
+// own in shared memory, in stages of two words: AHEAD of them in flight, `room`
+// kept.  The second pass goes backwards, so that it begins with what the first left
+// in the ring, and asks L2 last for what it has not seen for longest.  Only the
+// thread that copies a word reads it, so nothing but its own copies is waited for.
+// With TWICE, L2 is told to keep what the second pass has to fetch from it, and to
+// drop the rest.  The passes call two(word k, word k + 1, k) for whole stages,
+// one(word, k) for the last word of an odd count.
+template <int NT, int AHEAD, bool TWICE>
+struct WordRing {
+    static constexpr uint32_t kNext = NT * 16, kStage = 2 * kNext;
+    const uint4* const src;
+    const uint32_t base, end;   // own slots
+    const int count, room;
+    uint32_t at;                // the stage to look at
+    uint64_t policy = 0;
+
+    __device__ __forceinline__ WordRing(const uint4* slots, const uint4* src_, int count_, int room_)
+        : src(src_), base(static_cast<uint32_t>(__cvta_generic_to_shared(slots))), end(base + room_ * kStage), count(count_),
+          room(room_), at(base) {}
+    // words k and k + 1 of those below n
+    __device__ __forceinline__ void issue(uint32_t to, const uint4* from, bool first, bool second) {
+        copy_async_if<TWICE>(first, to, from, policy);
+        copy_async_if<TWICE>(second, to + kNext, from + NT, policy);
+        copy_commit();
+    }
+    __device__ __forceinline__ void begin() {
+        if (TWICE) policy = keep_policy();
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) issue(base + i * kStage, src + 2 * i * NT, 2 * i < count, 2 * i + 1 < count);
+    }
+    // the largest value of the first stage, among the warp's
+    template <class T>
+    __device__ __forceinline__ float first_max() const {
+        copy_wait<AHEAD - 1>();
+        float m = -INFINITY;
+        if (count > 1) {
+            const uint4 x[2] = {shared_word(base), shared_word(base + kNext)};
+            m = words_max<T, 2>(x);
+        } else if (count == 1) {
+            m = word_max<T>(shared_word(base));
+        }
+        return warp_max(m);
+    }
+    template <class F, class G>
+    __device__ __forceinline__ void forth(F two, G one) {
+        uint32_t to = base + AHEAD * kStage;
+        if (to == end) to = base;
+        const uint4* from = src + 2 * AHEAD * NT;
+        int left = count - 2 * AHEAD;
+        const uint64_t drop = TWICE ? drop_policy() : 0;
+        for (int k = 0; k + 1 < count; k += 2) {
+            copy_wait<AHEAD - 1>();
+            two(shared_word(at), shared_word(at + kNext), k);
+            if (TWICE && left <= 2 * room) policy = drop;   // stays in the ring
+            issue(to, from, left > 0, left > 1);
+            from += 2 * NT;
+            left -= 2;
+            at += kStage;
+            if (at == end) at = base;
+            to += kStage;
+            if (to == end) to = base;
+        }
+        copy_wait<0>();   // nothing but the last word of an odd count
+        if (count & 1) {
+            one(shared_word(at), count - 1);
+            at += kStage;
+            if (at == end) at = base;
+        }
+    }
+    // forth by eight words: two(word k, word k + 1, k mod 8), the latter a constant; an
+    // odd count ends with a word that adds nothing
+    template <class T, class F>
+    __device__ __forceinline__ void forth_by_eight(F two) {
+        uint32_t to = base + AHEAD * kStage;
+        if (to == end) to = base;
+        const uint4* from = src + 2 * AHEAD * NT;
+        int left = count - 2 * AHEAD;
+        const auto step = [&](int u, bool both) {
+            copy_wait<AHEAD - 1>();
+            two(shared_word(at), both ? shared_word(at + kNext) : RowWords<T>::nothing(), u);
+            issue(to, from, left > 0, left > 1);
+            from += 2 * NT;
+            left -= 2;
+            at += kStage;
+            if (at == end) at = base;
+            to += kStage;
+            if (to == end) to = base;
+        };
+        int k = 0;
+        for (; k + 8 <= count; k += 8) {
+#pragma unroll
+            for (int u = 0; u < 8; u += 2) step(u, true);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; u += 2)
+            if (k + u < count) step(u, k + u + 1 < count);
+    }
+    template <class F, class G>
+    __device__ __forceinline__ void back(F two, G one) {   // after forth: from the last to the first
+        int left = ((count + 1) >> 1) - room;              // stages to fetch
+        const uint4* from = src + 2 * (left - 1) * static_cast<int64_t>(NT);
+        if (TWICE) policy = drop_policy();
+        const auto step = [&](auto f) {
+            copy_wait<AHEAD - 1>();
+            if (at == base) at = end;
+            at -= kStage;
+            f();
+            issue(at, from, left > 0, left > 0);
+            from -= 2 * NT;
+            --left;
+        };
+        if (count & 1) step([&] { one(shared_word(at), count - 1); });
+        for (int k = (count & ~1) - 2; k >= 0; k -= 2) step([&] { two(shared_word(at), shared_word(at + kNext), k); });
+    }
+};
+
+// A sum with one reference throughout.  No word is looked at before it is added: a
+// sum that leaves [0, 2^60] says afterwards that the reference was too low, or that
+// a NaN or an infinity was there.
+template <class T>
+struct BlindSum {
+    Ref ref;
+    uint64_t s2 = 0;
+    __device__ __forceinline__ BlindSum(float m, float c) : ref(m, c) {}
+    // words that hold listed entries, a bit each, leave them out
+    template <int N>
+    __device__ __forceinline__ void add(const uint4 (&x)[N], uint32_t listed, float c) {
+        constexpr int VEC = kRowVec<T>;
+        uint64_t e[N][VEC / 2];
+#pragma unroll
+        for (int i = 0; i < N; ++i) word_weights<T>(x[i], ref, c, e[i]);
+        if (listed != 0u) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                float f[VEC];
+                unpair_word<T>(e[i], f);
+#pragma unroll
+                for (int v = 0; v < VEC; v += 2)
+                    e[i][v / 2] = pair((listed >> (i * VEC + v)) & 1u ? 0.f : f[v], (listed >> (i * VEC + v)) & 2u ? 0.f : f[v + 1]);
+            }
+        }
+        uint64_t sum = sum_pairs<T>(e[0]);
+        if constexpr (N == 2) sum = add2(sum, sum_pairs<T>(e[1]));
+        s2 = add2(s2, sum);
+    }
+    // as a MaxSum; false where it does not hold
+    __device__ __forceinline__ bool into(MaxSum& ms, float c) const {
+        float a, b;
+        unpair(s2, a, b);
+        const float sum = a + b;
+        if (!(ref.m > -INFINITY && ref.plain() && sum <= 1.152921504606846976e18f)) return false;
+        ms.raise(ref.m, c);
+        ms.s2 = s2;
+        if (sum > 2097152.f) ms.raise(ref.m + __log2f(sum) / c, c);
+        return true;
+    }
+};
+
+// Lets a kernel have `bytes` of dynamic shared memory, once per device and size.
+template <auto KERNEL>
+static int allow_smem(size_t bytes) {
+    static std::atomic<size_t> allowed[64];
+    int dev = 0;
+    DWA_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 64 && allowed[dev].load(std::memory_order_relaxed) >= bytes) return DWA_OK;
+    DWA_CUDA_TRY(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+    if (dev < 64) allowed[dev].store(bytes, std::memory_order_relaxed);
+    return DWA_OK;
+}
+
 int check_logits(const DwaLogitsDims* d, const char* what);   // distill.cu
 
 }  // namespace dwa
