@@ -27,7 +27,8 @@ extern std::atomic<uint64_t> g_launches_total;
 constexpr int kSelThreads = 256;
 constexpr int kSelGroups = 8 * kSelThreads;   // groups of words whose maxima are compared
 constexpr int kSelList = 2048;                // candidates held
-constexpr int kTopRing = 3;                   // stages of two words that a thread of top_logits has in flight
+constexpr int kTopRing = 2;                   // stages of two words that a thread of top_logits has in flight
+constexpr int kPairsMost = 46 * 1024;         // bytes of maxima that leave room for three CTAs an SM
 constexpr int kTryTop = 256;                  // entries sorted first when only a mass or a floor limits the row
 constexpr int kSelMaxCluster = 8;
 constexpr int kBins = 2048;                   // bins of a wide cut: 32 octaves of weight, 64 bins each, at first
@@ -150,8 +151,8 @@ struct SelShared {
         unsigned long long hist[256];
         uint32_t bin[kBins];             // a wide cut's histogram
     };
-    union {
-        unsigned long long list[kSelList];   // candidates; sorted: the K largest in descending order
+    union alignas(16) {
+        unsigned long long list[kSelList];   // first the words that stream by; candidates; sorted: the K largest in descending order
         unsigned long long sum[kBins];       // the bins so far
     };
     uint16_t chosen[kSelGroups];
@@ -183,9 +184,18 @@ struct WordTop {
             m = max_nan(m, word_max<T>(x));
         }
     }
+    __device__ __forceinline__ void add(const WordTop& o) {
+        if constexpr (sizeof(T) == 2) m = __hmax2_nan(m, o.m);
+        else m = max_nan(m, o.m);
+    }
     __device__ __forceinline__ float value() const {
         if constexpr (sizeof(T) == 2) return max_nan(__low2float(m), __high2float(m));
         else return m;
+    }
+    // the upper 16 bits
+    __device__ __forceinline__ uint16_t prefix() const {
+        if constexpr (sizeof(T) == 2) return __bfloat16_as_ushort(__hmax_nan(__low2bfloat16(m), __high2bfloat16(m)));
+        else return static_cast<uint16_t>(__float_as_uint(m) >> 16);
     }
 };
 
@@ -209,10 +219,11 @@ __device__ __forceinline__ void scan_chunk(const RowWords<T>& w, Chunk ch, float
     });
 }
 
-// The same for long chunks, whose words stream through shared memory.
+// The same, with the words streaming through shared memory; `pairs`, if any, gets the
+// (upper 16 bits of the) maxima of the thread's words two by two, kSelThreads apart.
 template <class T>
-__device__ __forceinline__ void stream_chunk(const RowWords<T>& w, Chunk ch, float c, uint4* slots, float (&top)[8],
-                                             float& edge, MaxSum& ms) {
+__device__ __forceinline__ void stream_chunk(const RowWords<T>& w, Chunk ch, float c, uint4* slots, uint16_t* pairs,
+                                             float (&top)[8], float& edge, MaxSum& ms) {
     int first, last;
     w.own_whole(ch.lo, ch.hi, threadIdx.x, kSelThreads, first, last);
     const int count = max(last - first, 0);
@@ -221,9 +232,14 @@ __device__ __forceinline__ void stream_chunk(const RowWords<T>& w, Chunk ch, flo
     ring.begin();
     WordTop<T> tops[8];
     BlindSum<T> sum(ring.template first_max<T>(), c);
-    ring.template forth_by_eight<T>([&](uint4 x, uint4 y, int u) {
-        tops[u].add(x);
-        tops[u + 1].add(y);
+    ring.template forth_by_eight<T>([&](uint4 x, uint4 y, int u, int k) {
+        WordTop<T> of_x, of_y;
+        of_x.add(x);
+        of_y.add(y);
+        tops[u].add(of_x);
+        tops[u + 1].add(of_y);
+        of_x.add(of_y);
+        if (pairs) pairs[k / 2 * kSelThreads + threadIdx.x] = of_x.prefix();
         sum.add({x, y}, 0u, c);
     });
 #pragma unroll
@@ -399,9 +415,10 @@ __device__ void sort_list(SelShared& sh, int n) {
 }
 
 // Rank 0: the K largest entries of the row, and a few more, into sh.list in any
-// order; their number.
+// order; their number.  `pairs`, if any, has the maxima of stream_chunk: of the
+// groups' words it tells which to read (P = 1).
 template <class T>
-__device__ int collect_top(SelShared& sh, const RowWords<T>& w, int log_P, int K) {
+__device__ int collect_top(SelShared& sh, const RowWords<T>& w, int log_P, int K, const uint16_t* pairs) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint32_t g[8];
 #pragma unroll
@@ -494,7 +511,12 @@ __device__ int collect_top(SelShared& sh, const RowWords<T>& w, int log_P, int K
                 const int q = sh.chosen[i >> log_rounds], r = q / kSelThreads;
                 const Chunk ch(w.words, r >> log_per, log_P);
                 const int word = ch.lo + q % kSelThreads + ((r & ((1 << log_per) - 1)) + (k << log_per)) * kSelThreads;
-                if (word < ch.hi && w.whole(word)) {
+                bool look = word < ch.hi && w.whole(word);
+                if (pairs && look) {
+                    const int x = q % kSelThreads, own = (r & 7) + 8 * k - (x == 0 ? w.full_lo : 0);
+                    look = ordered(__uint_as_float(pairs[(own >> 1) * kSelThreads + x] << 16)) >> 16 >= t;
+                }
+                if (look) {
                     at[u] = word;
                     x[u] = w.word(word);
                 }
@@ -529,8 +551,9 @@ __device__ int collect_top(SelShared& sh, const RowWords<T>& w, int log_P, int K
 
 // Rank 0: the K largest entries of the row into sh.list, in descending order.
 template <class T>
-__device__ __forceinline__ void sort_top(SelShared& sh, const RowWords<T>& w, int log_P, int K) {
-    sort_list(sh, collect_top(sh, w, log_P, K));
+__device__ __forceinline__ void sort_top(SelShared& sh, const RowWords<T>& w, int log_P, int K,
+                                         const uint16_t* pairs = nullptr) {
+    sort_list(sh, collect_top(sh, w, log_P, K, pairs));
 }
 
 struct TopArgs {
@@ -541,6 +564,7 @@ struct TopArgs {
     void* values;
     int32_t* indices;
     float* lse;
+    bool pairs;
 };
 
 template <class T>
@@ -554,8 +578,9 @@ __global__ void __launch_bounds__(kSelThreads, 4) top_logits_kernel(const __grid
     const RowWords<T> w(static_cast<const T*>(a.z) + row_offset(a.d, r), a.d.V);
     float top[8], edge;
     MaxSum ms;
-    extern __shared__ __align__(16) uint4 slots[];
-    stream_chunk<T>(w, Chunk(w.words, p, a.log_P), a.c, slots, top, edge, ms);
+    extern __shared__ __align__(16) uint16_t maxima[];
+    uint16_t* const pairs = a.pairs ? maxima : nullptr;
+    stream_chunk<T>(w, Chunk(w.words, p, a.log_P), a.c, reinterpret_cast<uint4*>(sh.list), pairs, top, edge, ms);
     push_groups(sh, p, P, top, edge, ms, a.c);
     if (p != 0) return;
     if (tid == 0) {
@@ -563,7 +588,7 @@ __global__ void __launch_bounds__(kSelThreads, 4) top_logits_kernel(const __grid
         row_stats(sh, P, a.c, m, s);
         a.lse[r] = m != m || isinf(m) ? m : static_cast<float>(0.6931471805599453 * (Ref(m, a.c).a(a.c) + log2f(s)));
     }
-    sort_top(sh, w, a.log_P, a.K);
+    sort_top(sh, w, a.log_P, a.K, pairs);
     for (int k = tid; k < a.K; k += kSelThreads) {
         const unsigned long long key = sh.list[k];
         static_cast<T*>(a.values)[static_cast<int64_t>(r) * a.K + k] = Elem<T>::from_f(unordered(static_cast<uint32_t>(key >> 32)));
@@ -1255,7 +1280,7 @@ __global__ void __launch_bounds__(kSelThreads, 4) sample_kernel(const __grid_con
                 const double total = masses ? s * exp2(Ref(m, c).a(c) - static_cast<double>(m) * c) : 0.;
                 const double limit = masses ? q.top_p * total : INFINITY;
                 if (limit <= kTryTop || q.min_p > 0.f) {   // else more than kTryTop of the largest weight
-                    const int n = collect_top(sh, w, a.log_P, kTryTop);
+                    const int n = collect_top(sh, w, a.log_P, kTryTop, nullptr);
                     if (may_hold_all(sh, n, q, m, limit)) {
                         sort_list(sh, n);
                         done = sample_listed(sh, a, w, r, q, noise, m, kTryTop, total, false);
@@ -1301,10 +1326,14 @@ static cudaError_t launch_rows(K kernel, size_t smem, const A& a, cudaStream_t s
 }
 
 template <class T>
-static int launch_top(cudaStream_t st, const TopArgs& a) {
-    constexpr size_t ring = 2 * kTopRing * kSelThreads * 16;
-    if (int rc = allow_smem<top_logits_kernel<T>>(ring)) return rc;
-    DWA_TIMED("top_logits", st, (launch_rows(top_logits_kernel<T>, ring, a, st)));
+static int launch_top(cudaStream_t st, TopArgs a) {
+    static_assert(2 * kTopRing * kSelThreads * 16 <= sizeof(SelShared::list), "the ring lies where the list will");
+    const int words = (a.d.V + 2 * kRowVec<T> - 2) / kRowVec<T> / a.P + 1;
+    size_t pairs = static_cast<size_t>((words + 2 * kSelThreads - 1) / (2 * kSelThreads)) * kSelThreads * 2;
+    a.pairs = a.P == 1 && pairs <= kPairsMost;
+    if (!a.pairs) pairs = 0;
+    if (int rc = allow_smem<top_logits_kernel<T>>(pairs)) return rc;
+    DWA_TIMED("top_logits", st, (launch_rows(top_logits_kernel<T>, pairs, a, st)));
     DWA_LAUNCH_CHECK("top_logits_kernel");
     ++g_launches_total;
     return DWA_OK;
@@ -1328,7 +1357,7 @@ extern "C" int dwa_top_logits(void* stream, const DwaLogitsDims* dims, const voi
         reinterpret_cast<uintptr_t>(values) % dtype_bytes(dims->dtype))
         return fail(DWA_ERR_INVALID_ARG, "top_logits: a pointer is not aligned to its element");
     const int log_P = log_ctas_per_row(*dims, false);
-    const TopArgs a = {logits, *dims, K, 1 << log_P, log_P, kLog2e / temperature, temperature, values, indices, lse};
+    const TopArgs a = {logits, *dims, K, 1 << log_P, log_P, kLog2e / temperature, temperature, values, indices, lse, false};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return dims->dtype == DWA_BF16 ? launch_top<__nv_bfloat16>(st, a) : launch_top<float>(st, a);
 }

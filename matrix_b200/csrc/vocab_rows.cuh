@@ -430,7 +430,7 @@ struct WordRing {
             if (at == end) at = base;
         }
     }
-    // forth by eight words: two(word k, word k + 1, k mod 8), the latter a constant; an
+    // forth by eight words: two(word k, word k + 1, k mod 8, k), k mod 8 a constant; an
     // odd count ends with a word that adds nothing
     template <class T, class F>
     __device__ __forceinline__ void forth_by_eight(F two) {
@@ -438,9 +438,9 @@ struct WordRing {
         if (to == end) to = base;
         const uint4* from = src + 2 * AHEAD * NT;
         int left = count - 2 * AHEAD;
-        const auto step = [&](int u, bool both) {
+        const auto step = [&](int k, int u, bool both) {
             copy_wait<AHEAD - 1>();
-            two(shared_word(at), both ? shared_word(at + kNext) : RowWords<T>::nothing(), u);
+            two(shared_word(at), both ? shared_word(at + kNext) : RowWords<T>::nothing(), u, k);
             issue(to, from, left > 0, left > 1);
             from += 2 * NT;
             left -= 2;
@@ -452,11 +452,11 @@ struct WordRing {
         int k = 0;
         for (; k + 8 <= count; k += 8) {
 #pragma unroll
-            for (int u = 0; u < 8; u += 2) step(u, true);
+            for (int u = 0; u < 8; u += 2) step(k + u, u, true);
         }
 #pragma unroll
         for (int u = 0; u < 8; u += 2)
-            if (k + u < count) step(u, k + u + 1 < count);
+            if (k + u < count) step(k + u, u, k + u + 1 < count);
     }
     template <class F, class G>
     __device__ __forceinline__ void back(F two, G one) {   // after forth: from the last to the first
