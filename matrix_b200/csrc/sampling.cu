@@ -369,17 +369,18 @@ __device__ void sort_list(SelShared& sh, int n) {
         __syncthreads();
         if (tid < n) sh.list[rank] = key;
     } else if (n <= 2 * kSelThreads) {   // 64 a warp, then each behind the larger keys of the other warps
-        const int base = 64 * warp;
+        const int base = 64 * warp, runs = (n + 63) / 64;
         unsigned long long key[2] = {base + lane < n ? sh.list[base + lane] : 0ull,
                                      base + lane + 32 < n ? sh.list[base + lane + 32] : 0ull};
-        sort_warp(key[0], key[1]);
-        sh.list[base + lane] = key[0];
-        sh.list[base + lane + 32] = key[1];
+        if (warp < runs) {
+            sort_warp(key[0], key[1]);
+            sh.list[base + lane] = key[0];
+            sh.list[base + lane + 32] = key[1];
+        }
         __syncthreads();
         int at[2] = {lane, lane + 32};
-        const int runs = (n + 63) / 64;
         for (int r = 0; r < runs; ++r) {
-            if (r == warp) continue;
+            if (r == warp || warp >= runs) continue;
             const unsigned long long* run = sh.list + 64 * r;
             int c[2] = {0, 0};
 #pragma unroll
@@ -414,6 +415,52 @@ __device__ void sort_list(SelShared& sh, int n) {
     __syncthreads();
 }
 
+// A 16-bit number that at least K of `all` reach, eight a lane, and, but for equal
+// ones, hardly more than 9/8 K: their range in four a round, about four rounds for
+// the maxima of a row of like entries.  share(v, round, f) calls f with every warp's v.
+template <class F>
+__device__ __forceinline__ uint32_t reached(const uint32_t (&g)[8], int K, int all, F share) {
+    uint32_t t = g[0], above = g[0];   // K or more reach t, fewer exceed `above`
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        t = min(t, g[i]);
+        above = max(above, g[i]);
+    }
+    share(__reduce_min_sync(0xffffffffu, t) << 16 | __reduce_max_sync(0xffffffffu, above), 1, [&](uint32_t v) {
+        t = min(t, v >> 16);
+        above = max(above, v & 0xffffu);
+    });
+#pragma unroll 1
+    for (int round = 0; t < above && all > K + K / 8 + 8; ++round) {
+        const uint32_t step = (above - t + 4) / 4, t1 = t + step, t2 = t1 + step, t3 = t2 + step;
+        uint32_t cnt = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            cnt += (g[i] >= t1 ? 1u : 0u) + (g[i] >= t2 ? 1u << 10 : 0u) + (g[i] >= t3 ? 1u << 20 : 0u);
+        int c1 = 0, c2 = 0, c3 = 0;
+        share(__reduce_add_sync(0xffffffffu, cnt), round, [&](uint32_t v) {
+            c1 += v & 1023u;
+            c2 += v >> 10 & 1023u;
+            c3 += v >> 20;
+        });
+        if (c3 >= K) {
+            t = t3;
+            all = c3;
+        } else if (c2 >= K) {
+            above = min(above, t3 - 1);
+            t = t2;
+            all = c2;
+        } else if (c1 >= K) {
+            above = min(above, t2 - 1);
+            t = t1;
+            all = c1;
+        } else {
+            above = t1 - 1;
+        }
+    }
+    return t;
+}
+
 // Rank 0: the K largest entries of the row, and a few more, into sh.list in any
 // order; their number.  `pairs`, if any, has the maxima of stream_chunk: of the
 // groups' words it tells which to read (P = 1).
@@ -423,61 +470,37 @@ __device__ int collect_top(SelShared& sh, const RowWords<T>& w, int log_P, int K
     uint32_t g[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) g[i] = sh.group[i * kSelThreads + tid] >> 16;
-    // a 16-bit prefix t that at least K maxima reach, and hardly more (an eighth, but
-    // for equal ones): their range in four a round, about four rounds of a row of
-    // like entries
-    uint32_t t = g[0], above = g[0];   // fewer than K exceed `above`
+    // a 16-bit prefix that at least K maxima reach, and hardly more.  Up to half as many
+    // as there are threads: of the threads' maxima, by one warp without a barrier (of
+    // these, K mean at most 1.4 K of the entries of a row in random order)
+    uint32_t t;
+    if (K <= kSelThreads / 2) {
+        uint32_t most = g[0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) {
-        t = min(t, g[i]);
-        above = max(above, g[i]);
-    }
-    t = __reduce_min_sync(0xffffffffu, t);
-    above = __reduce_max_sync(0xffffffffu, above);
-    if (lane == 0) sh.warp_count[1][warp] = t << 16 | above;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kSelThreads / 32; ++i) {
-        t = min(t, sh.warp_count[1][i] >> 16);
-        above = max(above, sh.warp_count[1][i] & 0xffffu);
-    }
-    int reach = kSelGroups;
-#pragma unroll 1
-    for (int round = 0; t < above && reach > K + K / 8 + 8; ++round) {
-        const uint32_t step = (above - t + 4) / 4, t1 = t + step, t2 = t1 + step, t3 = t2 + step;
-        uint32_t cnt = 0u;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            cnt += (g[i] >= t1 ? 1u : 0u) + (g[i] >= t2 ? 1u << 10 : 0u) + (g[i] >= t3 ? 1u << 20 : 0u);
-        cnt = __reduce_add_sync(0xffffffffu, cnt);
-        uint32_t* wc = sh.warp_count[round & 1];
-        if (lane == 0) wc[warp] = cnt;
+        for (int i = 1; i < 8; ++i) most = max(most, g[i]);
+        sh.chosen[tid] = static_cast<uint16_t>(most);
         __syncthreads();
-        int c1 = 0, c2 = 0, c3 = 0;
+        if (warp == 0) {
+            uint32_t q[8];
 #pragma unroll
-        for (int i = 0; i < kSelThreads / 32; ++i) {
-            const uint32_t v = wc[i];
-            c1 += v & 1023u;
-            c2 += v >> 10 & 1023u;
-            c3 += v >> 20;
+            for (int i = 0; i < 8; ++i) q[i] = sh.chosen[32 * i + lane];
+            t = reached(q, K, kSelThreads, [](uint32_t v, int, auto f) { f(v); });
+            if (lane == 0) sh.warp_count[0][0] = t;
         }
-        if (c3 >= K) {
-            t = t3;
-            reach = c3;
-        } else if (c2 >= K) {
-            above = min(above, t3 - 1);
-            t = t2;
-            reach = c2;
-        } else if (c1 >= K) {
-            above = min(above, t2 - 1);
-            t = t1;
-            reach = c1;
-        } else {
-            above = t1 - 1;
-        }
+        if (tid == 0) sh.n_chosen = sh.n_list = 0;
+        __syncthreads();
+        t = sh.warp_count[0][0];
+    } else {
+        t = reached(g, K, kSelGroups, [&](uint32_t v, int round, auto f) {
+            uint32_t* wc = sh.warp_count[round & 1];
+            if (lane == 0) wc[warp] = v;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kSelThreads / 32; ++i) f(wc[i]);
+        });
+        if (tid == 0) sh.n_chosen = sh.n_list = 0;
+        __syncthreads();
     }
-    if (tid == 0) sh.n_chosen = sh.n_list = 0;
-    __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         if (g[i] >= t) sh.chosen[atomicAdd(&sh.n_chosen, 1)] = static_cast<uint16_t>(i * kSelThreads + tid);
