@@ -629,7 +629,7 @@ DWA_API int dwa_top_logits(void* stream, const DwaLogitsDims* dims, const void* 
 typedef struct DwaDistillDims {
     int32_t K;
     int32_t teacher_dtype;   /* DWA_F32 or DWA_BF16 */
-    float   temperature;     /* T > 0 */
+    float   temperature;     /* in [1e-30, 1e30] */
     int32_t reverse;
 } DwaDistillDims;
 

@@ -30,8 +30,8 @@
 // the loss 159 us (6.8 TB/s), with the gradient 375 us (5.7 TB/s of the 2.1 GB that
 // it has to move, and 9% more reads than that; 407 us without hints to L2, 457 us
 // with both passes forwards; 541 us as two kernels, the loss and its backward, of
-// which the backward runs at 6.5 TB/s); 600 us when clusters of four hold each row, because the CTAs of a
-// cluster wait for the slowest.
+// which the backward runs at 6.5 TB/s); 600 us when clusters of four hold each row,
+// because the CTAs of a cluster wait for the slowest.
 
 #include <atomic>
 
